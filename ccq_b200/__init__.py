@@ -14,6 +14,8 @@ from .ops import (  # noqa: F401
     reduce_lambda_grad,
     reshape_lambda_3d,
 )
+from .delta_rule import GatedDeltaRule, gated_delta_rule, gated_delta_step  # noqa: F401
+from .norm import LayerNorm, gated_rms_norm, layer_norm, rms_norm  # noqa: F401
 from ._lib import CCQError, last_launch_count, last_path  # noqa: F401
 
 __version__ = '0.1.0'

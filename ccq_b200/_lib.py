@@ -21,12 +21,19 @@ PATHS = {0: 'none', 1: 'simt', 2: 'tcgen05', 3: 'decode'}
 EXPORTS = ('ccq_last_error', 'ccq_last_path', 'ccq_version', 'ccq_last_launch_count',
            'ccq_workspace_size', 'ccq_workspace_size_for', 'ccq_device_status', 'ccq_clean_fwd', 'ccq_clean_bwd',
            'ccq_decode_step', 'ccq_clean_bwd_noalloc', 'ccq_noalloc_status', 'ccq_clean_l2norm_fwd',
-           'ccq_clean_l2norm_bwd', 'ccq_decode_step_l2norm')
+           'ccq_clean_l2norm_bwd', 'ccq_decode_step_l2norm', 'ccq_gdr_workspace_size', 'ccq_gdr_fwd', 'ccq_gdr_bwd',
+           'ccq_gdr_step', 'ccq_layer_norm_workspace_size', 'ccq_layer_norm_fwd', 'ccq_layer_norm_bwd')
 CCQ_WS_HAVE_FWD_OUTPUTS, CCQ_WS_L2NORM = 1, 2
+CCQ_NORM_LAYER, CCQ_NORM_RMS = 0, 1
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
+_L = ctypes.c_int64
+_F = ctypes.c_float
+# what the three gated-delta-rule entry points share: dtype, B, T, H, HV, K, V; q, k, v; g, beta; scale;
+# cu_seqlens, n_seqs, initial state
+_GDR = [_I] * 7 + [_P] * 3 + [_I, _P, _I, _P, _F, _P, _I, _P]
 
 _SIGS = {
     'ccq_last_error': (ctypes.c_char_p, []),
@@ -50,6 +57,13 @@ _SIGS = {
                                   _P, _P, _P, _P, _SZ, _P]),
     'ccq_clean_l2norm_bwd': (_I, [_I, _I, _I, _I, _I, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P,
                                   _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    'ccq_gdr_workspace_size': (_SZ, [_I] * 10),
+    'ccq_gdr_fwd': (_I, _GDR + [_P, _P, _P, _SZ, _P]),
+    'ccq_gdr_bwd': (_I, _GDR + [_P] * 8 + [_P, _SZ, _P]),
+    'ccq_gdr_step': (_I, _GDR + [_P, _P, _P]),
+    'ccq_layer_norm_workspace_size': (_SZ, [_I, _L, _I]),
+    'ccq_layer_norm_fwd': (_I, [_I, _I, _L, _I, _F] + [_P] * 9),
+    'ccq_layer_norm_bwd': (_I, [_I, _I, _L, _I] + [_P] * 12 + [_P, _SZ, _P]),
 }
 
 _lib = None

@@ -83,6 +83,35 @@ cudaError_t l2norm_rows_scale(int dtype, const void* x, void* y, const float* r_
 cudaError_t l2norm_rows_bwd(int dtype, void* d, const void* d_ext, const void* y, const float* r_in, int slot,
                             int64_t rows, int K, cudaStream_t st);
 
+// Layer norm (layer_norm.cu): rows of D elements, D <= LN_MAX_D
+enum { LN_LAYER = 0, LN_RMS = 1 };
+constexpr int LN_MAX_D = 16384;
+struct LayerNormArgs {
+  int dtype, form, D;
+  int64_t rows;
+  float eps;
+  const void* x;         // [rows, D]
+  const void* residual;  // added to x first, or nullptr
+  const float* weight;   // [D] or nullptr
+  const float* bias;     // [D] or nullptr
+  const void* gate;      // [rows, D] or nullptr: y *= gate sigmoid(gate)
+  void* y;
+  void* h;               // x + residual, written when residual is given
+  float2* stats;         // [rows] mean, 1 / sqrt(var + eps): written by the forward, read by the backward
+  // backward
+  const void* dy;
+  const void* dh;        // gradient arriving on h, or nullptr
+  void* dx;              // also the gradient of residual
+  void* dgate;
+  float* dweight;        // or nullptr
+  float* dbias;          // or nullptr
+  float* partial;        // workspace
+  cudaStream_t stream;
+};
+size_t layer_norm_bwd_workspace(int64_t rows, int D);
+cudaError_t layer_norm_fwd(const LayerNormArgs& a, int* launches);
+cudaError_t layer_norm_bwd(const LayerNormArgs& a, int* launches);
+
 // decode step (K % 4 == 0, K <= 256)
 cudaError_t decode_step(const CleanArgs& a, int* launches);
 

@@ -7,6 +7,7 @@
 
 #include "../../include/ccq_b200.h"
 #include "args.h"
+#include "gdr.h"
 
 namespace {
 
@@ -461,3 +462,230 @@ extern "C" int ccq_clean_bwd_noalloc(int dtype, int B, int T, int H, int K, cons
   return st;
 }
 
+
+// ------------------------------------------------------------------------------------------------
+// Gated delta rule and layer norm
+// ------------------------------------------------------------------------------------------------
+namespace {
+
+bool known_dtype(int dt) { return dt == CCQ_F32 || dt == CCQ_BF16 || dt == CCQ_F16; }
+
+// Checks what the three gated-delta-rule entry points share and fills the argument bundle.
+int gdr_args(ccq::GdrArgs* out, int dtype, int B, int T, int H, int HV, int K, int V, const void* q, const void* k,
+             const void* v, int g_dtype, const void* g, int beta_dtype, const void* beta, float scale,
+             const int64_t* cu, int n_seqs, const float* initial_state, void* workspace, size_t workspace_bytes,
+             void* stream) {
+  if (!known_dtype(dtype)) return fail(CCQ_ERR_INVALID, "unknown dtype %d", dtype);
+  if (!known_dtype(g_dtype) || !known_dtype(beta_dtype))
+    return fail(CCQ_ERR_INVALID, "unknown gate dtypes %d, %d", g_dtype, beta_dtype);
+  if (B < 1 || T < 0 || H < 1 || HV < 1 || K < 1 || V < 1)
+    return fail(CCQ_ERR_INVALID, "bad sizes B=%d T=%d H=%d HV=%d K=%d V=%d", B, T, H, HV, K, V);
+  if (HV % H != 0) return fail(CCQ_ERR_INVALID, "HV=%d must be a multiple of H=%d", HV, H);
+  if (K > 256) return fail(CCQ_ERR_UNSUPPORTED, "key size K=%d > 256 is not supported", K);
+  if (V > 65536) return fail(CCQ_ERR_UNSUPPORTED, "value size V=%d > 65536 is not supported", V);
+  if (HV > 65535) return fail(CCQ_ERR_UNSUPPORTED, "HV=%d > 65535 is not supported", HV);
+  if (T > 0 && (q == nullptr || k == nullptr || v == nullptr || g == nullptr || beta == nullptr))
+    return fail(CCQ_ERR_INVALID, "q, k, v, g and beta are required");
+  if (cu == nullptr) {
+    if (n_seqs != B) return fail(CCQ_ERR_INVALID, "dense batch: n_seqs (%d) must equal B (%d)", n_seqs, B);
+  } else {
+    if (B != 1) return fail(CCQ_ERR_INVALID, "varlen batch (cu_seqlens given) needs B == 1, got %d", B);
+    if (n_seqs < 1) return fail(CCQ_ERR_INVALID, "varlen batch needs n_seqs >= 1");
+  }
+  if (n_seqs > 65535) return fail(CCQ_ERR_UNSUPPORTED, "n_seqs=%d > 65535", n_seqs);
+  if ((int64_t)n_seqs * HV > 0x7FFFFFFF) return fail(CCQ_ERR_UNSUPPORTED, "n_seqs * HV is too large");
+  if ((int64_t)B * T > 0x7FFFFFFF) return fail(CCQ_ERR_UNSUPPORTED, "B * T is too large");
+  ccq::GdrArgs a;
+  memset(&a, 0, sizeof(a));
+  a.dtype = dtype; a.B = B; a.T = T; a.H = H; a.HV = HV; a.K = K; a.V = V; a.n_seqs = n_seqs;
+  a.q = q; a.k = k; a.v = v;
+  a.g_dtype = g_dtype; a.g = g; a.beta_dtype = beta_dtype; a.beta = beta;
+  a.scale = scale;
+  a.cu_seqlens = cu;
+  a.initial_state = initial_state;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  a.stream = (cudaStream_t)stream;
+  *out = a;
+  return CCQ_OK;
+}
+
+int need_workspace(const char* who, size_t need, const void* ws, size_t got) {
+  if (need > 0 && (ws == nullptr || got < need))
+    return fail(CCQ_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, got);
+  return CCQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t ccq_gdr_workspace_size(int op, int dtype, int B, int T, int H, int HV, int K, int V, int n_seqs, int varlen) {
+  if (B < 1 || T < 0 || H < 1 || HV < 1 || K < 1 || K > 256 || V < 1 || n_seqs < 1) return 0;
+  ccq::GdrArgs a;
+  memset(&a, 0, sizeof(a));
+  a.dtype = dtype; a.B = B; a.T = T; a.H = H; a.HV = HV; a.K = K; a.V = V; a.n_seqs = n_seqs;
+  static const int64_t some_offsets = 0;
+  a.cu_seqlens = varlen ? &some_offsets : nullptr;  // only whether it is given counts
+  return ccq::gdr_simt_workspace(a, op == CCQ_OP_BWD);
+}
+
+int ccq_gdr_fwd(int dtype, int B, int T, int H, int HV, int K, int V, const void* q, const void* k, const void* v,
+                int g_dtype, const void* g, int beta_dtype, const void* beta, float scale, const int64_t* cu_seqlens,
+                int n_seqs, const float* initial_state, void* o, float* final_state, void* workspace,
+                size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  ccq::GdrArgs a;
+  int st = gdr_args(&a, dtype, B, T, H, HV, K, V, q, k, v, g_dtype, g, beta_dtype, beta, scale, cu_seqlens, n_seqs,
+                    initial_state, workspace, workspace_bytes, stream);
+  if (st != CCQ_OK) return st;
+  if (T > 0 && o == nullptr) return fail(CCQ_ERR_INVALID, "the output o is required");
+  a.o = o;
+  a.final_state = final_state;
+  st = need_workspace("ccq_gdr_fwd", ccq::gdr_simt_workspace(a, false), workspace, workspace_bytes);
+  if (st != CCQ_OK) return st;
+  int launches = 0;
+  cudaError_t e = ccq::gdr_simt_fwd(a, &launches);
+  if (e != cudaSuccess) return cuda_fail(e, "ccq_gdr_fwd launch");
+  g_path = CCQ_PATH_SIMT;
+  g_launches = launches;
+  return CCQ_OK;
+}
+
+int ccq_gdr_bwd(int dtype, int B, int T, int H, int HV, int K, int V, const void* q, const void* k, const void* v,
+                int g_dtype, const void* g, int beta_dtype, const void* beta, float scale, const int64_t* cu_seqlens,
+                int n_seqs, const float* initial_state, const void* d_o, const float* dfinal_state, void* dq, void* dk,
+                void* dv, void* dg, void* dbeta, float* dinitial_state, void* workspace, size_t workspace_bytes,
+                void* stream) {
+  g_err[0] = 0;
+  ccq::GdrArgs a;
+  int st = gdr_args(&a, dtype, B, T, H, HV, K, V, q, k, v, g_dtype, g, beta_dtype, beta, scale, cu_seqlens, n_seqs,
+                    initial_state, workspace, workspace_bytes, stream);
+  if (st != CCQ_OK) return st;
+  if (T > 0 && (d_o == nullptr || dq == nullptr || dk == nullptr || dv == nullptr || dg == nullptr || dbeta == nullptr))
+    return fail(CCQ_ERR_INVALID, "d_o, dq, dk, dv, dg and dbeta are required");
+  a.d_o = d_o;
+  a.dfinal_state = dfinal_state;
+  a.dq = dq; a.dk = dk; a.dv = dv; a.dg = dg; a.dbeta = dbeta;
+  a.dinitial_state = dinitial_state;
+  st = need_workspace("ccq_gdr_bwd", ccq::gdr_simt_workspace(a, true), workspace, workspace_bytes);
+  if (st != CCQ_OK) return st;
+  int launches = 0;
+  cudaError_t e = ccq::gdr_simt_bwd(a, &launches);
+  if (e != cudaSuccess) return cuda_fail(e, "ccq_gdr_bwd launch");
+  g_path = CCQ_PATH_SIMT;
+  g_launches = launches;
+  return CCQ_OK;
+}
+
+int ccq_gdr_step(int dtype, int B, int T, int H, int HV, int K, int V, const void* q, const void* k, const void* v,
+                 int g_dtype, const void* g, int beta_dtype, const void* beta, float scale, const int64_t* cu_seqlens,
+                 int n_seqs, const float* state_in, float* state_out, void* o, void* stream) {
+  g_err[0] = 0;
+  ccq::GdrArgs a;
+  int st = gdr_args(&a, dtype, B, T, H, HV, K, V, q, k, v, g_dtype, g, beta_dtype, beta, scale, cu_seqlens, n_seqs,
+                    state_in, nullptr, 0, stream);
+  if (st != CCQ_OK) return st;
+  if (state_out == nullptr) return fail(CCQ_ERR_INVALID, "state_out is required");
+  if (T > 0 && o == nullptr) return fail(CCQ_ERR_INVALID, "the output o is required");
+  a.final_state = state_out;
+  a.o = o;
+  int launches = 0;
+  cudaError_t e = ccq::gdr_step(a, &launches);
+  if (e != cudaSuccess) return cuda_fail(e, "ccq_gdr_step launch");
+  g_path = CCQ_PATH_DECODE;
+  g_launches = launches;
+  return CCQ_OK;
+}
+
+size_t ccq_layer_norm_workspace_size(int op, int64_t rows, int D) {
+  if (op != CCQ_OP_BWD || rows < 0 || D < 1 || D > ccq::LN_MAX_D) return 0;
+  return ccq::layer_norm_bwd_workspace(rows, D);
+}
+
+}  // extern "C"
+
+namespace {
+
+int ln_args(ccq::LayerNormArgs* out, int dtype, int form, int64_t rows, int D, float eps, const void* x,
+            const void* residual, const float* weight, const float* bias, const void* gate, void* stream) {
+  if (!known_dtype(dtype)) return fail(CCQ_ERR_INVALID, "unknown dtype %d", dtype);
+  if (form != CCQ_NORM_LAYER && form != CCQ_NORM_RMS) return fail(CCQ_ERR_INVALID, "unknown norm form %d", form);
+  if (rows < 0 || D < 1) return fail(CCQ_ERR_INVALID, "bad sizes rows=%lld D=%d", (long long)rows, D);
+  if (D > ccq::LN_MAX_D) return fail(CCQ_ERR_UNSUPPORTED, "row size D=%d > %d is not supported", D, ccq::LN_MAX_D);
+  if (rows > 0x7FFFFFFF) return fail(CCQ_ERR_UNSUPPORTED, "rows=%lld is too large", (long long)rows);
+  if (!(eps >= 0.f)) return fail(CCQ_ERR_INVALID, "eps must not be negative");
+  if (rows > 0 && x == nullptr) return fail(CCQ_ERR_INVALID, "x is required");
+  ccq::LayerNormArgs a;
+  memset(&a, 0, sizeof(a));
+  a.dtype = dtype;
+  a.form = form;
+  a.rows = rows;
+  a.D = D;
+  a.eps = eps;
+  a.x = x;
+  a.residual = residual;
+  a.weight = weight;
+  a.bias = bias;
+  a.gate = gate;
+  a.stream = (cudaStream_t)stream;
+  *out = a;
+  return CCQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ccq_layer_norm_fwd(int dtype, int form, int64_t rows, int D, float eps, const void* x, const void* residual,
+                       const float* weight, const float* bias, const void* gate, void* y, void* h, float* stats,
+                       void* stream) {
+  g_err[0] = 0;
+  ccq::LayerNormArgs a;
+  int st = ln_args(&a, dtype, form, rows, D, eps, x, residual, weight, bias, gate, stream);
+  if (st != CCQ_OK) return st;
+  if (rows > 0 && y == nullptr) return fail(CCQ_ERR_INVALID, "the output y is required");
+  if (rows > 0 && residual != nullptr && h == nullptr) return fail(CCQ_ERR_INVALID, "h is required with residual");
+  if ((uintptr_t)stats & 7) return fail(CCQ_ERR_INVALID, "stats must be 8-byte aligned");
+  a.y = y;
+  a.h = h;
+  a.stats = reinterpret_cast<float2*>(stats);
+  int launches = 0;
+  cudaError_t e = ccq::layer_norm_fwd(a, &launches);
+  if (e != cudaSuccess) return cuda_fail(e, "ccq_layer_norm_fwd launch");
+  g_path = CCQ_PATH_SIMT;
+  g_launches = launches;
+  return CCQ_OK;
+}
+
+int ccq_layer_norm_bwd(int dtype, int form, int64_t rows, int D, const void* x, const void* residual,
+                       const float* weight, const float* bias, const void* gate, const float* stats, const void* dy,
+                       const void* dh, void* dx, void* dgate, float* dweight, float* dbias, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  g_err[0] = 0;
+  ccq::LayerNormArgs a;
+  int st = ln_args(&a, dtype, form, rows, D, 0.f, x, residual, weight, bias, gate, stream);
+  if (st != CCQ_OK) return st;
+  if (rows > 0 && (stats == nullptr || dy == nullptr || dx == nullptr))
+    return fail(CCQ_ERR_INVALID, "stats, dy and dx are required");
+  if (rows > 0 && gate != nullptr && dgate == nullptr) return fail(CCQ_ERR_INVALID, "dgate is required with gate");
+  if ((uintptr_t)stats & 7) return fail(CCQ_ERR_INVALID, "stats must be 8-byte aligned");
+  a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
+  a.dy = dy;
+  a.dh = dh;
+  a.dx = dx;
+  a.dgate = dgate;
+  a.dweight = dweight;
+  a.dbias = dbias;
+  a.partial = reinterpret_cast<float*>(workspace);
+  st = need_workspace("ccq_layer_norm_bwd", ccq::layer_norm_bwd_workspace(rows, D), workspace, workspace_bytes);
+  if (st != CCQ_OK) return st;
+  int launches = 0;
+  cudaError_t e = ccq::layer_norm_bwd(a, &launches);
+  if (e != cudaSuccess) return cuda_fail(e, "ccq_layer_norm_bwd launch");
+  g_path = CCQ_PATH_SIMT;
+  g_launches = launches;
+  return CCQ_OK;
+}
+
+}  // extern "C"

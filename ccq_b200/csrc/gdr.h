@@ -1,0 +1,116 @@
+// Gated delta rule: argument bundle and the pieces its kernels share.
+//
+//   S <- e^{g_t} S;  u_t = beta_t (v_t - S^T k_t);  S <- S + k_t u_t^T;  o_t = scale S^T q_t
+//
+// per (document, value head), S [K, V] fp32.  A key head serves HV / H value heads.  In chunks of C
+// tokens (rows of Q, K, V), with G the running sum of g inside the chunk, Gam = e^G, w = e^{G_C - G},
+// D_ij = e^{G_i - G_j} (j <= i) and S0 the state before the chunk:
+//
+//   R = beta (V - Gam K S0)      T = (1 + strict(beta_i D_ij k_i.k_j))^{-1}      U = T R
+//   O = scale Gam Q S0 + P U     P = scale tril(D_ij q_i.k_j)                    S1 = Gam_C S0 + K^T (w U)
+//
+// and backwards, from dO and dS1:
+//
+//   dU = P^T dO + w K dS1    dR = T^T dU    dV = beta dR
+//   dS0 = Gam_C dS1 + (scale Gam Q)^T dO - (beta Gam K)^T dR
+//   dQ = scale Gam dO S0^T + W K,                 W = scale tril(D dO U^T)
+//   dK = -beta Gam dR S0^T + W^T Q + (N + N^T) K + w U dS1^T,   N = -strict(beta_i D_ij dR_i.U_j)
+//   dbeta_i = dR_i . (V - Gam K S0)_i - sum_j D_ij (k_i.k_j) (dR_i . U_j),  j < i
+//   dg_t = <dS1, S1> + sum_{i >= t} (dO_i . O_i - V_i . dV_i)      (i inside the chunk)
+//
+// The last line is what collecting every e^G gives: the terms with q sum to dO . O, those with k to
+// dR . (2 U - beta V), and what is left of the scores and of R is 2 dR . (beta V - U).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "args.h"
+#ifdef __CUDACC__
+#include "common.cuh"
+#endif
+
+namespace ccq {
+
+struct GdrArgs {
+  int dtype, B, T, H, HV, K, V, n_seqs;
+  const void* q;     // [B, T, H, K]
+  const void* k;     // [B, T, H, K]
+  const void* v;     // [B, T, HV, V]
+  int g_dtype, beta_dtype;
+  const void* g;     // [B, T, HV] log decay
+  const void* beta;  // [B, T, HV]
+  float scale;
+  const int64_t* cu_seqlens;
+  const float* initial_state;  // [n_seqs, HV, K, V] or nullptr
+  void* o;                     // [B, T, HV, V]
+  float* final_state;          // [n_seqs, HV, K, V] or nullptr
+  // backward
+  const void* d_o;
+  const float* dfinal_state;  // or nullptr
+  void* dq;
+  void* dk;
+  void* dv;
+  void* dg;             // g's type
+  void* dbeta;          // beta's type
+  float* dinitial_state;  // or nullptr
+  void* workspace;
+  size_t workspace_bytes;
+  cudaStream_t stream;
+};
+
+// Exact path: fp32 arithmetic on the CUDA cores, any K <= 256 and any V, fp32 / bf16 / fp16.
+size_t gdr_simt_workspace(const GdrArgs& a, bool bwd);
+cudaError_t gdr_simt_fwd(const GdrArgs& a, int* launches);
+cudaError_t gdr_simt_bwd(const GdrArgs& a, int* launches);
+
+// Token by token over a cache (any T, meant for a few tokens): state_in may equal state_out.
+cudaError_t gdr_step(const GdrArgs& a, int* launches);
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float gate_load(const void* p, int dt, int64_t i) {
+  if (dt == DT_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dt == DT_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void gate_store(void* p, int dt, int64_t i, float x) {
+  if (dt == DT_F32) reinterpret_cast<float*>(p)[i] = x;
+  else if (dt == DT_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
+}
+// A decay below e^-1000 is zero in every type here; the bound keeps sums of g finite when a
+// caller resets the state with g = -inf (a NaN stays one).
+__device__ __forceinline__ float clamp_g(float g) { return g < -1000.f ? -1000.f : g; }
+
+// Chunk slots.  Dense: n * ceil(T / C) + c.  Varlen: floor(bos / C) + n + c (see chunk_slot0).
+__host__ __device__ inline int64_t gdr_slots(const GdrArgs& a, int C) {
+  return a.cu_seqlens ? chunk_slots_total(a.T, a.n_seqs, C) : (int64_t)a.n_seqs * ((a.T + C - 1) / C);
+}
+__device__ __forceinline__ int64_t gdr_slot0(const GdrArgs& a, int n, const Seq& sq, int C) {
+  return a.cu_seqlens ? chunk_slot0(n, sq.bos, C) : (int64_t)n * ((a.T + C - 1) / C);
+}
+// The document and chunk of a slot; false where the slot holds no chunk.
+__device__ __forceinline__ bool gdr_slot_find(const GdrArgs& a, int64_t slot, int C, int* n_out, int* c_out, Seq* sq_out) {
+  int n;
+  if (a.cu_seqlens == nullptr) {
+    n = (int)(slot / ((a.T + C - 1) / C));
+  } else {
+    int lo = 0, hi = a.n_seqs - 1;  // last n whose first slot is <= slot (first slots increase with n)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      const Seq s = seq_of(mid, a.T, a.cu_seqlens);
+      if (chunk_slot0(mid, s.bos, C) <= slot) lo = mid; else hi = mid - 1;
+    }
+    n = lo;
+  }
+  const Seq sq = seq_of(n, a.T, a.cu_seqlens);
+  const int64_t c = slot - gdr_slot0(a, n, sq, C);
+  *n_out = n;
+  *c_out = (int)c;
+  *sq_out = sq;
+  return c >= 0 && c * C < sq.len;
+}
+#endif
+
+}  // namespace ccq

@@ -269,6 +269,76 @@ int ccq_decode_step_l2norm(int dtype, int B, int T, int H, int K,
                            float* cov_out, float* mean_out,
                            void* q_clean, void* k_norm, void* stream);
 
+/*
+ * Gated delta rule: the token mixer that reads the cleaned queries (the backbone operator of
+ * ccq/ops/ccq_gdn/fused_chunk.py:54 and ccq/ops/ccq_gdn/fused_recurrent.py:66).  Per (document, value
+ * head), with a state S [K, V] in fp32:
+ *
+ *   S <- exp(g_t) S;   u_t = beta_t (v_t - S^T k_t);   S <- S + k_t u_t^T;   o_t = scale S^T q_t
+ *
+ *   q, k: [B, T, H, K];  v, o: [B, T, HV, V] in the activation dtype, HV a multiple of H (value head h
+ *   reads key head h / (HV / H));  g (log decay, at most 0 in use) and beta: [B, T, HV], each of its own
+ *   dtype (fp32, bf16 or fp16);  states: [n_seqs, HV, K, V] fp32, NULL initial_state = zeros.
+ *   K <= 256; inputs must be finite, except that g = -inf resets the state (any g below -1000 does).
+ *   final_state may be NULL.  Documents of length zero return their initial state.
+ * All sums, the state and the running sums of g are fp32 or wider.
+ */
+size_t ccq_gdr_workspace_size(int op /* CCQ_OP_FWD or CCQ_OP_BWD */, int dtype, int B, int T, int H, int HV,
+                              int K, int V, int n_seqs, int varlen);
+
+int ccq_gdr_fwd(int dtype, int B, int T, int H, int HV, int K, int V,
+                const void* q, const void* k, const void* v,
+                int g_dtype, const void* g, int beta_dtype, const void* beta, float scale,
+                const int64_t* cu_seqlens, int n_seqs, const float* initial_state,
+                void* o, float* final_state,
+                void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Gradients of the above from d_o and, where given, dfinal_state.  dq and dk are summed over the value
+ * heads of a key head; dg and dbeta have the dtypes of g and beta; dinitial_state may be NULL.  With no
+ * initial_state, dg of a document's first token is exactly zero (nothing decays there).
+ */
+int ccq_gdr_bwd(int dtype, int B, int T, int H, int HV, int K, int V,
+                const void* q, const void* k, const void* v,
+                int g_dtype, const void* g, int beta_dtype, const void* beta, float scale,
+                const int64_t* cu_seqlens, int n_seqs, const float* initial_state,
+                const void* d_o, const float* dfinal_state,
+                void* dq, void* dk, void* dv, void* dg, void* dbeta, float* dinitial_state,
+                void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The same recurrence token by token over a cache (generation: one token or a few per document).
+ * state_in (NULL = zeros) and state_out may be the same buffer.  No workspace.
+ */
+int ccq_gdr_step(int dtype, int B, int T, int H, int HV, int K, int V,
+                 const void* q, const void* k, const void* v,
+                 int g_dtype, const void* g, int beta_dtype, const void* beta, float scale,
+                 const int64_t* cu_seqlens, int n_seqs, const float* state_in, float* state_out,
+                 void* o, void* stream);
+
+/*
+ * Layer norm over the last axis of [rows, D] (1 <= D <= 16384), forward and backward:
+ *   h = x (+ residual);  n = (h - mean) / sqrt(var + eps)  (CCQ_NORM_RMS: mean = 0, var = mean of h^2)
+ *   y = n weight (+ bias);  with gate: y *= gate sigmoid(gate)
+ *   weight and bias: fp32 [D] or NULL;  residual and gate: [rows, D] in x's dtype or NULL;
+ *   h: written when residual is given (the sum in x's dtype; the norm reads the unrounded sum);
+ *   stats: fp32 [rows, 2] mean and 1 / sqrt(var + eps), NULL when no backward follows.
+ * Backward: dh is the gradient arriving on h (or NULL); dx is also the gradient of residual; dweight and
+ * dbias may be NULL.  They are summed in a fixed order: the same inputs give the same bits.
+ */
+typedef enum { CCQ_NORM_LAYER = 0, CCQ_NORM_RMS = 1 } ccq_norm_form;
+
+size_t ccq_layer_norm_workspace_size(int op, int64_t rows, int D);
+
+int ccq_layer_norm_fwd(int dtype, int form, int64_t rows, int D, float eps, const void* x, const void* residual,
+                       const float* weight, const float* bias, const void* gate, void* y, void* h, float* stats,
+                       void* stream);
+
+int ccq_layer_norm_bwd(int dtype, int form, int64_t rows, int D, const void* x, const void* residual,
+                       const float* weight, const float* bias, const void* gate, const float* stats,
+                       const void* dy, const void* dh, void* dx, void* dgate, float* dweight, float* dbias,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
