@@ -527,7 +527,10 @@ size_t ccq_gdr_workspace_size(int op, int dtype, int B, int T, int H, int HV, in
   a.dtype = dtype; a.B = B; a.T = T; a.H = H; a.HV = HV; a.K = K; a.V = V; a.n_seqs = n_seqs;
   static const int64_t some_offsets = 0;
   a.cu_seqlens = varlen ? &some_offsets : nullptr;  // only whether it is given counts
-  return ccq::gdr_simt_workspace(a, op == CCQ_OP_BWD);
+  // a 16-bit call takes the exact path when a tensor is not 16-byte aligned: room for either
+  const size_t simt = ccq::gdr_simt_workspace(a, op == CCQ_OP_BWD);
+  const size_t tc = ccq::gdr_tc_supported(a) ? ccq::gdr_tc_workspace(a, op == CCQ_OP_BWD) : 0;
+  return tc > simt ? tc : simt;
 }
 
 int ccq_gdr_fwd(int dtype, int B, int T, int H, int HV, int K, int V, const void* q, const void* k, const void* v,
@@ -542,14 +545,16 @@ int ccq_gdr_fwd(int dtype, int B, int T, int H, int HV, int K, int V, const void
   if (T > 0 && o == nullptr) return fail(CCQ_ERR_INVALID, "the output o is required");
   a.o = o;
   a.final_state = final_state;
-  st = need_workspace("ccq_gdr_fwd", ccq::gdr_simt_workspace(a, false), workspace, workspace_bytes);
+  const bool tc = ccq::gdr_tc_supported(a);
+  st = need_workspace("ccq_gdr_fwd", tc ? ccq::gdr_tc_workspace(a, false) : ccq::gdr_simt_workspace(a, false), workspace,
+                      workspace_bytes);
   if (st != CCQ_OK) return st;
   int launches = 0;
-  cudaError_t e = ccq::gdr_simt_fwd(a, &launches);
+  cudaError_t e = tc ? ccq::gdr_tc_fwd(a, &launches) : ccq::gdr_simt_fwd(a, &launches);
   if (e != cudaSuccess) return cuda_fail(e, "ccq_gdr_fwd launch");
-  g_path = CCQ_PATH_SIMT;
+  g_path = tc ? CCQ_PATH_TCGEN05 : CCQ_PATH_SIMT;
   g_launches = launches;
-  return CCQ_OK;
+  return tc ? checked_finish("ccq_gdr_fwd", workspace, a.stream) : CCQ_OK;
 }
 
 int ccq_gdr_bwd(int dtype, int B, int T, int H, int HV, int K, int V, const void* q, const void* k, const void* v,

@@ -6,20 +6,21 @@
 // tokens (rows of Q, K, V), with G the running sum of g inside the chunk, Gam = e^G, w = e^{G_C - G},
 // D_ij = e^{G_i - G_j} (j <= i) and S0 the state before the chunk:
 //
-//   R = beta (V - Gam K S0)      T = (1 + strict(beta_i D_ij k_i.k_j))^{-1}      U = T R
-//   O = scale Gam Q S0 + P U     P = scale tril(D_ij q_i.k_j)                    S1 = Gam_C S0 + K^T (w U)
+//   R = V - Gam K S0      T = (1 + strict(D_ij k_i.k_j beta_j))^{-1}       E = T R      U = beta E
+//   O = scale Gam Q S0 + P U     P = scale tril(D_ij q_i.k_j)                S1 = Gam_C S0 + K^T (w U)
 //
-// and backwards, from dO and dS1:
+// (E, the part of V that the state does not hold yet, rather than U: beta then multiplies and never
+// divides, so that beta = 0 needs no case of its own.)  Backwards, from dO and dS1, with L = strict(D k k^T):
 //
-//   dU = P^T dO + w K dS1    dR = T^T dU    dV = beta dR
-//   dS0 = Gam_C dS1 + (scale Gam Q)^T dO - (beta Gam K)^T dR
+//   dE = beta (P^T dO + w K dS1)      dV = T^T dE
+//   dS0 = Gam_C dS1 + (scale Gam Q)^T dO - (Gam K)^T dV
 //   dQ = scale Gam dO S0^T + W K,                 W = scale tril(D dO U^T)
-//   dK = -beta Gam dR S0^T + W^T Q + (N + N^T) K + w U dS1^T,   N = -strict(beta_i D_ij dR_i.U_j)
-//   dbeta_i = dR_i . (V - Gam K S0)_i - sum_j D_ij (k_i.k_j) (dR_i . U_j),  j < i
+//   dK = -Gam dV S0^T + W^T Q + (N + N^T) K + w U dS1^T,   N_ij = -D_ij dV_i.U_j  (j < i)
+//   dbeta_j = sum_i P_ij dO_i.E_j + w_j k_j.(dS1 E_j) - sum_i L_ij dV_i.E_j
 //   dg_t = <dS1, S1> + sum_{i >= t} (dO_i . O_i - V_i . dV_i)      (i inside the chunk)
 //
-// The last line is what collecting every e^G gives: the terms with q sum to dO . O, those with k to
-// dR . (2 U - beta V), and what is left of the scores and of R is 2 dR . (beta V - U).
+// The last line is what collecting every e^G gives: the terms with q sum to dO . O, and those with k, the
+// scores and R to -V . dV.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -64,6 +65,13 @@ struct GdrArgs {
 size_t gdr_simt_workspace(const GdrArgs& a, bool bwd);
 cudaError_t gdr_simt_fwd(const GdrArgs& a, int* launches);
 cudaError_t gdr_simt_bwd(const GdrArgs& a, int* launches);
+
+// Tensor-core path (gdr_tc*.cu): 16-bit inputs, K a multiple of 8 up to 128, V a multiple of 8,
+// 16-byte aligned tensors and workspace.  Word 0 of the workspace receives the device error code.
+bool gdr_tc_supported(const GdrArgs& a);
+size_t gdr_tc_workspace(const GdrArgs& a, bool bwd);
+cudaError_t gdr_tc_fwd(const GdrArgs& a, int* launches);
+cudaError_t gdr_tc_bwd(const GdrArgs& a, int* launches);
 
 // Token by token over a cache (any T, meant for a few tokens): state_in may equal state_out.
 cudaError_t gdr_step(const GdrArgs& a, int* launches);

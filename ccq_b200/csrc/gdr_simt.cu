@@ -1,5 +1,7 @@
 // Gated delta rule, exact path: fp32 arithmetic on the CUDA cores, any K <= 256, any V, every type.
-// Formulas: gdr.h.  Chunks of 32 tokens; four kernels over fp32 buffers in the workspace:
+// Formulas: gdr.h, written here with beta on the rows: (1 + strict(beta_i L_ij)) U = beta R, so that its T
+// is diag(beta) T diag(beta)^{-1} of gdr.h, and dR = T^T dU, dV = beta dR; dbeta_i = dR_i . R_i - sum_j L_ij
+// dR_i . U_j.  Chunks of 32 tokens; four kernels over fp32 buffers in the workspace:
 //   prep    per (chunk, value head): D, L = strict(D k k^T), T, P and the per-token factors;
 //   scan    per (document, value head, 32 columns of V): the state in shared memory, chunk by chunk;
 //           for the backward it also keeps S0, U, V - Gam K S0 and dO . O;

@@ -1,0 +1,62 @@
+// Tensor-core path of the gated delta rule: when it applies, its workspace and its launches.
+#include <string.h>
+
+#include "gdr_tc.cuh"
+
+namespace ccq {
+namespace {
+
+using namespace gdrtc;
+
+size_t carve(const GdrArgs& a, bool bwd, Ws* w) {
+  const size_t sh = (size_t)gdr_slots(a, C) * a.HV;
+  uint8_t* base = reinterpret_cast<uint8_t*>(a.workspace);
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t* p = base ? base + off : nullptr;
+    off += ws_align(bytes);
+    return p;
+  };
+  const size_t nvt = (a.V + VT - 1) / VT;
+  Ws t;
+  memset(&t, 0, sizeof(t));
+  t.err = reinterpret_cast<int*>(take(256));
+  t.mats = take(sh * MATS);
+  t.aux = reinterpret_cast<float*>(take(sh * AX_N * 4));
+  if (bwd) {
+    t.S0 = reinterpret_cast<uint16_t*>(take(sh * a.K * a.V * 2));
+    t.dS1 = reinterpret_cast<uint16_t*>(take(sh * a.K * a.V * 2));
+    t.E = reinterpret_cast<uint16_t*>(take(sh * C * a.V * 2));
+    t.dotO = reinterpret_cast<float*>(take(nvt * sh * C * 4));
+    t.dotV = reinterpret_cast<float*>(take(nvt * sh * C * 4));
+  }
+  if (w) *w = t;
+  return off;
+}
+
+}  // namespace
+
+bool gdr_tc_supported(const GdrArgs& a) {
+  if (a.dtype != DT_BF16 && a.dtype != DT_F16) return false;
+  if (a.T < 1 || a.K > 128 || a.K % 8 != 0 || a.V % 8 != 0) return false;
+  const uintptr_t p = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o | (uintptr_t)a.d_o |
+                      (uintptr_t)a.dq | (uintptr_t)a.dk | (uintptr_t)a.dv | (uintptr_t)a.workspace;
+  return (p & 15) == 0 && tc::encode_fn() != nullptr;
+}
+
+size_t gdr_tc_workspace(const GdrArgs& a, bool bwd) {
+  GdrArgs b = a;
+  b.workspace = nullptr;
+  return carve(b, bwd, nullptr);
+}
+
+cudaError_t gdr_tc_fwd(const GdrArgs& a, int* launches) {
+  Ws w;
+  carve(a, false, &w);
+  cudaError_t e = cudaMemsetAsync(w.err, 0, 8, a.stream);
+  if (e == cudaSuccess) e = prep(a, w, launches);
+  if (e == cudaSuccess) e = scan(a, w, false, launches);
+  return e;
+}
+
+}  // namespace ccq

@@ -1,0 +1,220 @@
+// Gated delta rule, tensor-core path: what its kernels share.  bf16 or fp16, K a multiple of 8 up to
+// 128, V a multiple of 8, 16-byte aligned tensors; chunks of 64 tokens.  Formulas: gdr.h.
+//
+//   prep   (gdr_tc_prep.cu)   per (chunk, value head): T and P and the per-token factors, to the workspace
+//   scan   (gdr_tc_scan.cu)   per (document, value head, 128 columns of V): the state, chunk by chunk
+//   rscan  (gdr_tc_rscan.cu)  the same in reverse for the state's gradient
+//   grads  (gdr_tc_grads.cu)  per (chunk, key head): dq, dk, dg, dbeta
+//
+// Precision.  The tensor cores multiply 16-bit operands.  What enters as an operand of the two scans and is
+// not an input (S, E, T, P and their gradients' counterparts) is given as a sum of two 16-bit numbers,
+// hi + lo, which keeps 2^-17 of it: the state and its gradient then stay at fp32 accuracy over any number
+// of chunks (measured 4e-6 against 64 bits), as they would not with one rounding each (2.4e-3).  The
+// products cost two or three MMAs instead of one; the scans are bound by the latency of one chunk's
+// chain of three products, not by the MMA rate.  The gradient kernel, whose outputs are rounded to 16
+// bits next and feed no recurrence, uses single 16-bit operands.
+#pragma once
+
+#include "gdr.h"
+
+namespace ccq {
+namespace gdrtc {
+
+constexpr int C = 64;             // tokens per chunk
+constexpr int VT = 128;           // columns of V per block of the scans (TMEM lanes)
+constexpr uint32_t PANEL = 64 * 128;        // 64 rows of 128 bytes, 128-byte swizzle
+constexpr uint32_t TILE = 2 * PANEL;        // 64 rows x 128 columns
+constexpr uint32_t MATS = 4 * PANEL;        // T hi, T lo, P beta hi, P beta lo: 64 x 64 each, swizzled as in shared memory
+// per (chunk, value head) floats, 64 tokens each: Gam, scale Gam, w beta, beta, w, G (hi and lo part); then Gam_C
+constexpr int AX_G = 0, AX_SG = 64, AX_WB = 128, AX_B = 192, AX_W = 256, AX_GH = 320, AX_GL = 384, AX_GC = 448, AX_N = 452;
+
+// Workspace regions; every kernel indexes them by sh = slot * HV + value head.
+struct Ws {
+  int* err;            // word 0: device error code of the scans
+  uint8_t* mats;       // [slots * HV][MATS]
+  float* aux;          // [slots * HV][AX_N]
+  // backward only
+  uint16_t* S0;        // [slots * HV][V][K] state before the chunk, transposed, 16-bit
+  uint16_t* dS1;       // [slots * HV][V][K] gradient of the state after it
+  uint16_t* E;         // [slots * HV][C][V]
+  float* dotO;         // [V tiles][slots * HV][C]: dO . O
+  float* dotV;         // [V tiles][slots * HV][C]: V . dV
+};
+
+cudaError_t prep(const GdrArgs& a, const Ws& w, int* launches);
+cudaError_t scan(const GdrArgs& a, const Ws& w, bool bwd, int* launches);
+cudaError_t rscan(const GdrArgs& a, const Ws& w, int* launches);
+cudaError_t grads(const GdrArgs& a, const Ws& w, int* launches);
+
+}  // namespace gdrtc
+}  // namespace ccq
+
+#ifdef __CUDACC__
+#include "tc_common.cuh"
+#include "tma_host.h"
+
+namespace ccq {
+namespace gdrtc {
+
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ void fma2(float* d, const float* a, const float* b, const float* c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pair(a[0], a[1])), "l"(pair(b[0], b[1])), "l"(pair(c[0], c[1])));
+  unpair(r, d[0], d[1]);
+}
+__device__ __forceinline__ void add2f(float* d, const float* a, const float* b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a[0], a[1])), "l"(pair(b[0], b[1])));
+  unpair(r, d[0], d[1]);
+}
+__device__ __forceinline__ void mul2f(float* d, const float* a, const float* b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pair(a[0], a[1])), "l"(pair(b[0], b[1])));
+  unpair(r, d[0], d[1]);
+}
+
+// 2 n values as n packed hi words and n packed lo words
+template <int AB16, int N>
+__device__ __forceinline__ void split(const float* x, uint32_t* hi, uint32_t* lo) {
+  const float m1[2] = {-1.f, -1.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    hi[i] = tc::pack2<AB16>(x[2 * i], x[2 * i + 1]);
+    const float2 f = tc::unpack2<AB16>(hi[i]);
+    const float h[2] = {f.x, f.y};
+    float r[2];
+    fma2(r, h, m1, x + 2 * i);
+    lo[i] = tc::pack2<AB16>(r[0], r[1]);
+  }
+}
+
+// 16 fp32 values of this thread's lane as 8 packed columns at hi and 8 at lo
+template <int AB16>
+__device__ __forceinline__ void st_split16(uint32_t hi_addr, uint32_t lo_addr, const float* x) {
+  uint32_t hi[8], lo[8];
+  split<AB16, 8>(x, hi, lo);
+  tc::tmem_st8(hi_addr, hi);
+  tc::tmem_st8(lo_addr, lo);
+}
+
+// 16 consecutive fp32 columns of this thread's lane
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+template <int AB16>
+__device__ __forceinline__ float h2f(uint16_t x) {
+  if (AB16) return __uint_as_float((uint32_t)x << 16);
+  return __half2float(__ushort_as_half(x));
+}
+template <int AB16>
+__device__ __forceinline__ uint16_t f2h(float x) {
+  if (AB16) return __bfloat16_as_ushort(__float2bfloat16_rn(x));
+  return __half_as_ushort(__float2half_rn(x));
+}
+
+// A [64 tokens x 128 columns] tile of two swizzled panels, read or written one column per thread:
+// `col` 0..127 is the thread's column.
+struct Column {
+  uint32_t base, chunk, byte;
+  __device__ __forceinline__ Column(uint32_t tile, int col)
+      : base(tile + (uint32_t)(col >> 6) * PANEL), chunk((uint32_t)(col & 63) >> 3), byte((uint32_t)(col & 7) * 2) {}
+  __device__ __forceinline__ uint32_t at(int row) const { return base + tc::sw128(row, chunk) + byte; }
+};
+__device__ __forceinline__ uint16_t lds16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts16(uint32_t addr, uint16_t v) {
+  asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+// untiled bulk copy global -> shared; addresses and size are multiples of 16 bytes
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   tc::smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+               : "memory");
+}
+
+// rows [from, 64) of a tile of `panels` panels set to zero by `count` threads, this one being `t`
+__device__ __forceinline__ void zero_rows(uint32_t tile, int panels, int from, int t, int count) {
+  for (int i = t; i < panels * (64 - from) * 8; i += count) {
+    const int p = i / ((64 - from) * 8), r = i % ((64 - from) * 8);
+    sts128(tile + p * PANEL + (from + (r >> 3)) * 128 + (r & 7) * 16, make_uint4(0, 0, 0, 0));
+  }
+}
+
+// rows [0, valid) of a staged [64 x 128] tile to a [tokens, HV, V] tensor with plain stores
+__device__ __forceinline__ void copy_rows(uint32_t tile, uint16_t* dst, int64_t row0, int HV, int hv, int V, int v0,
+                                          int valid, int t, int count) {
+  for (int i = t; i < valid * 16; i += count) {
+    const int r = i >> 4, ch = i & 15;
+    if (v0 + ch * 8 < V)
+      *reinterpret_cast<uint4*>(dst + ((row0 + r) * HV + hv) * V + v0 + ch * 8) =
+          lds128(tile + (ch >> 3) * PANEL + tc::sw128(r, ch & 7));
+  }
+}
+
+// pipe_wait for the MMA thread: polls without suspending (a suspended try_wait wakes a few hundred cycles
+// late, and this thread's waits are all on the chunk's critical path), bounded like the others.
+__device__ __forceinline__ bool spin_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int code) {
+  if (tc::mbar_test(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!tc::mbar_test(bar, parity)) {
+    if (*abort) return false;
+    if (clock64() - t0 > (1ll << 31)) {
+      *abort = 1;
+      atomicOr(err, code);
+      return false;
+    }
+  }
+  return true;
+}
+
+// sum over the 32 lanes of 2^k values a thread, in place: afterwards lane l holds in x[0 .. n/32) (n >= 32)
+// the sums of values l * n / 32 + ...; each step halves what a thread keeps
+template <int N>
+__device__ __forceinline__ void lane_sums(float* x, int lane) {
+#pragma unroll
+  for (int o = 16, n = N; o > 0; o >>= 1, n >>= 1) {
+    const bool up = (lane & o) != 0;
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const float send = up ? x[i] : x[i + n / 2], keep = up ? x[i + n / 2] : x[i];
+      x[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+}
+
+inline cudaError_t token_map(CUtensorMap* m, const GdrArgs& a, const void* p, int heads, int width) {
+  return tc::make_token_map(m, p, (int64_t)a.B * a.T, heads, width, C, a.dtype == DT_BF16);
+}
+
+}  // namespace gdrtc
+}  // namespace ccq
+#endif

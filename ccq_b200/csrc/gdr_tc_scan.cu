@@ -1,0 +1,402 @@
+// Tensor-core path of the gated delta rule, forward scan: one block per (document, value head, 128
+// columns of V) walks the document in chunks of 64 tokens.  Everything is held transposed, one column of V
+// per TMEM lane, so that the three products of a chunk chain through TMEM without a transposition:
+//
+//   X^T | Y^T = S^T [K ; Q]^T   [128 x 128]  A: S hi + lo (TMEM), B: the K and Q rows, one above the other
+//   E^T  = V^T T^T              [128 x 128]  A: the V tile, read MN-major, B: [T hi | T lo] side by side
+//        + (-Gam X)^T T^T                    A: Gam X hi + lo (chain warps, back to TMEM), B: T hi, lo
+//   dS^T = (w beta E)^T K       [128 x K]    A: hi + lo (chain warps), B: the K rows, read MN-major
+//   S^T  = Gam_C S^T + dS^T                  (chain warps: S is kept in their registers in fp32)
+//   O^T  = scale Gam Y^T + E^T (P beta)^T    (beside the chain; output warps)
+//
+// The chunks are sequential, so the kernel is bound by the latency of that chain (three MMA groups, three
+// TMEM round trips) and not by the MMA rate or by memory; a second block on an SM does not fit (TMEM is
+// full), and splitting K or V further would not shorten the chain.  An MMA with its A operand in TMEM
+// takes about 64 cycles for any N up to 128 here, so what can share an A operand is put side by side in N.
+// The rest of a chunk's period is instructions of the chain warps between the products, so V enters by an MMA
+// of its own (beside the chain) and the factors by packed two-value arithmetic.
+//
+// BWD: instead of O it writes what the backward reads: S0 (16-bit, transposed), E (16-bit) and dO . O.
+//
+// Warps (448 threads): 0-3 output (one per TMEM quadrant), 4-11 chain (two per quadrant, each half of the
+// columns), 12 TMA, 13 MMA.  TMEM columns: S hi, S lo (64 each), X | Y, then dS (128), E, then E P^T
+// (128), Gam X / E as operands (64), w beta E as operand (64): all 512.  Every wait is bounded; see tc_common.cuh.
+#include "gdr_tc.cuh"
+
+namespace ccq {
+namespace gdrtc {
+namespace {
+using namespace tc;
+
+constexpr int THREADS = 448;
+constexpr uint32_t T_SH = 0, T_SL = 64, T_X = 128, T_D = 256, T_RH = 384, T_RL = 416, T_WH = 448, T_WL = 480;
+
+struct Small {
+  uint64_t full[2], empty[2], s_ready, x_full, r_ready, u_full, u_ready, d_full, o1_read, o_full, o2_free, kz, done;
+  float red[4][C];
+  uint32_t tmem;
+  int abort;
+};
+
+template <bool BWD>
+struct Lay {  // offsets of one stage, then of the rest
+  static constexpr uint32_t KQ = 0, V = 2 * TILE, DO = 3 * TILE, M = (BWD ? 4 : 3) * TILE, AX = M + MATS;
+  static constexpr uint32_t STAGE = (AX + AX_N * 4 + 1023) & ~1023u;
+  static constexpr uint32_t OUT = 2 * STAGE, SMALL = OUT + (BWD ? 0 : TILE);
+  static constexpr uint32_t BYTES = SMALL + sizeof(Small) + 1024;
+};
+static_assert(Lay<true>::BYTES <= 232448 && Lay<false>::BYTES <= 232448, "shared memory");
+
+template <int AB16, int KD, bool BWD>
+__global__ void __launch_bounds__(THREADS, 1)
+    scan_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+                const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmo, GdrArgs a, Ws w) {
+  using L = Lay<BWD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Small& S_ = *reinterpret_cast<Small*>(sm + L::SMALL);
+  const uint32_t sb = smem_u32(sm);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = blockIdx.x / a.HV, hv = blockIdx.x % a.HV, h = hv / (a.HV / a.H);
+  const int v0 = blockIdx.y * VT;
+  const Seq sq = seq_of(n, a.T, a.cu_seqlens);
+  const int nch = (sq.len + C - 1) / C;
+  const int64_t sh0 = gdr_slot0(a, n, sq, C) * a.HV + hv;  // chunk c is at sh0 + c * HV
+  const int64_t st = ((int64_t)n * a.HV + hv) * a.K * a.V;
+  constexpr int NP = KD / 64;  // panels of K and Q
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&S_.full[i], 1);
+      mbar_init(&S_.empty[i], 13);  // last commit, 8 chain warps, 4 output warps
+    }
+    mbar_init(&S_.s_ready, 8);
+    mbar_init(&S_.r_ready, 8);
+    mbar_init(&S_.u_ready, 8);
+    mbar_init(&S_.x_full, 1);
+    mbar_init(&S_.u_full, 1);
+    mbar_init(&S_.d_full, 1);
+    mbar_init(&S_.o_full, 1);
+    mbar_init(&S_.o1_read, 4);
+    mbar_init(&S_.o2_free, 4);
+    mbar_init(&S_.kz, 4);
+    mbar_init(&S_.done, 1);
+    S_.abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 13) tmem_alloc(&S_.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tb = S_.tmem;
+  volatile int* ab = &S_.abort;
+  int* err = w.err;
+
+  if (warp == 12) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int issued = 0;
+      for (int c = 0; c < nch; ++c) {
+        const int s = c & 1;
+        if (c >= 2 && !pipe_wait(&S_.empty[s], ((c - 2) >> 1) & 1, ab, err, 1)) break;
+        if (*ab) break;
+        uint8_t* p = sm + s * L::STAGE;
+        uint64_t* bar = &S_.full[s];
+        mbar_arrive_expect_tx(bar, 2 * NP * PANEL + (BWD ? 2 : 1) * TILE + MATS + AX_N * 4);
+        const int row = (int)(sq.bos + (int64_t)c * C);
+        const int64_t sh = sh0 + (int64_t)c * a.HV;
+        for (int i = 0; i < NP; ++i) tma_load_3d(p + L::KQ + 2 * i * PANEL, &tmk, bar, 64 * i, h, row);
+        tma_load_3d(p + L::V, &tmv, bar, v0, hv, row);
+        tma_load_3d(p + L::V + PANEL, &tmv, bar, v0 + 64, hv, row);
+        bulk_load(p + L::AX, w.aux + sh * AX_N, AX_N * 4, bar);
+        bulk_load(p + L::M, w.mats + sh * MATS, MATS, bar);
+        for (int i = 0; i < NP; ++i) tma_load_3d(p + L::KQ + (2 * i + 1) * PANEL, &tmq, bar, 64 * i, h, row);
+        if (BWD) {
+          tma_load_3d(p + L::DO, &tmo, bar, v0, hv, row);
+          tma_load_3d(p + L::DO + PANEL, &tmo, bar, v0 + 64, hv, row);
+        }
+        ++issued;
+      }
+      // never leave the block with copies in flight
+      for (int c = (issued > 2 ? issued - 2 : 0); c < issued; ++c) own_copy_wait(&S_.full[c & 1], (c >> 1) & 1, ab, err, 2);
+    }
+  } else if (warp == 13) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const uint32_t id64 = idesc_f16(128, 64, AB16, 0, 0), id128 = idesc_f16(128, 128, AB16, 0, 0);
+      const uint32_t id_d = idesc_f16(128, KD, AB16, 0, 1), id_v = idesc_f16(128, 128, AB16, 1, 0);
+      for (int c = 0; c < nch; ++c) {
+        const int s = c & 1, ph = c & 1;
+        const uint32_t p = sb + s * L::STAGE;
+        const uint32_t T = p + L::M, P = T + 2 * PANEL;
+        // X^T | Y^T
+        if (!spin_wait(&S_.full[s], (c >> 1) & 1, ab, err, 4)) break;
+        if ((c + 1) * C > sq.len && !spin_wait(&S_.kz, 0, ab, err, 8)) break;
+        if (!spin_wait(&S_.s_ready, ph, ab, err, 0x10)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int ks = 0; ks < KD / 16; ++ks)
+            umma_ts(tb + T_X, tb + (x ? T_SL : T_SH) + 8 * ks,
+                    sdesc(p + L::KQ + (ks >> 2) * 2 * PANEL + (ks & 3) * 32, 16, 1024), id128, x + ks > 0);
+        umma_commit(&S_.x_full);
+        // E^T = V^T T^T, then + (-Gam X)^T T^T; the hi and lo halves are added on reading
+        if (c > 0 && !spin_wait(&S_.o2_free, (c - 1) & 1, ab, err, 0x20)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+          umma(tb + T_D, sdesc(p + L::V + ks * 2048, PANEL, 1024), sdesc(T + ks * 32, 16, 1024), id_v, ks > 0);
+        if (!spin_wait(&S_.r_ready, ph, ab, err, 0x40)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RH + 8 * ks, sdesc(T + ks * 32, 16, 1024), id128, 1);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RL + 8 * ks, sdesc(T + ks * 32, 16, 1024), id64, 1);
+        umma_commit(&S_.u_full);
+        // dS^T = (w beta E)^T K over X | Y, then E^T (P beta)^T over E
+        if (!spin_wait(&S_.o1_read, ph, ab, err, 0x200)) break;
+        if (!spin_wait(&S_.u_ready, ph, ab, err, 0x80)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma_ts(tb + T_X, tb + (x ? T_WL : T_WH) + 8 * ks, sdesc(p + L::KQ + ks * 2048, 2 * PANEL, 1024), id_d, x + ks > 0);
+        umma_commit(&S_.d_full);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RH + 8 * ks, sdesc(P + ks * 32, 16, 1024), id128, ks > 0);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RL + 8 * ks, sdesc(P + ks * 32, 16, 1024), id64, 1);
+        umma_commit(&S_.o_full);
+        umma_commit(&S_.empty[s]);
+      }
+      umma_commit(&S_.done);  // TMEM is freed only after every issued MMA has completed
+      mbar_wait(&S_.done, 0);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ chain: Gam X, E, S
+    constexpr int KH = KD / 2;  // columns of K this thread keeps
+    const int quad = warp & 3, hh = (warp - 4) >> 2;
+    const int vl = quad * 32 + lane;
+    const bool vin = v0 + vl < a.V;
+    const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
+    float S[KH];
+#pragma unroll
+    for (int i = 0; i < KH; ++i) {
+      const int k = KH * hh + i;
+      S[i] = (a.initial_state && vin && k < a.K) ? a.initial_state[st + (int64_t)k * a.V + v0 + vl] : 0.f;
+    }
+    // S as the operand of chunk c (and, for the backward, to the workspace)
+    auto put_state = [&](int c) {
+      uint16_t* g = BWD && vin ? w.S0 + ((sh0 + (int64_t)c * a.HV) * a.V + v0 + vl) * a.K + KH * hh : nullptr;
+#pragma unroll
+      for (int i = 0; i < KH; i += 16) {
+        uint32_t hi[8], lo[8];
+        split<AB16, 8>(S + i, hi, lo);
+        tmem_st8(tl + T_SH + hh * (KH / 2) + i / 2, hi);
+        tmem_st8(tl + T_SL + hh * (KH / 2) + i / 2, lo);
+        if (BWD && vin) {
+          if (KH * hh + i < a.K) *reinterpret_cast<uint4*>(g + i) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          if (KH * hh + i + 8 < a.K) *reinterpret_cast<uint4*>(g + i + 8) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&S_.s_ready);
+    };
+    if (nch > 0) put_state(0);
+    for (int c = 0; c < nch; ++c) {
+      const int s = c & 1, ph = c & 1;
+      const float* ax = reinterpret_cast<const float*>(sm + s * L::STAGE + L::AX);
+      const int i0 = 32 * hh;
+      pipe_wait(&S_.full[s], (c >> 1) & 1, ab, err, 0x400);
+      pipe_wait(&S_.x_full, ph, ab, err, 0x800);
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 32; i += 16) {
+        float x[16];
+        tmem_ld16(tl + T_X + i0 + i, x);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(ax + AX_G + i0 + i + j);
+          const float bb[4] = {-b.x, -b.y, -b.z, -b.w};
+          mul2f(x + j, x + j, bb);
+          mul2f(x + j + 2, x + j + 2, bb + 2);
+        }
+        st_split16<AB16>(tl + T_RH + 16 * hh + i / 2, tl + T_RL + 16 * hh + i / 2, x);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&S_.r_ready);
+      pipe_wait(&S_.u_full, ph, ab, err, 0x1000);
+      tc_fence_after();
+      const float gam[2] = {ax[AX_GC], ax[AX_GC]};
+      uint32_t e16[16];
+#pragma unroll
+      for (int i = 0; i < 32; i += 16) {
+        float x[16], y[16];
+        tmem_ld16(tl + T_D + i0 + i, x);
+        tmem_ld16(tl + T_D + 64 + i0 + i, y);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) add2f(x + j, x + j, y + j);
+        uint32_t lo[8];
+        split<AB16, 8>(x, e16 + i / 2, lo);
+        tmem_st8(tl + T_RH + 16 * hh + i / 2, e16 + i / 2);
+        tmem_st8(tl + T_RL + 16 * hh + i / 2, lo);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + i + j);
+          const float bb[4] = {b.x, b.y, b.z, b.w};
+          mul2f(x + j, x + j, bb);
+          mul2f(x + j + 2, x + j + 2, bb + 2);
+        }
+        st_split16<AB16>(tl + T_WH + 16 * hh + i / 2, tl + T_WL + 16 * hh + i / 2, x);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&S_.u_ready);
+      warp_arrive(&S_.empty[s]);
+      if (BWD && vin) {
+        uint16_t* g = w.E + ((sh0 + (int64_t)c * a.HV) * C + i0) * a.V + v0 + vl;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) g[(int64_t)i * a.V] = (uint16_t)(e16[i / 2] >> (16 * (i & 1)));
+      }
+      pipe_wait(&S_.d_full, ph, ab, err, 0x2000);
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < KH; i += 16) {
+        float x[16];
+        tmem_ld16(tl + T_X + KH * hh + i, x);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) fma2(S + i + j, gam, S + i + j, x + j);
+      }
+      if (c + 1 < nch) put_state(c + 1);
+    }
+    if (!BWD && a.final_state && vin) {
+#pragma unroll
+      for (int i = 0; i < KH; ++i) {
+        const int k = KH * hh + i;
+        if (k < a.K) a.final_state[st + (int64_t)k * a.V + v0 + vl] = S[i];
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ output
+    const int vl = warp * 32 + lane;
+    const uint32_t tl = tb + ((uint32_t)(warp * 32) << 16);
+    const int64_t slots = gdr_slots(a, C);
+    for (int c = 0; c < nch; ++c) {
+      const int s = c & 1, ph = c & 1;
+      const int valid = min(C, sq.len - c * C);
+      const uint32_t p = sb + s * L::STAGE;
+      const float* ax = reinterpret_cast<const float*>(sm + s * L::STAGE + L::AX);
+      const int64_t row0 = sq.bos + (int64_t)c * C;
+      pipe_wait(&S_.full[s], (c >> 1) & 1, ab, err, 0x4000);
+      if (valid < C) {
+        // the rows past the document belong to another one: what a product sums over must be zero
+        for (int i = 0; i < NP; ++i) zero_rows(p + L::KQ + 2 * i * PANEL, 1, valid, threadIdx.x, 128);
+        zero_rows(p + L::V, 2, valid, threadIdx.x, 128);
+        fence_async_smem();
+        warp_arrive(&S_.kz);
+      }
+      float y[64];
+      pipe_wait(&S_.x_full, ph, ab, err, 0x8000);
+      tc_fence_after();
+      tmem_ld64(tl + T_X + 64, y);
+      tc_fence_before();
+      warp_arrive(&S_.o1_read);
+#pragma unroll
+      for (int i = 0; i < 64; i += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(ax + AX_SG + i);
+        y[i] *= b.x;
+        y[i + 1] *= b.y;
+        y[i + 2] *= b.z;
+        y[i + 3] *= b.w;
+      }
+      pipe_wait(&S_.o_full, ph, ab, err, 0x10000);
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 64; i += 16) {
+        float x[16], z[16];
+        tmem_ld16(tl + T_D + i, x);
+        tmem_ld16(tl + T_D + 64 + i, z);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) y[i + j] += x[j] + z[j];
+      }
+      tc_fence_before();
+      warp_arrive(&S_.o2_free);
+      if (!BWD) {
+        warp_arrive(&S_.empty[s]);
+        const uint32_t out = sb + L::OUT;
+        if (threadIdx.x == 0) bulk_wait_read();  // the stores of the chunk before have read the tile
+        bar_sync<1, 128>();
+        const Column O(out, vl);
+#pragma unroll
+        for (int i = 0; i < 64; ++i) sts16(O.at(i), f2h<AB16>(y[i]));
+        if (valid == C) {
+          fence_async_smem();
+          bar_sync<1, 128>();
+          if (threadIdx.x == 0) {
+            tma_store_3d(&tmo, sm + L::OUT, v0, hv, (int)row0);
+            if (v0 + 64 < a.V) tma_store_3d(&tmo, sm + L::OUT + PANEL, v0 + 64, hv, (int)row0);
+            bulk_commit();
+          }
+        } else {
+          bar_sync<1, 128>();
+          copy_rows(out, reinterpret_cast<uint16_t*>(a.o), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, 128);
+        }
+      } else {
+        const Column D(p + L::DO, vl);
+#pragma unroll
+        for (int i = 0; i < 64; ++i) y[i] = i < valid ? y[i] * h2f<AB16>(lds16(D.at(i))) : 0.f;
+        warp_arrive(&S_.empty[s]);
+        lane_sums<64>(y, lane);
+        S_.red[warp][2 * lane] = y[0];
+        S_.red[warp][2 * lane + 1] = y[1];
+        bar_sync<1, 128>();
+        if (threadIdx.x < C) {
+          const int i = threadIdx.x;
+          w.dotO[((int64_t)blockIdx.y * slots * a.HV + sh0 + (int64_t)c * a.HV) * C + i] =
+              S_.red[0][i] + S_.red[1][i] + S_.red[2][i] + S_.red[3][i];
+        }
+        bar_sync<1, 128>();
+      }
+    }
+    if (!BWD && threadIdx.x == 0) bulk_wait_all();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 13) tmem_dealloc(tb, 512);
+}
+
+template <int AB16, int KD, bool BWD>
+cudaError_t launch(const GdrArgs& a, const Ws& w) {
+  CUtensorMap q, k, v, o;
+  cudaError_t e = token_map(&q, a, a.q, a.H, a.K);
+  if (e == cudaSuccess) e = token_map(&k, a, a.k, a.H, a.K);
+  if (e == cudaSuccess) e = token_map(&v, a, a.v, a.HV, a.V);
+  if (e == cudaSuccess) e = token_map(&o, a, BWD ? a.d_o : a.o, a.HV, a.V);
+  constexpr uint32_t bytes = Lay<BWD>::BYTES;
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(scan_kernel<AB16, KD, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) return e;
+  scan_kernel<AB16, KD, BWD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), THREADS, bytes, a.stream>>>(q, k, v, o, a, w);
+  return cudaGetLastError();
+}
+
+template <int AB16>
+cudaError_t pick(const GdrArgs& a, const Ws& w, bool bwd) {
+  if (a.K <= 64) return bwd ? launch<AB16, 64, true>(a, w) : launch<AB16, 64, false>(a, w);
+  return bwd ? launch<AB16, 128, true>(a, w) : launch<AB16, 128, false>(a, w);
+}
+
+}  // namespace
+
+cudaError_t scan(const GdrArgs& a, const Ws& w, bool bwd, int* launches) {
+  ++*launches;
+  return a.dtype == DT_BF16 ? pick<1>(a, w, bwd) : pick<0>(a, w, bwd);
+}
+
+}  // namespace gdrtc
+}  // namespace ccq
