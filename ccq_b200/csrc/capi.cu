@@ -573,14 +573,16 @@ int ccq_gdr_bwd(int dtype, int B, int T, int H, int HV, int K, int V, const void
   a.dfinal_state = dfinal_state;
   a.dq = dq; a.dk = dk; a.dv = dv; a.dg = dg; a.dbeta = dbeta;
   a.dinitial_state = dinitial_state;
-  st = need_workspace("ccq_gdr_bwd", ccq::gdr_simt_workspace(a, true), workspace, workspace_bytes);
+  const bool tc = ccq::gdr_tc_supported(a);
+  st = need_workspace("ccq_gdr_bwd", tc ? ccq::gdr_tc_workspace(a, true) : ccq::gdr_simt_workspace(a, true), workspace,
+                      workspace_bytes);
   if (st != CCQ_OK) return st;
   int launches = 0;
-  cudaError_t e = ccq::gdr_simt_bwd(a, &launches);
+  cudaError_t e = tc ? ccq::gdr_tc_bwd(a, &launches) : ccq::gdr_simt_bwd(a, &launches);
   if (e != cudaSuccess) return cuda_fail(e, "ccq_gdr_bwd launch");
-  g_path = CCQ_PATH_SIMT;
+  g_path = tc ? CCQ_PATH_TCGEN05 : CCQ_PATH_SIMT;
   g_launches = launches;
-  return CCQ_OK;
+  return tc ? checked_finish("ccq_gdr_bwd", workspace, a.stream) : CCQ_OK;
 }
 
 int ccq_gdr_step(int dtype, int B, int T, int H, int HV, int K, int V, const void* q, const void* k, const void* v,

@@ -29,6 +29,9 @@ size_t carve(const GdrArgs& a, bool bwd, Ws* w) {
     t.E = reinterpret_cast<uint16_t*>(take(sh * C * a.V * 2));
     t.dotO = reinterpret_cast<float*>(take(nvt * sh * C * 4));
     t.dotV = reinterpret_cast<float*>(take(nvt * sh * C * 4));
+    const size_t ah = (size_t)gdr_slots(a, C * ANCHOR) * a.HV;
+    t.Sf = reinterpret_cast<float*>(take(ah * a.K * a.V * 4));
+    t.anchor = reinterpret_cast<float*>(take(nvt * ah * 8 * 4));
   }
   if (w) *w = t;
   return off;
@@ -56,6 +59,17 @@ cudaError_t gdr_tc_fwd(const GdrArgs& a, int* launches) {
   cudaError_t e = cudaMemsetAsync(w.err, 0, 8, a.stream);
   if (e == cudaSuccess) e = prep(a, w, launches);
   if (e == cudaSuccess) e = scan(a, w, false, launches);
+  return e;
+}
+
+cudaError_t gdr_tc_bwd(const GdrArgs& a, int* launches) {
+  Ws w;
+  carve(a, true, &w);
+  cudaError_t e = cudaMemsetAsync(w.err, 0, 8, a.stream);
+  if (e == cudaSuccess) e = prep(a, w, launches);
+  if (e == cudaSuccess) e = scan(a, w, true, launches);
+  if (e == cudaSuccess) e = rscan(a, w, launches);
+  if (e == cudaSuccess) e = grads(a, w, launches);
   return e;
 }
 

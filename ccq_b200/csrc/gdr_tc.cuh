@@ -28,6 +28,12 @@ constexpr uint32_t MATS = 4 * PANEL;        // T hi, T lo, P beta hi, P beta lo:
 // per (chunk, value head) floats, 64 tokens each: Gam, scale Gam, w beta, beta, w, G (hi and lo part); then Gam_C
 constexpr int AX_G = 0, AX_SG = 64, AX_WB = 128, AX_B = 192, AX_W = 256, AX_GH = 320, AX_GL = 384, AX_GC = 448, AX_N = 452;
 
+// <dS, S> at a chunk's end, which every dg of the chunk holds, is the sum of the later tokens' dO . O - V . dV
+// plus its value at a later place.  Both dot products are kept to fp32, and every ANCHOR chunks <dS, S>
+// itself is formed from fp32 states, so that neither the 16-bit copies of the states (which left 5e-3 in
+// dg) nor a long document's sum of rounding errors gets into dg.
+constexpr int ANCHOR = 8;
+
 // Workspace regions; every kernel indexes them by sh = slot * HV + value head.
 struct Ws {
   int* err;            // word 0: device error code of the scans
@@ -39,6 +45,8 @@ struct Ws {
   uint16_t* E;         // [slots * HV][C][V]
   float* dotO;         // [V tiles][slots * HV][C]: dO . O
   float* dotV;         // [V tiles][slots * HV][C]: V . dV
+  float* Sf;           // [slots of 512 * HV][K][V] fp32 state after every ANCHOR chunks and after the last one
+  float* anchor;       // [V tiles][slots of 512 * HV][8]: <dS, S> there, one part per chain warp
 };
 
 cudaError_t prep(const GdrArgs& a, const Ws& w, int* launches);

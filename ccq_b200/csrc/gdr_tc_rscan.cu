@@ -1,0 +1,403 @@
+// Tensor-core path of the gated delta rule, reverse scan: one block per (document, value head, 128
+// columns of V) walks the document backwards in chunks of 64 tokens with dS, the gradient of the state
+// after the chunk.  Transposed as in the scan, one column of V per TMEM lane:
+//
+//   Z^T  = dO^T (P beta)        [128 x 64]   A: the dO tile, read MN-major, B: P beta hi, lo, read MN-major
+//   Y^T  = dS^T K^T             [128 x 64]   A: dS hi + lo (TMEM), B: the K rows
+//   dE^T = Z^T + w beta Y^T                  (chain warps; split to hi + lo, back to TMEM)
+//   dV^T = dE^T T               [128 x 128]  A: dE hi, B: [T hi | T lo]; and dE lo with T hi
+//   D^T  = (scale Gam dO)^T Q   [128 x K]    A: hi + lo (output warps, beside the chain), B: Q, MN-major
+//        + (-Gam dV)^T K                     A: hi + lo (chain warps), B: the K rows, MN-major
+//   dS^T = Gam_C dS^T + D^T                  (chain warps: dS is kept in their registers in fp32)
+//
+// Written out: dV, V . dV per token, for the gradient kernel dS (16-bit, transposed) of every chunk, and every
+// ANCHOR chunks <dS, S>.
+// Bound, as the scan, by the latency of one chunk's chain.  Warps as in the scan.  TMEM columns: dS hi, lo
+// (64 each), Y and Z (64 each), then dV (128), D (128), dE, then Gam dV as operand (64), scaled dO (64).
+#include "gdr_tc.cuh"
+
+namespace ccq {
+namespace gdrtc {
+namespace {
+using namespace tc;
+
+constexpr int THREADS = 448;
+constexpr uint32_t T_SH = 0, T_SL = 64, T_Y = 128, T_Z = 192, T_D = 256, T_EH = 384, T_EL = 416, T_GH = 448, T_GL = 480;
+
+struct Small {
+  uint64_t full[2], empty[2], s_ready, y_full, e_ready, f_full, f_ready, f_read, g_ready, d_full, kz, done;
+  float red[4][C];
+  uint32_t tmem;
+  int abort;
+};
+
+constexpr uint32_t L_KQ = 0, L_V = 2 * TILE, L_DO = 3 * TILE, L_M = 4 * TILE, L_AX = L_M + MATS;
+constexpr uint32_t L_STAGE = (L_AX + AX_N * 4 + 1023) & ~1023u;
+constexpr uint32_t L_OUT = 2 * L_STAGE, L_SMALL = L_OUT + TILE;
+constexpr uint32_t L_BYTES = L_SMALL + sizeof(Small) + 1024;
+static_assert(L_BYTES <= 232448, "shared memory");
+
+template <int AB16, int KD>
+__global__ void __launch_bounds__(THREADS, 1)
+    rscan_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+                 const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmo,
+                 const __grid_constant__ CUtensorMap tmdv, GdrArgs a, Ws w) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Small& S_ = *reinterpret_cast<Small*>(sm + L_SMALL);
+  const uint32_t sb = smem_u32(sm);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = blockIdx.x / a.HV, hv = blockIdx.x % a.HV, h = hv / (a.HV / a.H);
+  const int v0 = blockIdx.y * VT;
+  const Seq sq = seq_of(n, a.T, a.cu_seqlens);
+  const int nch = (sq.len + C - 1) / C;
+  const int64_t sh0 = gdr_slot0(a, n, sq, C) * a.HV + hv;  // chunk c is at sh0 + c * HV
+  const int64_t st = ((int64_t)n * a.HV + hv) * a.K * a.V;
+  constexpr int NP = KD / 64;  // panels of K and Q
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&S_.full[i], 1);
+      mbar_init(&S_.empty[i], 13);  // last commit, 8 chain warps, 4 output warps
+    }
+    mbar_init(&S_.s_ready, 8);
+    mbar_init(&S_.e_ready, 8);
+    mbar_init(&S_.f_ready, 8);
+    mbar_init(&S_.f_read, 4);
+    mbar_init(&S_.g_ready, 4);
+    mbar_init(&S_.kz, 4);
+    mbar_init(&S_.y_full, 1);
+    mbar_init(&S_.f_full, 1);
+    mbar_init(&S_.d_full, 1);
+    mbar_init(&S_.done, 1);
+    S_.abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 13) tmem_alloc(&S_.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tb = S_.tmem;
+  volatile int* ab = &S_.abort;
+  int* err = w.err;
+  const bool part = sq.len % C != 0;  // the last chunk, the first one here, is partial
+
+  if (warp == 12) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int issued = 0;
+      for (int t = 0; t < nch; ++t) {
+        const int s = t & 1, c = nch - 1 - t;
+        if (t >= 2 && !pipe_wait(&S_.empty[s], ((t - 2) >> 1) & 1, ab, err, 1)) break;
+        if (*ab) break;
+        uint8_t* p = sm + s * L_STAGE;
+        uint64_t* bar = &S_.full[s];
+        mbar_arrive_expect_tx(bar, 2 * NP * PANEL + 2 * TILE + MATS + AX_N * 4);
+        const int row = (int)(sq.bos + (int64_t)c * C);
+        const int64_t sh = sh0 + (int64_t)c * a.HV;
+        for (int i = 0; i < NP; ++i) tma_load_3d(p + L_KQ + 2 * i * PANEL, &tmk, bar, 64 * i, h, row);
+        tma_load_3d(p + L_DO, &tmo, bar, v0, hv, row);
+        tma_load_3d(p + L_DO + PANEL, &tmo, bar, v0 + 64, hv, row);
+        bulk_load(p + L_AX, w.aux + sh * AX_N, AX_N * 4, bar);
+        bulk_load(p + L_M, w.mats + sh * MATS, MATS, bar);
+        for (int i = 0; i < NP; ++i) tma_load_3d(p + L_KQ + (2 * i + 1) * PANEL, &tmq, bar, 64 * i, h, row);
+        tma_load_3d(p + L_V, &tmv, bar, v0, hv, row);
+        tma_load_3d(p + L_V + PANEL, &tmv, bar, v0 + 64, hv, row);
+        ++issued;
+      }
+      // never leave the block with copies in flight
+      for (int t = (issued > 2 ? issued - 2 : 0); t < issued; ++t) own_copy_wait(&S_.full[t & 1], (t >> 1) & 1, ab, err, 2);
+    }
+  } else if (warp == 13) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const uint32_t id_y = idesc_f16(128, 64, AB16, 0, 0), id_z = idesc_f16(128, 64, AB16, 1, 1);
+      const uint32_t id_d = idesc_f16(128, KD, AB16, 0, 1), id_f = idesc_f16(128, 128, AB16, 0, 1);
+      const uint32_t id_f2 = idesc_f16(128, 64, AB16, 0, 1);
+      for (int t = 0; t < nch; ++t) {
+        const int s = t & 1, ph = t & 1;
+        const uint32_t p = sb + s * L_STAGE;
+        const uint32_t T = p + L_M, P = T + 2 * PANEL;
+        if (!spin_wait(&S_.full[s], (t >> 1) & 1, ab, err, 4)) break;
+        if (t == 0 && part && !spin_wait(&S_.kz, 0, ab, err, 8)) break;
+        // Z^T over the dV of the chunk before
+        if (t > 0 && !spin_wait(&S_.f_read, (t - 1) & 1, ab, err, 0x20)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma(tb + T_Z, sdesc(p + L_DO + ks * 2048, PANEL, 1024), sdesc(P + x * PANEL + ks * 2048, PANEL, 1024), id_z,
+                 x + ks > 0);
+        // Y^T
+        if (!spin_wait(&S_.s_ready, ph, ab, err, 0x10)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int ks = 0; ks < KD / 16; ++ks)
+            umma_ts(tb + T_Y, tb + (x ? T_SL : T_SH) + 8 * ks,
+                    sdesc(p + L_KQ + (ks >> 2) * 2 * PANEL + (ks & 3) * 32, 16, 1024), id_y, x + ks > 0);
+        umma_commit(&S_.y_full);
+        // D^T = (scale Gam dO)^T Q
+        if (!spin_wait(&S_.g_ready, ph, ab, err, 0x40)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma_ts(tb + T_D, tb + (x ? T_GL : T_GH) + 8 * ks, sdesc(p + L_KQ + PANEL + ks * 2048, 2 * PANEL, 1024), id_d,
+                    x + ks > 0);
+        // dV^T = dE^T T; the hi and lo halves are added on reading
+        if (!spin_wait(&S_.e_ready, ph, ab, err, 0x80)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+          umma_ts(tb + T_Y, tb + T_EH + 8 * ks, sdesc(T + ks * 2048, PANEL, 1024), id_f, ks > 0);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_Y, tb + T_EL + 8 * ks, sdesc(T + ks * 2048, PANEL, 1024), id_f2, 1);
+        umma_commit(&S_.f_full);
+        // D^T += (-Gam dV)^T K
+        if (!spin_wait(&S_.f_ready, ph, ab, err, 0x200)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma_ts(tb + T_D, tb + (x ? T_EL : T_EH) + 8 * ks, sdesc(p + L_KQ + ks * 2048, 2 * PANEL, 1024), id_d, 1);
+        umma_commit(&S_.d_full);
+        umma_commit(&S_.empty[s]);
+      }
+      umma_commit(&S_.done);  // TMEM is freed only after every issued MMA has completed
+      mbar_wait(&S_.done, 0);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ chain: dE, Gam dV, dS
+    constexpr int KH = KD / 2;  // columns of K this thread keeps
+    const int quad = warp & 3, hh = (warp - 4) >> 2;
+    const int vl = quad * 32 + lane;
+    const bool vin = v0 + vl < a.V;
+    const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
+    float S[KH];
+#pragma unroll
+    for (int i = 0; i < KH; ++i) {
+      const int k = KH * hh + i;
+      S[i] = (a.dfinal_state && vin && k < a.K) ? a.dfinal_state[st + (int64_t)k * a.V + v0 + vl] : 0.f;
+    }
+    // dS as the operand of chunk c, and to the workspace
+    auto put_state = [&](int c) {
+      uint16_t* g = w.dS1 + ((sh0 + (int64_t)c * a.HV) * a.V + v0 + vl) * a.K + KH * hh;
+#pragma unroll
+      for (int i = 0; i < KH; i += 16) {
+        uint32_t hi[8], lo[8];
+        split<AB16, 8>(S + i, hi, lo);
+        tmem_st8(tl + T_SH + hh * (KH / 2) + i / 2, hi);
+        tmem_st8(tl + T_SL + hh * (KH / 2) + i / 2, lo);
+        if (vin) {
+          if (KH * hh + i < a.K) *reinterpret_cast<uint4*>(g + i) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          if (KH * hh + i + 8 < a.K) *reinterpret_cast<uint4*>(g + i + 8) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&S_.s_ready);
+    };
+    // <dS, S> at the end of anchor group b, this warp's part
+    const int64_t anchors = gdr_slots(a, C * ANCHOR);
+    auto put_anchor = [&](int b, bool zero) {
+      const int64_t at = (gdr_slot0(a, n, sq, C * ANCHOR) + b) * a.HV + hv;
+      float d = 0.f;
+      if (vin && !zero) {
+        const float* g = w.Sf + at * a.K * a.V + v0 + vl;
+#pragma unroll
+        for (int i = 0; i < KH; ++i)
+          if (KH * hh + i < a.K) d = fmaf(S[i], g[(int64_t)(KH * hh + i) * a.V], d);
+      }
+      d = warp_sum(d);
+      if (lane == 0) w.anchor[((int64_t)blockIdx.y * anchors * a.HV + at) * 8 + warp - 4] = d;
+    };
+    if (nch > 0) {
+      put_state(nch - 1);
+      put_anchor((nch - 1) / ANCHOR, a.dfinal_state == nullptr);
+    }
+    const int i0 = 32 * hh;
+    for (int t = 0; t < nch; ++t) {
+      const int s = t & 1, ph = t & 1, c = nch - 1 - t;
+      const float* ax = reinterpret_cast<const float*>(sm + s * L_STAGE + L_AX);
+      pipe_wait(&S_.full[s], (t >> 1) & 1, ab, err, 0x400);
+      pipe_wait(&S_.y_full, ph, ab, err, 0x800);
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 32; i += 16) {
+        float y[16], z[16];
+        tmem_ld16(tl + T_Y + i0 + i, y);
+        tmem_ld16(tl + T_Z + i0 + i, z);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + i + j);
+          const float bb[4] = {b.x, b.y, b.z, b.w};
+          fma2(z + j, bb, y + j, z + j);
+          fma2(z + j + 2, bb + 2, y + j + 2, z + j + 2);
+        }
+        st_split16<AB16>(tl + T_EH + 16 * hh + i / 2, tl + T_EL + 16 * hh + i / 2, z);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&S_.e_ready);
+      pipe_wait(&S_.f_full, ph, ab, err, 0x1000);
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 32; i += 16) {
+        float x[16], y[16];
+        tmem_ld16(tl + T_Y + i0 + i, x);
+        tmem_ld16(tl + T_Y + 64 + i0 + i, y);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(ax + AX_G + i0 + i + j);
+          const float bb[4] = {-b.x, -b.y, -b.z, -b.w};
+          add2f(x + j, x + j, y + j);
+          add2f(x + j + 2, x + j + 2, y + j + 2);
+          mul2f(x + j, x + j, bb);
+          mul2f(x + j + 2, x + j + 2, bb + 2);
+        }
+        st_split16<AB16>(tl + T_EH + 16 * hh + i / 2, tl + T_EL + 16 * hh + i / 2, x);
+      }
+      const float gam[2] = {ax[AX_GC], ax[AX_GC]};
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&S_.f_ready);
+      warp_arrive(&S_.empty[s]);
+      pipe_wait(&S_.d_full, ph, ab, err, 0x2000);
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < KH; i += 16) {
+        float x[16];
+        tmem_ld16(tl + T_D + KH * hh + i, x);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) fma2(S + i + j, gam, S + i + j, x + j);
+      }
+      if (c > 0) put_state(c - 1);
+      if (c > 0 && c % ANCHOR == 0) put_anchor(c / ANCHOR - 1, false);
+    }
+    if (a.dinitial_state && vin) {
+#pragma unroll
+      for (int i = 0; i < KH; ++i) {
+        const int k = KH * hh + i;
+        if (k < a.K) a.dinitial_state[st + (int64_t)k * a.V + v0 + vl] = S[i];
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ output: scaled dO, dV, V . dV
+    const int vl = warp * 32 + lane;
+    const uint32_t tl = tb + ((uint32_t)(warp * 32) << 16);
+    const int64_t slots = gdr_slots(a, C);
+    for (int t = 0; t < nch; ++t) {
+      const int s = t & 1, ph = t & 1, c = nch - 1 - t;
+      const int valid = min(C, sq.len - c * C);
+      const uint32_t p = sb + s * L_STAGE;
+      const float* ax = reinterpret_cast<const float*>(sm + s * L_STAGE + L_AX);
+      const int64_t row0 = sq.bos + (int64_t)c * C;
+      pipe_wait(&S_.full[s], (t >> 1) & 1, ab, err, 0x4000);
+      if (valid < C) {
+        // the rows past the document belong to another one: what a product sums over must be zero
+        for (int i = 0; i < 2 * NP; ++i) zero_rows(p + L_KQ + i * PANEL, 1, valid, threadIdx.x, 128);
+        zero_rows(p + L_DO, 2, valid, threadIdx.x, 128);
+        fence_async_smem();
+        warp_arrive(&S_.kz);
+      }
+      if (t > 0) pipe_wait(&S_.d_full, (t - 1) & 1, ab, err, 0x8000);  // the operand of the chunk before is read
+      tc_fence_after();
+      {
+        const Column D(p + L_DO, vl);
+#pragma unroll
+        for (int i = 0; i < 64; i += 16) {
+          float x[16];
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(ax + AX_SG + i + j);
+            const float bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[j + e] = i + j + e < valid ? bb[e] * h2f<AB16>(lds16(D.at(i + j + e))) : 0.f;
+          }
+          st_split16<AB16>(tl + T_GH + i / 2, tl + T_GL + i / 2, x);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      warp_arrive(&S_.g_ready);
+      float y[64];
+      pipe_wait(&S_.f_full, ph, ab, err, 0x10000);
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 64; i += 16) {
+        float x[16];
+        tmem_ld16(tl + T_Y + i, y + i);
+        tmem_ld16(tl + T_Y + 64 + i, x);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) add2f(y + i + j, y + i + j, x + j);
+      }
+      tc_fence_before();
+      warp_arrive(&S_.f_read);
+      if (threadIdx.x == 0) bulk_wait_read();  // the stores of the chunk before have read the tile
+      bar_sync<1, 128>();
+      const Column O(sb + L_OUT, vl), V(p + L_V, vl);
+#pragma unroll
+      for (int i = 0; i < 64; ++i) sts16(O.at(i), f2h<AB16>(y[i]));
+#pragma unroll
+      for (int i = 0; i < 64; ++i) y[i] = i < valid ? y[i] * h2f<AB16>(lds16(V.at(i))) : 0.f;
+      warp_arrive(&S_.empty[s]);
+      lane_sums<64>(y, lane);
+      S_.red[warp][2 * lane] = y[0];
+      S_.red[warp][2 * lane + 1] = y[1];
+      fence_async_smem();
+      bar_sync<1, 128>();
+      if (valid == C) {
+        if (threadIdx.x == 0) {
+          tma_store_3d(&tmdv, sm + L_OUT, v0, hv, (int)row0);
+          if (v0 + 64 < a.V) tma_store_3d(&tmdv, sm + L_OUT + PANEL, v0 + 64, hv, (int)row0);
+          bulk_commit();
+        }
+      } else {
+        copy_rows(sb + L_OUT, reinterpret_cast<uint16_t*>(a.dv), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, 128);
+      }
+      if (threadIdx.x < C) {
+        const int i = threadIdx.x;
+        w.dotV[((int64_t)blockIdx.y * slots * a.HV + sh0 + (int64_t)c * a.HV) * C + i] =
+            S_.red[0][i] + S_.red[1][i] + S_.red[2][i] + S_.red[3][i];
+      }
+      bar_sync<1, 128>();  // the sums are read before the next chunk's are written
+    }
+    if (threadIdx.x == 0) bulk_wait_all();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 13) tmem_dealloc(tb, 512);
+}
+
+template <int AB16, int KD>
+cudaError_t launch(const GdrArgs& a, const Ws& w) {
+  CUtensorMap q, k, v, o, dv;
+  cudaError_t e = token_map(&q, a, a.q, a.H, a.K);
+  if (e == cudaSuccess) e = token_map(&k, a, a.k, a.H, a.K);
+  if (e == cudaSuccess) e = token_map(&v, a, a.v, a.HV, a.V);
+  if (e == cudaSuccess) e = token_map(&o, a, a.d_o, a.HV, a.V);
+  if (e == cudaSuccess) e = token_map(&dv, a, a.dv, a.HV, a.V);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(rscan_kernel<AB16, KD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L_BYTES);
+  if (e != cudaSuccess) return e;
+  rscan_kernel<AB16, KD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), THREADS, L_BYTES, a.stream>>>(q, k, v, o, dv, a, w);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t rscan(const GdrArgs& a, const Ws& w, int* launches) {
+  ++*launches;
+  const bool small = a.K <= 64;
+  if (a.dtype == DT_BF16) return small ? launch<1, 64>(a, w) : launch<1, 128>(a, w);
+  return small ? launch<0, 64>(a, w) : launch<0, 128>(a, w);
+}
+
+}  // namespace gdrtc
+}  // namespace ccq

@@ -16,7 +16,8 @@
 // The rest of a chunk's period is instructions of the chain warps between the products, so V enters by an MMA
 // of its own (beside the chain) and the factors by packed two-value arithmetic.
 //
-// BWD: instead of O it writes what the backward reads: S0 (16-bit, transposed), E (16-bit) and dO . O.
+// BWD: instead of O it writes what the backward reads: S0 (16-bit, transposed), E (16-bit), dO . O and,
+// every ANCHOR chunks, S in fp32.
 //
 // Warps (448 threads): 0-3 output (one per TMEM quadrant), 4-11 chain (two per quadrant, each half of the
 // columns), 12 TMA, 13 MMA.  TMEM columns: S hi, S lo (64 each), X | Y, then dS (128), E, then E P^T
@@ -272,6 +273,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int j = 0; j < 16; j += 2) fma2(S + i + j, gam, S + i + j, x + j);
       }
       if (c + 1 < nch) put_state(c + 1);
+      if (BWD && vin && ((c + 1) % ANCHOR == 0 || c + 1 == nch)) {
+        float* g = w.Sf + ((gdr_slot0(a, n, sq, C * ANCHOR) + c / ANCHOR) * a.HV + hv) * a.K * a.V + v0 + vl;
+#pragma unroll
+        for (int i = 0; i < KH; ++i)
+          if (KH * hh + i < a.K) g[(int64_t)(KH * hh + i) * a.V] = S[i];
+      }
     }
     if (!BWD && a.final_state && vin) {
 #pragma unroll
