@@ -42,7 +42,7 @@ struct Ws {
   // backward only
   uint16_t* S0;        // [slots * HV][V][K] state before the chunk, transposed, 16-bit
   uint16_t* dS1;       // [slots * HV][V][K] gradient of the state after it
-  uint16_t* E;         // [slots * HV][C][V]
+  uint16_t* E;         // [slots * HV][V][C] E transposed, 16-bit
   float* dotO;         // [V tiles][slots * HV][C]: dO . O
   float* dotV;         // [V tiles][slots * HV][C]: V . dV
   float* Sf;           // [slots of 512 * HV][K][V] fp32 state after every ANCHOR chunks and after the last one
@@ -217,6 +217,34 @@ __device__ __forceinline__ void lane_sums(float* x, int lane) {
       x[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
     }
   }
+}
+
+// 64 16-bit values of row `row` (32 packed words) into a swizzled panel of 128 rows
+__device__ __forceinline__ void stage_row(uint32_t panel, int row, const float* r) {
+  const uint32_t* u = reinterpret_cast<const uint32_t*>(r);
+#pragma unroll
+  for (int ch = 0; ch < 8; ++ch)
+    sts128(panel + tc::sw128(row, ch), make_uint4(u[4 * ch], u[4 * ch + 1], u[4 * ch + 2], u[4 * ch + 3]));
+}
+// such a panel to a [V][width] matrix of (chunk, value head) sh, columns from x, by one thread
+__device__ __forceinline__ void store_panel(const CUtensorMap* m, const uint8_t* panel, int x, int v0, int V, int64_t sh) {
+  tc::tma_store_3d(m, panel, x, v0, (int)sh);
+  if (v0 + 64 < V) tc::tma_store_3d(m, panel + PANEL, x, v0 + 64, (int)sh);
+  tc::bulk_commit();
+}
+
+// [n][V][width] matrices (the saved states and E), box 64 of width x 64 of V
+inline cudaError_t matrix_map(CUtensorMap* m, const GdrArgs& a, const void* p, int width, int64_t n) {
+  auto fn = tc::encode_fn();
+  if (fn == nullptr) return cudaErrorNotSupported;
+  cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)a.V, (cuuint64_t)n};
+  cuuint64_t strides[2] = {(cuuint64_t)width * 2, (cuuint64_t)width * a.V * 2};
+  cuuint32_t box[3] = {64, 64, 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  CUresult r = fn(m, a.dtype == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void*>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
 inline cudaError_t token_map(CUtensorMap* m, const GdrArgs& a, const void* p, int heads, int width) {

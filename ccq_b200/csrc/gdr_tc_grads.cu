@@ -25,14 +25,6 @@ constexpr uint32_t L_B = 8 * PANEL;                // two steps
 constexpr uint32_t L_W = L_B + 2 * B_SIZE, L_N = L_W + PANEL;
 constexpr uint32_t L_AX = L_N + PANEL;             // two
 constexpr uint32_t AX_BYTES = (AX_N * 4 + 127) & ~127u;
-struct Small {
-  uint64_t full[2];
-  float ke[4][C], db[4][C], dg[3];
-  int abort;
-};
-constexpr uint32_t L_SMALL = L_AX + 2 * AX_BYTES;
-constexpr uint32_t BYTES = L_SMALL + sizeof(Small) + 1024;
-static_assert(BYTES <= 232448, "shared memory");
 
 __device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -75,35 +67,51 @@ __device__ __forceinline__ uint32_t bt_addr(uint32_t panel, int k0, int c0, int 
   return panel + sw128(k0 + (lane & 15), c0 + (lane >> 4));
 }
 
-// Walks the items of a block and their steps.
+// One step as the block's warps see it, written by thread 0 two steps ahead.
+struct Step {
+  int live, hv, h, row0, valid, first_v, last_v, first, last, qk, ax, more, zero_first;
+  int64_t sh, anchor;
+};
+
+__device__ __forceinline__ int nvt128(const GdrArgs& a) { return (a.V + VT - 1) / VT; }
+
+// The position of the next step to load (thread 0's; in shared memory to spare the others its registers).
 struct Walk {
-  int64_t item;       // slot * H + key head
-  int n, c, h, g, vt;
+  int item, items, count, n, c, g, vt, loaded;  // item = slot * H + key head
   Seq sq;
-  int count;          // items seen so far
   bool live;
-  __device__ __forceinline__ void find(const GdrArgs& a, int64_t items) {
-    for (; item < items; item += gridDim.x) {
-      h = (int)(item % a.H);
+  __device__ __forceinline__ void find(const GdrArgs& a) {
+    for (; item < items; item += gridDim.x)
       if (gdr_slot_find(a, item / a.H, C, &n, &c, &sq)) {
         live = true;
         g = vt = 0;
         return;
       }
-    }
     live = false;
   }
-  __device__ __forceinline__ void next(const GdrArgs& a, int64_t items, int group, int nvt) {
+  __device__ __forceinline__ void next(const GdrArgs& a, int group, int nvt) {
     if (++vt < nvt) return;
     vt = 0;
     if (++g < group) return;
     item += gridDim.x;
     ++count;
-    find(a, items);
+    find(a);
   }
 };
 
-template <int AB16, int KD>
+struct Small {
+  uint64_t full[2];
+  Step step[2];
+  Walk walk;
+  float ke[4][C], db[4][C], dg[17];
+  int abort;
+};
+constexpr uint32_t L_SMALL = L_AX + 2 * AX_BYTES;
+constexpr uint32_t BYTES = L_SMALL + sizeof(Small) + 1024;
+static_assert(BYTES <= 232448, "shared memory");
+
+// ONE: a key head serves one value head, so nothing is carried from one value head to the next
+template <int AB16, int KD, bool ONE>
 __global__ void __launch_bounds__(THREADS, 1)
     grads_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                  const __grid_constant__ CUtensorMap tmo, const __grid_constant__ CUtensorMap tmdv,
@@ -118,8 +126,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int mt = warp >> 2, nq = warp & 3;  // rows 16 mt.., columns KD / 4 nq.. of K (16 nq.. of the 64 x 64 products)
   const int g = lane >> 2, tq = lane & 3;
   constexpr int NP = KD / 64, NT = KD / 32;  // panels of K; 8-column tiles of K a warp holds
-  const int64_t slots = gdr_slots(a, C), items = slots * a.H;
-  const int group = a.HV / a.H, nvt = (a.V + 63) / 64, nvt128 = (a.V + VT - 1) / VT;
+  const int group = a.HV / a.H, nvt = (a.V + 63) / 64;
   if (tid == 0) {
     mbar_init(&S_.full[0], 1);
     mbar_init(&S_.full[1], 1);
@@ -127,88 +134,103 @@ __global__ void __launch_bounds__(THREADS, 1)
     fence_barrier_init();
   }
   __syncthreads();
-  Walk it, pf;
-  it.item = blockIdx.x;
-  it.count = 0;
-  it.find(a, items);
-  pf = it;
-  int64_t loaded = 0;
-  // thread 0: the loads of step `loaded`, at pf
+  Walk& pf = S_.walk;
+  // thread 0: describes and loads the next step
   auto load = [&]() {
+    const int b = pf.loaded & 1;
+    Step& s = S_.step[b];
+    s.live = pf.live;
     if (!pf.live) return;
-    const int b = (int)(loaded & 1);
-    uint64_t* bar = &S_.full[b];
-    uint8_t* p = sm + L_B + b * B_SIZE;
-    const int hv = pf.h * group + pf.g;
-    const int64_t slot = pf.item / a.H, sh = slot * a.HV + hv;
-    const int row = (int)(pf.sq.bos + (int64_t)pf.c * C);
-    const bool first = pf.vt == 0, qk = first && pf.g == 0;
-    if (tid == 0) {
-      mbar_arrive_expect_tx(bar, 2 * NP * PANEL + 3 * PANEL + (first ? AX_N * 4 : 0) + (qk ? 2 * NP * PANEL : 0));
-      if (qk) {
-        uint8_t* d = sm + L_QK + (pf.count & 1) * 4 * PANEL;
+    {
+      uint64_t* bar = &S_.full[b];
+      uint8_t* p = sm + L_B + b * B_SIZE;
+      const int slot = pf.item / a.H, h = pf.item - slot * a.H, hv = h * group + pf.g;
+      const int64_t sh = (int64_t)slot * a.HV + hv;
+      const int row = (int)(pf.sq.bos + (int64_t)pf.c * C);
+      const int nch = (pf.sq.len + C - 1) / C;
+      s.hv = hv;
+      s.h = h;
+      s.row0 = row;
+      s.valid = min(C, pf.sq.len - pf.c * C);
+      s.first_v = pf.vt == 0;
+      s.last_v = pf.vt == nvt - 1;
+      s.first = s.first_v && pf.g == 0;
+      s.last = s.last_v && pf.g == group - 1;
+      s.qk = pf.count & 1;
+      s.ax = (pf.count * group + pf.g) & 1;
+      s.more = min(ANCHOR - 1 - pf.c % ANCHOR, nch - 1 - pf.c);
+      s.zero_first = pf.c == 0 && a.initial_state == nullptr;
+      s.sh = sh;
+      s.anchor = (gdr_slot0(a, pf.n, pf.sq, C * ANCHOR) + pf.c / ANCHOR) * a.HV + hv;
+      mbar_arrive_expect_tx(bar, 2 * NP * PANEL + 3 * PANEL + (s.first_v ? AX_N * 4 : 0) + (s.first ? 2 * NP * PANEL : 0));
+      if (s.first) {
+        uint8_t* d = sm + L_QK + s.qk * 4 * PANEL;
         for (int i = 0; i < NP; ++i) {
-          tma_load_3d(d + i * PANEL, &tmq, bar, 64 * i, pf.h, row);
-          tma_load_3d(d + (2 + i) * PANEL, &tmk, bar, 64 * i, pf.h, row);
+          tma_load_3d(d + i * PANEL, &tmq, bar, 64 * i, h, row);
+          tma_load_3d(d + (2 + i) * PANEL, &tmk, bar, 64 * i, h, row);
         }
       }
-      if (first) bulk_load(sm + L_AX + ((pf.count * group + pf.g) & 1) * AX_BYTES, w.aux + sh * AX_N, AX_N * 4, bar);
+      if (s.first_v) bulk_load(sm + L_AX + s.ax * AX_BYTES, w.aux + sh * AX_N, AX_N * 4, bar);
       tma_load_3d(p + B_DO, &tmo, bar, 64 * pf.vt, hv, row);
       tma_load_3d(p + B_DV, &tmdv, bar, 64 * pf.vt, hv, row);
-      tma_load_3d(p + B_E, &tme, bar, 64 * pf.vt, 0, (int)(sh * C));
+      tma_load_3d(p + B_E, &tme, bar, 0, 64 * pf.vt, (int)sh);
       for (int i = 0; i < NP; ++i) {
         tma_load_3d(p + B_S + i * PANEL, &tms, bar, 64 * i, 64 * pf.vt, (int)sh);
         tma_load_3d(p + B_DS + i * PANEL, &tmds, bar, 64 * i, 64 * pf.vt, (int)sh);
       }
     }
-    ++loaded;
-    pf.next(a, items, group, nvt);
+    ++pf.loaded;
+    pf.next(a, group, nvt);
   };
-  load();
-  load();
-  float dq[NT][4], dk[NT][4];
+  if (tid == 0) {
+    pf.loaded = 0;
+    pf.items = (int)(gdr_slots(a, C) * a.H);
+    pf.item = blockIdx.x;
+    pf.count = 0;
+    pf.find(a);
+    load();
+    load();
+  }
+  __syncthreads();
+  float dq[NT][4], dk[NT][4];  // ONE: dO S0^T and dV S0^T grow into them
   float xq[NT][4], xv[NT][4], xe[NT][4], pe[2][4], ve[2][4];  // dO S0^T, dV S0^T, E dS1^T, dO E^T, dV E^T
   float dot = 0.f, later = 0.f;
-  for (int64_t step = 0; it.live; ++step) {
-    const int b = (int)(step & 1);
-    const int hv = it.h * group + it.g;
-    const int64_t slot = it.item / a.H, sh = slot * a.HV + hv;
-    const int t0 = it.c * C, valid = min(C, it.sq.len - t0);
-    const int64_t row0 = it.sq.bos + t0;
+  for (int step = 0;; ++step) {
+    const int b = step & 1;
+    const Step& s = S_.step[b];
+    if (!s.live) break;
+    // what is read after the step's last barrier, when thread 0 may already describe the step after the next
+    const int valid = s.valid, row0 = s.row0, head = s.h;
+    const bool last = s.last;
     const uint32_t p = sb + L_B + b * B_SIZE;
-    const uint32_t Q = sb + L_QK + (it.count & 1) * 4 * PANEL, K = Q + 2 * PANEL;
-    const float* ax = reinterpret_cast<const float*>(sm + L_AX + ((it.count * group + it.g) & 1) * AX_BYTES);
-    if (it.vt == 0) {
+    const uint32_t Q = sb + L_QK + s.qk * 4 * PANEL, K = Q + 2 * PANEL;
+    const float* ax = reinterpret_cast<const float*>(sm + L_AX + s.ax * AX_BYTES);
+    if (s.first_v) {
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           xq[i][j] = xv[i][j] = xe[i][j] = 0.f;
-          if (it.g == 0) dq[i][j] = dk[i][j] = 0.f;
+          if (!ONE && s.first) dq[i][j] = dk[i][j] = 0.f;
         }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) pe[i][j] = ve[i][j] = 0.f;
+      // dO . O - V . dV: of this chunk's tokens in warps 0 and 1, of the chunks up to the next anchor in the
+      // others; and <dS, S> there
       dot = later = 0.f;
-      if (tid < C) {
-        // dO . O - V . dV of this chunk's token, and of the chunks up to the next anchor; then <dS, S> there
-        const int nch = (it.sq.len + C - 1) / C, more = min(ANCHOR - 1 - it.c % ANCHOR, nch - 1 - it.c);
-        const int64_t anchors = gdr_slots(a, C * ANCHOR);
-        const int64_t an = (gdr_slot0(a, it.n, it.sq, C * ANCHOR) + it.c / ANCHOR) * a.HV + hv;
-        for (int v = 0; v < nvt128; ++v) {
-          const int64_t at = ((int64_t)v * slots * a.HV + sh) * C + tid;
+      const int64_t vs = gdr_slots(a, C) * a.HV, va = gdr_slots(a, C * ANCHOR) * a.HV;
+      for (int v = 0; v < nvt128(a); ++v) {
+        if ((tid >> 6) <= s.more) {
+          const int64_t at = (v * vs + s.sh + (int64_t)(tid >> 6) * a.HV) * C + (tid & 63);
           dot += w.dotO[at] - w.dotV[at];
-          for (int i = 1; i <= more; ++i) {
-            const int64_t x = at + (int64_t)i * a.HV * C;
-            later += w.dotO[x] - w.dotV[x];
-          }
-          if (tid < 8) later += w.anchor[((int64_t)v * anchors * a.HV + an) * 8 + tid];
         }
+        if (tid < 8) later += w.anchor[(v * va + s.anchor) * 8 + tid];
       }
     }
-    pipe_wait(&S_.full[b], (uint32_t)(step >> 1) & 1, &S_.abort, w.err, 0x200000);
-    if (valid < C && it.vt == 0 && it.g == 0) {
+    pipe_wait(&S_.full[b], (step >> 1) & 1, &S_.abort, w.err, 0x200000);
+    if (valid < C && s.first) {
       // the rows past the document belong to another one: what a product sums over must be zero
       for (int i = 0; i < NP; ++i) {
         zero_rows(Q + i * PANEL, 1, valid, tid, THREADS);
@@ -216,13 +238,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       __syncthreads();
     }
-#pragma unroll
+#pragma unroll 1
     for (int ks = 0; ks < 4; ++ks) {
       uint32_t fo[4], fv[4], fe[4], be[4];
       ldsm4(fo, a_addr(p + B_DO, 16 * mt, 2 * ks, lane));
       ldsm4(fv, a_addr(p + B_DV, 16 * mt, 2 * ks, lane));
-      ldsm4(fe, a_addr(p + B_E, 16 * mt, 2 * ks, lane));
-      ldsm4(be, b_addr(p + B_E, 16 * nq, 2 * ks, lane));
+      ldsm4t(fe, at_addr(p + B_E, 16 * ks, 2 * mt, lane));
+      ldsm4t(be, bt_addr(p + B_E, 16 * ks, 2 * nq, lane));
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         mma16<AB16>(pe[j], fo, be[2 * j], be[2 * j + 1]);
@@ -242,12 +264,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         mma16<AB16>(xe[2 * j + 1], fe, bd[2], bd[3]);
       }
     }
-    const bool last_v = it.vt == nvt - 1, last = last_v && it.g == group - 1;
-    if (last_v) {
+    if (s.last_v) {
       // q k^T and k k^T of this warp's 16 x 16 tile, where it reaches the lower triangle
       float qk[2][4] = {}, kk[2][4] = {};
       if (nq <= mt) {
-#pragma unroll
+#pragma unroll 1
         for (int ks = 0; ks < KD / 16; ++ks) {
           uint32_t fq[4], fk[4], bk[4];
           const uint32_t pan = (ks >> 2) * PANEL;
@@ -306,8 +327,10 @@ __global__ void __launch_bounds__(THREADS, 1)
           ke[hr] = fmaf(kf.x, xe[j][2 * hr], fmaf(kf.y, xe[j][2 * hr + 1], ke[hr]));
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            dq[j][2 * hr + e] = fmaf(ax[AX_SG + i], xq[j][2 * hr + e], dq[j][2 * hr + e]);
-            dk[j][2 * hr + e] += ax[AX_WB + i] * xe[j][2 * hr + e] - ax[AX_G + i] * xv[j][2 * hr + e];
+            const float x = ax[AX_SG + i] * xq[j][2 * hr + e];
+            const float y = ax[AX_WB + i] * xe[j][2 * hr + e] - ax[AX_G + i] * xv[j][2 * hr + e];
+            dq[j][2 * hr + e] = ONE ? x : dq[j][2 * hr + e] + x;
+            dk[j][2 * hr + e] = ONE ? y : dk[j][2 * hr + e] + y;
           }
         }
       }
@@ -317,9 +340,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         ke[hr] += __shfl_xor_sync(0xffffffffu, ke[hr], 2);
         if (tq == 0) S_.ke[nq][i0 + 8 * hr] = ke[hr];
       }
+      {
+        const float r = warp_sum(warp < 2 ? later : dot + later);
+        if (lane == 0) S_.dg[warp] = r;
+      }
       __syncthreads();
       // W K, W^T Q, N K, N^T K
-#pragma unroll
+#pragma unroll 1
       for (int ks = 0; ks < 4; ++ks) {
         uint32_t fw[4], fwt[4], fn[4], fnt[4];
         ldsm4(fw, a_addr(sb + L_W, 16 * mt, 2 * ks, lane));
@@ -345,23 +372,24 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int j = tid;
         const float ke4 = S_.ke[0][j] + S_.ke[1][j] + S_.ke[2][j] + S_.ke[3][j];
         if (j < valid)
-          gate_store(a.dbeta, a.beta_dtype, (row0 + j) * a.HV + hv,
+          gate_store(a.dbeta, a.beta_dtype, (int64_t)(s.row0 + j) * a.HV + s.hv,
                      S_.db[0][j] + S_.db[1][j] + S_.db[2][j] + S_.db[3][j] + ax[AX_W + j] * ke4);
         // dg: reverse running sum; warp 1 holds tokens 32..63, whose sum warp 0 adds
-        float s = dot;
+        float r = dot;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const float u = __shfl_down_sync(0xffffffffu, s, o);
-          if (lane + o < 32) s += u;
+          const float u = __shfl_down_sync(0xffffffffu, r, o);
+          if (lane + o < 32) r += u;
         }
-        const float rest = warp_sum(later);
-        if (lane == 0) S_.dg[warp] = rest;
-        if (lane == 0 && warp == 1) S_.dg[2] = s;
+        if (lane == 0 && warp == 1) S_.dg[16] = r;
         bar_sync<2, 64>();
-        s += S_.dg[0] + S_.dg[1] + (warp == 0 ? S_.dg[2] : 0.f);
+        float rest = S_.dg[lane & 15];
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+        r += rest + (warp == 0 ? S_.dg[16] : 0.f);
         // nothing decays at the first token of a document that starts from a zero state
-        if (t0 + j == 0 && a.initial_state == nullptr) s = 0.f;
-        if (j < valid) gate_store(a.dg, a.g_dtype, (row0 + j) * a.HV + hv, s);
+        if (j == 0 && s.zero_first) r = 0.f;
+        if (j < valid) gate_store(a.dg, a.g_dtype, (int64_t)(s.row0 + j) * a.HV + s.hv, r);
       }
     }
     __syncthreads();  // the step's tiles, W, N and, after the last step, Q and K have been read
@@ -383,39 +411,26 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (tid == 0) {
           for (int i = 0; i < NP; ++i)
             if (64 * i < a.K) {
-              tma_store_3d(&tmdq, sm + (Q - sb) + i * PANEL, 64 * i, it.h, (int)row0);
-              tma_store_3d(&tmdk, sm + (K - sb) + i * PANEL, 64 * i, it.h, (int)row0);
+              tma_store_3d(&tmdq, sm + (Q - sb) + i * PANEL, 64 * i, head, row0);
+              tma_store_3d(&tmdk, sm + (K - sb) + i * PANEL, 64 * i, head, row0);
             }
           bulk_commit();
           bulk_wait_read();
         }
       } else {
-        copy_rows(Q, reinterpret_cast<uint16_t*>(a.dq), row0, a.H, it.h, a.K, 0, valid, tid, THREADS);
-        copy_rows(K, reinterpret_cast<uint16_t*>(a.dk), row0, a.H, it.h, a.K, 0, valid, tid, THREADS);
+        copy_rows(Q, reinterpret_cast<uint16_t*>(a.dq), row0, a.H, head, a.K, 0, valid, tid, THREADS);
+        copy_rows(K, reinterpret_cast<uint16_t*>(a.dk), row0, a.H, head, a.K, 0, valid, tid, THREADS);
         __syncthreads();
       }
     }
-    load();
-    it.next(a, items, group, nvt);
+    // the step is done: its description and buffers go to the one after the next.  A last step's dq and dk
+    // have left Q and K (thread 0 waited); the barrier at the end of the next step publishes the description.
+    if (tid == 0) load();
   }
   if (tid == 0) bulk_wait_all();
 }
 
-// The tile of one (chunk, value head) of the saved states: [V][K] per sh, box 64 of K x 64 of V
-cudaError_t state_map(CUtensorMap* m, const GdrArgs& a, const void* p, int64_t n) {
-  auto fn = tc::encode_fn();
-  if (fn == nullptr) return cudaErrorNotSupported;
-  cuuint64_t dims[3] = {(cuuint64_t)a.K, (cuuint64_t)a.V, (cuuint64_t)n};
-  cuuint64_t strides[2] = {(cuuint64_t)a.K * 2, (cuuint64_t)a.K * a.V * 2};
-  cuuint32_t box[3] = {64, 64, 1};
-  cuuint32_t es[3] = {1, 1, 1};
-  CUresult r = fn(m, a.dtype == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                  const_cast<void*>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
-}
-
-template <int AB16, int KD>
+template <int AB16, int KD, bool ONE>
 cudaError_t launch(const GdrArgs& a, const Ws& w) {
   const int64_t slots = gdr_slots(a, C), sh = slots * a.HV;
   CUtensorMap q, k, o, dv, e, s, ds, dq, dk;
@@ -423,26 +438,31 @@ cudaError_t launch(const GdrArgs& a, const Ws& w) {
   if (r == cudaSuccess) r = token_map(&k, a, a.k, a.H, a.K);
   if (r == cudaSuccess) r = token_map(&o, a, a.d_o, a.HV, a.V);
   if (r == cudaSuccess) r = token_map(&dv, a, a.dv, a.HV, a.V);
-  if (r == cudaSuccess) r = tc::make_token_map(&e, w.E, sh * C, 1, a.V, C, a.dtype == DT_BF16);
-  if (r == cudaSuccess) r = state_map(&s, a, w.S0, sh);
-  if (r == cudaSuccess) r = state_map(&ds, a, w.dS1, sh);
+  if (r == cudaSuccess) r = matrix_map(&e, a, w.E, C, sh);
+  if (r == cudaSuccess) r = matrix_map(&s, a, w.S0, a.K, sh);
+  if (r == cudaSuccess) r = matrix_map(&ds, a, w.dS1, a.K, sh);
   if (r == cudaSuccess) r = token_map(&dq, a, a.dq, a.H, a.K);
   if (r == cudaSuccess) r = token_map(&dk, a, a.dk, a.H, a.K);
-  if (r == cudaSuccess) r = cudaFuncSetAttribute(grads_kernel<AB16, KD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BYTES);
+  if (r == cudaSuccess) r = cudaFuncSetAttribute(grads_kernel<AB16, KD, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BYTES);
   if (r != cudaSuccess) return r;
   const int64_t items = slots * a.H;
   const unsigned grid = (unsigned)(items < 148 ? items : 148);  // one persistent block per SM
-  grads_kernel<AB16, KD><<<grid, THREADS, BYTES, a.stream>>>(q, k, o, dv, e, s, ds, dq, dk, a, w);
+  grads_kernel<AB16, KD, ONE><<<grid, THREADS, BYTES, a.stream>>>(q, k, o, dv, e, s, ds, dq, dk, a, w);
   return cudaGetLastError();
+}
+
+template <int AB16>
+cudaError_t pick(const GdrArgs& a, const Ws& w) {
+  const bool one = a.H == a.HV;
+  if (a.K <= 64) return one ? launch<AB16, 64, true>(a, w) : launch<AB16, 64, false>(a, w);
+  return one ? launch<AB16, 128, true>(a, w) : launch<AB16, 128, false>(a, w);
 }
 
 }  // namespace
 
 cudaError_t grads(const GdrArgs& a, const Ws& w, int* launches) {
   ++*launches;
-  const bool small = a.K <= 64;
-  if (a.dtype == DT_BF16) return small ? launch<1, 64>(a, w) : launch<1, 128>(a, w);
-  return small ? launch<0, 64>(a, w) : launch<0, 128>(a, w);
+  return a.dtype == DT_BF16 ? pick<1>(a, w) : pick<0>(a, w);
 }
 
 }  // namespace gdrtc

@@ -81,18 +81,20 @@ struct Small {
   float gh[C], gl[C], beta[C];  // G log2(e) as hi + lo
 };
 
-constexpr uint32_t OFF_A = MATS;                        // the rows' space (up to 32 KB) becomes the image of the matrices
-constexpr uint32_t OFF_X = OFF_A + C * LDA * 4;         // [32][36]
+// The rows (up to 32 KB) make room, once read, for A and for the images of P; the images of T then replace
+// A.  41 KB in all: five blocks on an SM.
+constexpr uint32_t OFF_P = (C * LDA * 4 + 1023) & ~1023u;
+constexpr uint32_t OFF_X = OFF_P + 2 * PANEL;           // [32][36]
 constexpr uint32_t OFF_S = OFF_X + 32 * 36 * 4;
 constexpr uint32_t BYTES = OFF_S + sizeof(Small) + 1024;
-static_assert(2 * TILE <= MATS, "rows fit the image");
+static_assert(2 * TILE <= OFF_X, "rows fit");
 
 template <int AB16, int KD>
 __global__ void __launch_bounds__(128)
     prep_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk, GdrArgs a, Ws w) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* A = reinterpret_cast<float*>(sm + OFF_A);  // [C][LDA]: A, then T
+  float* A = reinterpret_cast<float*>(sm);  // [C][LDA]: A, then T
   float* X = reinterpret_cast<float*>(sm + OFF_X);
   Small& S = *reinterpret_cast<Small*>(sm + OFF_S);
   const int64_t slot = blockIdx.x;
@@ -180,7 +182,7 @@ __global__ void __launch_bounds__(128)
       }
     }
   }
-  __syncthreads();  // the rows are read: their space becomes the image of the four matrices
+  __syncthreads();  // the rows are read: their space becomes A and the images of P
   {
     const int i0 = 16 * warp + (lane >> 2);
     const float gh[2] = {S.gh[i0], S.gh[i0 + 8]}, gl[2] = {S.gl[i0], S.gl[i0 + 8]};
@@ -191,8 +193,8 @@ __global__ void __launch_bounds__(128)
 #pragma unroll
         for (int hr = 0; hr < 2; ++hr) {
           const uint32_t at = sw128(i0 + 8 * hr, nt) + (lane & 3) * 4;
-          *reinterpret_cast<uint32_t*>(sm + 2 * PANEL + at) = 0;
-          *reinterpret_cast<uint32_t*>(sm + 3 * PANEL + at) = 0;
+          *reinterpret_cast<uint32_t*>(sm + OFF_P + at) = 0;
+          *reinterpret_cast<uint32_t*>(sm + OFF_P + PANEL + at) = 0;
           *reinterpret_cast<float2*>(A + (i0 + 8 * hr) * LDA + j0) = make_float2(0.f, 0.f);
         }
         continue;
@@ -212,8 +214,8 @@ __global__ void __launch_bounds__(128)
         uint32_t hi, lo;
         split<AB16, 1>(p, &hi, &lo);
         const uint32_t at = sw128(i, nt) + (lane & 3) * 4;
-        *reinterpret_cast<uint32_t*>(sm + 2 * PANEL + at) = hi;
-        *reinterpret_cast<uint32_t*>(sm + 3 * PANEL + at) = lo;
+        *reinterpret_cast<uint32_t*>(sm + OFF_P + at) = hi;
+        *reinterpret_cast<uint32_t*>(sm + OFF_P + PANEL + at) = lo;
       }
     }
   }
@@ -270,24 +272,32 @@ __global__ void __launch_bounds__(128)
   {
     const int i = tid >> 1, half = tid & 1;
     const float* row = A + i * LDA + 32 * half;
+    uint32_t hi[16], lo[16];
 #pragma unroll
     for (int cc = 0; cc < 4; ++cc) {
       const float4 u = *reinterpret_cast<const float4*>(row + 8 * cc), v = *reinterpret_cast<const float4*>(row + 8 * cc + 4);
       const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-      uint32_t hi[4], lo[4];
-      split<AB16, 4>(x, hi, lo);
+      split<AB16, 4>(x, hi + 4 * cc, lo + 4 * cc);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int cc = 0; cc < 4; ++cc) {
       const uint32_t at = sw128(i, 4 * half + cc);
-      *reinterpret_cast<uint4*>(sm + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(sm + PANEL + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      *reinterpret_cast<uint4*>(sm + at) = make_uint4(hi[4 * cc], hi[4 * cc + 1], hi[4 * cc + 2], hi[4 * cc + 3]);
+      *reinterpret_cast<uint4*>(sm + PANEL + at) = make_uint4(lo[4 * cc], lo[4 * cc + 1], lo[4 * cc + 2], lo[4 * cc + 3]);
     }
   }
   fence_async_smem();
   __syncthreads();
   if (tid == 0) {
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(w.mats + sh * MATS), "r"(sk), "r"(MATS)
-                 : "memory");
+    uint8_t* dst = w.mats + sh * MATS;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + i * 2 * PANEL),
+                   "r"(sk + i * OFF_P), "r"(2 * PANEL)
+                   : "memory");
     bulk_commit();
-    bulk_wait_all();
+    bulk_wait_read();  // shared memory must outlive the copy's reads; the writes end with the kernel
   }
 }
 

@@ -25,7 +25,7 @@ constexpr int THREADS = 448;
 constexpr uint32_t T_SH = 0, T_SL = 64, T_Y = 128, T_Z = 192, T_D = 256, T_EH = 384, T_EL = 416, T_GH = 448, T_GL = 480;
 
 struct Small {
-  uint64_t full[2], empty[2], s_ready, y_full, e_ready, f_full, f_ready, f_read, g_ready, d_full, kz, done;
+  uint64_t full[2], empty[2], s_ready, y_full, e_ready, f_full, f_ready, f_read, g_ready, h_read, d_full, kz, done;
   float red[4][C];
   uint32_t tmem;
   int abort;
@@ -41,7 +41,7 @@ template <int AB16, int KD>
 __global__ void __launch_bounds__(THREADS, 1)
     rscan_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                  const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmo,
-                 const __grid_constant__ CUtensorMap tmdv, GdrArgs a, Ws w) {
+                 const __grid_constant__ CUtensorMap tmdv, const __grid_constant__ CUtensorMap tms, GdrArgs a, Ws w) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Small& S_ = *reinterpret_cast<Small*>(sm + L_SMALL);
@@ -65,6 +65,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     mbar_init(&S_.f_ready, 8);
     mbar_init(&S_.f_read, 4);
     mbar_init(&S_.g_ready, 4);
+    mbar_init(&S_.h_read, 4);
     mbar_init(&S_.kz, 4);
     mbar_init(&S_.y_full, 1);
     mbar_init(&S_.f_full, 1);
@@ -184,20 +185,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int k = KH * hh + i;
       S[i] = (a.dfinal_state && vin && k < a.K) ? a.dfinal_state[st + (int64_t)k * a.V + v0 + vl] : 0.f;
     }
-    // dS as the operand of chunk c, and to the workspace
-    auto put_state = [&](int c) {
-      uint16_t* g = w.dS1 + ((sh0 + (int64_t)c * a.HV) * a.V + v0 + vl) * a.K + KH * hh;
+    // dS as the operand of the next chunk
+    auto put_state = [&]() {
 #pragma unroll
-      for (int i = 0; i < KH; i += 16) {
-        uint32_t hi[8], lo[8];
-        split<AB16, 8>(S + i, hi, lo);
-        tmem_st8(tl + T_SH + hh * (KH / 2) + i / 2, hi);
-        tmem_st8(tl + T_SL + hh * (KH / 2) + i / 2, lo);
-        if (vin) {
-          if (KH * hh + i < a.K) *reinterpret_cast<uint4*>(g + i) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if (KH * hh + i + 8 < a.K) *reinterpret_cast<uint4*>(g + i + 8) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-        }
-      }
+      for (int i = 0; i < KH; i += 16)
+        st_split16<AB16>(tl + T_SH + hh * (KH / 2) + i / 2, tl + T_SL + hh * (KH / 2) + i / 2, S + i);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.s_ready);
@@ -217,7 +209,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (lane == 0) w.anchor[((int64_t)blockIdx.y * anchors * a.HV + at) * 8 + warp - 4] = d;
     };
     if (nch > 0) {
-      put_state(nch - 1);
+      put_state();
       put_anchor((nch - 1) / ANCHOR, a.dfinal_state == nullptr);
     }
     const int i0 = 32 * hh;
@@ -276,7 +268,9 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 16; j += 2) fma2(S + i + j, gam, S + i + j, x + j);
       }
-      if (c > 0) put_state(c - 1);
+      pipe_wait(&S_.h_read, ph, ab, err, 0x20000);  // the output warps have dS
+      tc_fence_after();
+      if (c > 0) put_state();
       if (c > 0 && c % ANCHOR == 0) put_anchor(c / ANCHOR - 1, false);
     }
     if (a.dinitial_state && vin) {
@@ -326,6 +320,22 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_before();
       warp_arrive(&S_.g_ready);
       float y[64];
+      // the hi part of dS, to the workspace
+      pipe_wait(&S_.y_full, ph, ab, err, 0x40000);
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < NP; ++i) tmem_ld32(tl + T_SH + 32 * i, y + 32 * i);
+      tc_fence_before();
+      warp_arrive(&S_.h_read);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if (threadIdx.x == 0) bulk_wait_read();
+        bar_sync<1, 128>();
+        stage_row(sb + L_OUT, vl, y + 32 * i);
+        fence_async_smem();
+        bar_sync<1, 128>();
+        if (threadIdx.x == 0 && 64 * i < a.K) store_panel(&tms, sm + L_OUT, 64 * i, v0, a.V, sh0 + (int64_t)c * a.HV);
+      }
       pipe_wait(&S_.f_full, ph, ab, err, 0x10000);
       tc_fence_after();
 #pragma unroll
@@ -377,16 +387,17 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 template <int AB16, int KD>
 cudaError_t launch(const GdrArgs& a, const Ws& w) {
-  CUtensorMap q, k, v, o, dv;
+  CUtensorMap q, k, v, o, dv, st;
   cudaError_t e = token_map(&q, a, a.q, a.H, a.K);
   if (e == cudaSuccess) e = token_map(&k, a, a.k, a.H, a.K);
   if (e == cudaSuccess) e = token_map(&v, a, a.v, a.HV, a.V);
   if (e == cudaSuccess) e = token_map(&o, a, a.d_o, a.HV, a.V);
   if (e == cudaSuccess) e = token_map(&dv, a, a.dv, a.HV, a.V);
+  if (e == cudaSuccess) e = matrix_map(&st, a, w.dS1, a.K, gdr_slots(a, C) * a.HV);
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(rscan_kernel<AB16, KD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L_BYTES);
   if (e != cudaSuccess) return e;
-  rscan_kernel<AB16, KD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), THREADS, L_BYTES, a.stream>>>(q, k, v, o, dv, a, w);
+  rscan_kernel<AB16, KD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), THREADS, L_BYTES, a.stream>>>(q, k, v, o, dv, st, a, w);
   return cudaGetLastError();
 }
 

@@ -43,7 +43,7 @@ template <bool BWD>
 struct Lay {  // offsets of one stage, then of the rest
   static constexpr uint32_t KQ = 0, V = 2 * TILE, DO = 3 * TILE, M = (BWD ? 4 : 3) * TILE, AX = M + MATS;
   static constexpr uint32_t STAGE = (AX + AX_N * 4 + 1023) & ~1023u;
-  static constexpr uint32_t OUT = 2 * STAGE, SMALL = OUT + (BWD ? 0 : TILE);
+  static constexpr uint32_t OUT = 2 * STAGE, SMALL = OUT + TILE;
   static constexpr uint32_t BYTES = SMALL + sizeof(Small) + 1024;
 };
 static_assert(Lay<true>::BYTES <= 232448 && Lay<false>::BYTES <= 232448, "shared memory");
@@ -51,7 +51,8 @@ static_assert(Lay<true>::BYTES <= 232448 && Lay<false>::BYTES <= 232448, "shared
 template <int AB16, int KD, bool BWD>
 __global__ void __launch_bounds__(THREADS, 1)
     scan_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
-                const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmo, GdrArgs a, Ws w) {
+                const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmo,
+                const __grid_constant__ CUtensorMap tms, const __grid_constant__ CUtensorMap tme, GdrArgs a, Ws w) {
   using L = Lay<BWD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -188,31 +189,23 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int k = KH * hh + i;
       S[i] = (a.initial_state && vin && k < a.K) ? a.initial_state[st + (int64_t)k * a.V + v0 + vl] : 0.f;
     }
-    // S as the operand of chunk c (and, for the backward, to the workspace)
-    auto put_state = [&](int c) {
-      uint16_t* g = BWD && vin ? w.S0 + ((sh0 + (int64_t)c * a.HV) * a.V + v0 + vl) * a.K + KH * hh : nullptr;
+    // S as the operand of the next chunk
+    auto put_state = [&]() {
 #pragma unroll
-      for (int i = 0; i < KH; i += 16) {
-        uint32_t hi[8], lo[8];
-        split<AB16, 8>(S + i, hi, lo);
-        tmem_st8(tl + T_SH + hh * (KH / 2) + i / 2, hi);
-        tmem_st8(tl + T_SL + hh * (KH / 2) + i / 2, lo);
-        if (BWD && vin) {
-          if (KH * hh + i < a.K) *reinterpret_cast<uint4*>(g + i) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          if (KH * hh + i + 8 < a.K) *reinterpret_cast<uint4*>(g + i + 8) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
-        }
-      }
+      for (int i = 0; i < KH; i += 16)
+        st_split16<AB16>(tl + T_SH + hh * (KH / 2) + i / 2, tl + T_SL + hh * (KH / 2) + i / 2, S + i);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.s_ready);
     };
-    if (nch > 0) put_state(0);
+    if (nch > 0) put_state();
     for (int c = 0; c < nch; ++c) {
       const int s = c & 1, ph = c & 1;
       const float* ax = reinterpret_cast<const float*>(sm + s * L::STAGE + L::AX);
       const int i0 = 32 * hh;
       pipe_wait(&S_.full[s], (c >> 1) & 1, ab, err, 0x400);
       pipe_wait(&S_.x_full, ph, ab, err, 0x800);
+      if (BWD && c > 0) pipe_wait(&S_.o2_free, (c - 1) & 1, ab, err, 0x40000);  // E of the chunk before is read
       tc_fence_after();
 #pragma unroll
       for (int i = 0; i < 32; i += 16) {
@@ -233,7 +226,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       pipe_wait(&S_.u_full, ph, ab, err, 0x1000);
       tc_fence_after();
       const float gam[2] = {ax[AX_GC], ax[AX_GC]};
-      uint32_t e16[16];
 #pragma unroll
       for (int i = 0; i < 32; i += 16) {
         float x[16], y[16];
@@ -241,10 +233,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_ld16(tl + T_D + 64 + i0 + i, y);
 #pragma unroll
         for (int j = 0; j < 16; j += 2) add2f(x + j, x + j, y + j);
-        uint32_t lo[8];
-        split<AB16, 8>(x, e16 + i / 2, lo);
-        tmem_st8(tl + T_RH + 16 * hh + i / 2, e16 + i / 2);
-        tmem_st8(tl + T_RL + 16 * hh + i / 2, lo);
+        st_split16<AB16>(tl + T_RH + 16 * hh + i / 2, tl + T_RL + 16 * hh + i / 2, x);
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
           const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + i + j);
@@ -258,11 +247,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_before();
       warp_arrive(&S_.u_ready);
       warp_arrive(&S_.empty[s]);
-      if (BWD && vin) {
-        uint16_t* g = w.E + ((sh0 + (int64_t)c * a.HV) * C + i0) * a.V + v0 + vl;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) g[(int64_t)i * a.V] = (uint16_t)(e16[i / 2] >> (16 * (i & 1)));
-      }
       pipe_wait(&S_.d_full, ph, ab, err, 0x2000);
       tc_fence_after();
 #pragma unroll
@@ -272,7 +256,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 16; j += 2) fma2(S + i + j, gam, S + i + j, x + j);
       }
-      if (c + 1 < nch) put_state(c + 1);
+      if (c + 1 < nch) put_state();
       if (BWD && vin && ((c + 1) % ANCHOR == 0 || c + 1 == nch)) {
         float* g = w.Sf + ((gdr_slot0(a, n, sq, C * ANCHOR) + c / ANCHOR) * a.HV + hv) * a.K * a.V + v0 + vl;
 #pragma unroll
@@ -309,6 +293,19 @@ __global__ void __launch_bounds__(THREADS, 1)
       float y[64];
       pipe_wait(&S_.x_full, ph, ab, err, 0x8000);
       tc_fence_after();
+      if (BWD) {
+        // the hi part of S, to the workspace: read before o1_read lets the state change
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          tmem_ld32(tl + T_SH + 32 * i, y);
+          if (threadIdx.x == 0) bulk_wait_read();
+          bar_sync<1, 128>();
+          stage_row(sb + L::OUT, vl, y);
+          fence_async_smem();
+          bar_sync<1, 128>();
+          if (threadIdx.x == 0 && 64 * i < a.K) store_panel(&tms, sm + L::OUT, 64 * i, v0, a.V, sh0 + (int64_t)c * a.HV);
+        }
+      }
       tmem_ld64(tl + T_X + 64, y);
       tc_fence_before();
       warp_arrive(&S_.o1_read);
@@ -330,6 +327,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 16; ++j) y[i + j] += x[j] + z[j];
       }
+      float e[32];
+      if (BWD) tmem_ld32(tl + T_RH, e);  // the hi part of E
       tc_fence_before();
       warp_arrive(&S_.o2_free);
       if (!BWD) {
@@ -353,6 +352,12 @@ __global__ void __launch_bounds__(THREADS, 1)
           copy_rows(out, reinterpret_cast<uint16_t*>(a.o), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, 128);
         }
       } else {
+        if (threadIdx.x == 0) bulk_wait_read();
+        bar_sync<1, 128>();
+        stage_row(sb + L::OUT, vl, e);
+        fence_async_smem();
+        bar_sync<1, 128>();
+        if (threadIdx.x == 0) store_panel(&tme, sm + L::OUT, 0, v0, a.V, sh0 + (int64_t)c * a.HV);
         const Column D(p + L::DO, vl);
 #pragma unroll
         for (int i = 0; i < 64; ++i) y[i] = i < valid ? y[i] * h2f<AB16>(lds16(D.at(i))) : 0.f;
@@ -369,7 +374,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         bar_sync<1, 128>();
       }
     }
-    if (!BWD && threadIdx.x == 0) bulk_wait_all();
+    if (threadIdx.x == 0) bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
@@ -379,16 +384,20 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 template <int AB16, int KD, bool BWD>
 cudaError_t launch(const GdrArgs& a, const Ws& w) {
-  CUtensorMap q, k, v, o;
+  CUtensorMap q, k, v, o, st, e16;
   cudaError_t e = token_map(&q, a, a.q, a.H, a.K);
   if (e == cudaSuccess) e = token_map(&k, a, a.k, a.H, a.K);
   if (e == cudaSuccess) e = token_map(&v, a, a.v, a.HV, a.V);
   if (e == cudaSuccess) e = token_map(&o, a, BWD ? a.d_o : a.o, a.HV, a.V);
+  st = e16 = o;  // unused by the forward
+  const int64_t sh = gdr_slots(a, C) * a.HV;
+  if (BWD && e == cudaSuccess) e = matrix_map(&st, a, w.S0, a.K, sh);
+  if (BWD && e == cudaSuccess) e = matrix_map(&e16, a, w.E, C, sh);
   constexpr uint32_t bytes = Lay<BWD>::BYTES;
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(scan_kernel<AB16, KD, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e != cudaSuccess) return e;
-  scan_kernel<AB16, KD, BWD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), THREADS, bytes, a.stream>>>(q, k, v, o, a, w);
+  scan_kernel<AB16, KD, BWD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), THREADS, bytes, a.stream>>>(q, k, v, o, st, e16, a, w);
   return cudaGetLastError();
 }
 
