@@ -46,7 +46,7 @@ struct Ws {
   float* dotO;         // [V tiles][slots * HV][C]: dO . O
   float* dotV;         // [V tiles][slots * HV][C]: V . dV
   float* Sf;           // [slots of 512 * HV][K][V] fp32 state after every ANCHOR chunks and after the last one
-  float* anchor;       // [V tiles][slots of 512 * HV][8]: <dS, S> there, one part per chain warp
+  float* anchor;       // [V tiles][slots of 512 * HV][16]: <dS, S> there, one part per chain warp
 };
 
 cudaError_t prep(const GdrArgs& a, const Ws& w, int* launches);
@@ -113,7 +113,17 @@ __device__ __forceinline__ void st_split16(uint32_t hi_addr, uint32_t lo_addr, c
   tc::tmem_st8(lo_addr, lo);
 }
 
-// 16 consecutive fp32 columns of this thread's lane
+// 8 and 16 consecutive fp32 columns of this thread's lane
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float* v) {
+  uint32_t r[8];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(taddr));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
   uint32_t r[16];
   asm volatile(
@@ -188,6 +198,13 @@ __device__ __forceinline__ void copy_rows(uint32_t tile, uint16_t* dst, int64_t 
   }
 }
 
+// Warps of the scans (832 threads): 0-7 output (two per TMEM quadrant, half the tokens each), 8-23 chain (four
+// per quadrant, a quarter of the tokens and of K each), 24 TMA, 25 MMA.  A phase of the chain is bound by how
+// fast one warp's instructions go, not by the SM's issue rate (eight chain and four output warps took
+// 6.7 k cycles a chunk forward, 10-10.8 k in the backward's two scans).
+constexpr int SCAN_THREADS = 832, W_CHAIN = 8, W_TMA = 24, W_MMA = 25;
+constexpr int OUT_THREADS = 256, CHAIN_THREADS = 512, OUT_WARPS = 8, CHAIN_WARPS = 16;
+
 // pipe_wait for the MMA thread: polls without suspending (a suspended try_wait wakes a few hundred cycles
 // late, and this thread's waits are all on the chunk's critical path), bounded like the others.
 __device__ __forceinline__ bool spin_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int code) {
@@ -219,14 +236,7 @@ __device__ __forceinline__ void lane_sums(float* x, int lane) {
   }
 }
 
-// 64 16-bit values of row `row` (32 packed words) into a swizzled panel of 128 rows
-__device__ __forceinline__ void stage_row(uint32_t panel, int row, const float* r) {
-  const uint32_t* u = reinterpret_cast<const uint32_t*>(r);
-#pragma unroll
-  for (int ch = 0; ch < 8; ++ch)
-    sts128(panel + tc::sw128(row, ch), make_uint4(u[4 * ch], u[4 * ch + 1], u[4 * ch + 2], u[4 * ch + 3]));
-}
-// such a panel to a [V][width] matrix of (chunk, value head) sh, columns from x, by one thread
+// a swizzled panel of 128 rows to a [V][width] matrix of (chunk, value head) sh, columns from x, by one thread
 __device__ __forceinline__ void store_panel(const CUtensorMap* m, const uint8_t* panel, int x, int v0, int V, int64_t sh) {
   tc::tma_store_3d(m, panel, x, v0, (int)sh);
   if (v0 + 64 < V) tc::tma_store_3d(m, panel + PANEL, x, v0 + 64, (int)sh);

@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int64_t at = (v * vs + s.sh + (int64_t)(tid >> 6) * a.HV) * C + (tid & 63);
           dot += w.dotO[at] - w.dotV[at];
         }
-        if (tid < 8) later += w.anchor[(v * va + s.anchor) * 8 + tid];
+        if (tid < CHAIN_WARPS) later += w.anchor[(v * va + s.anchor) * CHAIN_WARPS + tid];
       }
     }
     pipe_wait(&S_.full[b], (step >> 1) & 1, &S_.abort, w.err, 0x200000);

@@ -12,7 +12,7 @@
 //
 // Written out: dV, V . dV per token, for the gradient kernel dS (16-bit, transposed) of every chunk, and every
 // ANCHOR chunks <dS, S>.
-// Bound, as the scan, by the latency of one chunk's chain.  Warps as in the scan.  TMEM columns: dS hi, lo
+// Bound, as the scan, by the latency of one chunk's chain.  TMEM columns: dS hi, lo
 // (64 each), Y and Z (64 each), then dV (128), D (128), dE, then Gam dV as operand (64), scaled dO (64).
 #include "gdr_tc.cuh"
 
@@ -21,11 +21,10 @@ namespace gdrtc {
 namespace {
 using namespace tc;
 
-constexpr int THREADS = 448;
 constexpr uint32_t T_SH = 0, T_SL = 64, T_Y = 128, T_Z = 192, T_D = 256, T_EH = 384, T_EL = 416, T_GH = 448, T_GL = 480;
 
 struct Small {
-  uint64_t full[2], empty[2], s_ready, y_full, e_ready, f_full, f_ready, f_read, g_ready, h_read, d_full, kz, done;
+  uint64_t full[2], empty[2], s_ready, y_full, e_ready, f_full, f_ready, f_read, g_ready, d_full, kz, done;
   float red[4][C];
   uint32_t tmem;
   int abort;
@@ -38,7 +37,7 @@ constexpr uint32_t L_BYTES = L_SMALL + sizeof(Small) + 1024;
 static_assert(L_BYTES <= 232448, "shared memory");
 
 template <int AB16, int KD>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(SCAN_THREADS, 1)
     rscan_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                  const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmo,
                  const __grid_constant__ CUtensorMap tmdv, const __grid_constant__ CUtensorMap tms, GdrArgs a, Ws w) {
@@ -58,15 +57,14 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&S_.full[i], 1);
-      mbar_init(&S_.empty[i], 13);  // last commit, 8 chain warps, 4 output warps
+      mbar_init(&S_.empty[i], 1 + CHAIN_WARPS + OUT_WARPS);  // last commit, every chain and output warp
     }
-    mbar_init(&S_.s_ready, 8);
-    mbar_init(&S_.e_ready, 8);
-    mbar_init(&S_.f_ready, 8);
-    mbar_init(&S_.f_read, 4);
-    mbar_init(&S_.g_ready, 4);
-    mbar_init(&S_.h_read, 4);
-    mbar_init(&S_.kz, 4);
+    mbar_init(&S_.s_ready, CHAIN_WARPS);
+    mbar_init(&S_.e_ready, CHAIN_WARPS);
+    mbar_init(&S_.f_ready, CHAIN_WARPS);
+    mbar_init(&S_.f_read, OUT_WARPS);
+    mbar_init(&S_.g_ready, OUT_WARPS);
+    mbar_init(&S_.kz, OUT_WARPS);
     mbar_init(&S_.y_full, 1);
     mbar_init(&S_.f_full, 1);
     mbar_init(&S_.d_full, 1);
@@ -74,7 +72,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     S_.abort = 0;
     fence_barrier_init();
   }
-  if (warp == 13) tmem_alloc(&S_.tmem, 512);
+  if (warp == W_MMA) tmem_alloc(&S_.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -83,7 +81,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   int* err = w.err;
   const bool part = sq.len % C != 0;  // the last chunk, the first one here, is partial
 
-  if (warp == 12) {
+  if (warp == W_TMA) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
       int issued = 0;
@@ -109,7 +107,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // never leave the block with copies in flight
       for (int t = (issued > 2 ? issued - 2 : 0); t < issued; ++t) own_copy_wait(&S_.full[t & 1], (t >> 1) & 1, ab, err, 2);
     }
-  } else if (warp == 13) {
+  } else if (warp == W_MMA) {
     // ------------------------------------------------------------------ MMA issuer
     if (lane == 0) {
       const uint32_t id_y = idesc_f16(128, 64, AB16, 0, 0), id_z = idesc_f16(128, 64, AB16, 1, 1);
@@ -140,15 +138,6 @@ __global__ void __launch_bounds__(THREADS, 1)
             umma_ts(tb + T_Y, tb + (x ? T_SL : T_SH) + 8 * ks,
                     sdesc(p + L_KQ + (ks >> 2) * 2 * PANEL + (ks & 3) * 32, 16, 1024), id_y, x + ks > 0);
         umma_commit(&S_.y_full);
-        // D^T = (scale Gam dO)^T Q
-        if (!spin_wait(&S_.g_ready, ph, ab, err, 0x40)) break;
-        tc_fence_after();
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            umma_ts(tb + T_D, tb + (x ? T_GL : T_GH) + 8 * ks, sdesc(p + L_KQ + PANEL + ks * 2048, 2 * PANEL, 1024), id_d,
-                    x + ks > 0);
         // dV^T = dE^T T; the hi and lo halves are added on reading
         if (!spin_wait(&S_.e_ready, ph, ab, err, 0x80)) break;
         tc_fence_after();
@@ -158,6 +147,15 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_Y, tb + T_EL + 8 * ks, sdesc(T + ks * 2048, PANEL, 1024), id_f2, 1);
         umma_commit(&S_.f_full);
+        // D^T = (scale Gam dO)^T Q
+        if (!spin_wait(&S_.g_ready, ph, ab, err, 0x40)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma_ts(tb + T_D, tb + (x ? T_GL : T_GH) + 8 * ks, sdesc(p + L_KQ + PANEL + ks * 2048, 2 * PANEL, 1024), id_d,
+                    x + ks > 0);
         // D^T += (-Gam dV)^T K
         if (!spin_wait(&S_.f_ready, ph, ab, err, 0x200)) break;
         tc_fence_after();
@@ -172,10 +170,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       umma_commit(&S_.done);  // TMEM is freed only after every issued MMA has completed
       mbar_wait(&S_.done, 0);
     }
-  } else if (warp >= 4) {
+  } else if (warp >= W_CHAIN) {
     // ------------------------------------------------------------------ chain: dE, Gam dV, dS
-    constexpr int KH = KD / 2;  // columns of K this thread keeps
-    const int quad = warp & 3, hh = (warp - 4) >> 2;
+    constexpr int KH = KD / 4;  // columns of K this thread keeps
+    const int quad = warp & 3, hh = (warp - W_CHAIN) >> 2;
     const int vl = quad * 32 + lane;
     const bool vin = v0 + vl < a.V;
     const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
@@ -185,11 +183,27 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int k = KH * hh + i;
       S[i] = (a.dfinal_state && vin && k < a.K) ? a.dfinal_state[st + (int64_t)k * a.V + v0 + vl] : 0.f;
     }
-    // dS as the operand of the next chunk
-    auto put_state = [&]() {
+    // dS as the operand of chunk c; its hi part also goes to `tile` (two panels of 128 rows), or straight
+    // to the workspace for the first chunk
+    auto put_state = [&](uint32_t tile) {
 #pragma unroll
-      for (int i = 0; i < KH; i += 16)
-        st_split16<AB16>(tl + T_SH + hh * (KH / 2) + i / 2, tl + T_SL + hh * (KH / 2) + i / 2, S + i);
+      for (int i = 0; i < KH; i += 16) {
+        uint32_t hi[8], lo[8];
+        split<AB16, 8>(S + i, hi, lo);
+        tmem_st8(tl + T_SH + hh * (KH / 2) + i / 2, hi);
+        tmem_st8(tl + T_SL + hh * (KH / 2) + i / 2, lo);
+        const int k = KH * hh + i;
+        const uint4 u = make_uint4(hi[0], hi[1], hi[2], hi[3]), v = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+        if (tile != 0) {
+          const uint32_t pan = tile + (k >> 6) * 2 * PANEL;
+          sts128(pan + sw128(vl, (k & 63) >> 3), u);
+          sts128(pan + sw128(vl, ((k & 63) >> 3) + 1), v);
+        } else if (vin) {
+          uint16_t* g = w.dS1 + ((sh0 + (int64_t)(nch - 1) * a.HV) * a.V + v0 + vl) * a.K + k;
+          if (k < a.K) *reinterpret_cast<uint4*>(g) = u;
+          if (k + 8 < a.K) *reinterpret_cast<uint4*>(g + 8) = v;
+        }
+      }
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.s_ready);
@@ -206,73 +220,83 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (KH * hh + i < a.K) d = fmaf(S[i], g[(int64_t)(KH * hh + i) * a.V], d);
       }
       d = warp_sum(d);
-      if (lane == 0) w.anchor[((int64_t)blockIdx.y * anchors * a.HV + at) * 8 + warp - 4] = d;
+      if (lane == 0) w.anchor[((int64_t)blockIdx.y * anchors * a.HV + at) * CHAIN_WARPS + warp - W_CHAIN] = d;
     };
     if (nch > 0) {
-      put_state();
+      put_state(0);
       put_anchor((nch - 1) / ANCHOR, a.dfinal_state == nullptr);
     }
-    const int i0 = 32 * hh;
+    const int i0 = 16 * hh;
     for (int t = 0; t < nch; ++t) {
       const int s = t & 1, ph = t & 1, c = nch - 1 - t;
       const float* ax = reinterpret_cast<const float*>(sm + s * L_STAGE + L_AX);
       pipe_wait(&S_.full[s], (t >> 1) & 1, ab, err, 0x400);
       pipe_wait(&S_.y_full, ph, ab, err, 0x800);
       tc_fence_after();
+      float x[16];
+      tmem_ld16(tl + T_Z + i0, x);
 #pragma unroll
-      for (int i = 0; i < 32; i += 16) {
-        float y[16], z[16];
-        tmem_ld16(tl + T_Y + i0 + i, y);
-        tmem_ld16(tl + T_Z + i0 + i, z);
+      for (int i = 0; i < 16; i += 8) {
+        float y[8];
+        tmem_ld8(tl + T_Y + i0 + i, y);
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
+        for (int j = 0; j < 8; j += 4) {
           const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + i + j);
           const float bb[4] = {b.x, b.y, b.z, b.w};
-          fma2(z + j, bb, y + j, z + j);
-          fma2(z + j + 2, bb + 2, y + j + 2, z + j + 2);
+          fma2(x + i + j, bb, y + j, x + i + j);
+          fma2(x + i + j + 2, bb + 2, y + j + 2, x + i + j + 2);
         }
-        st_split16<AB16>(tl + T_EH + 16 * hh + i / 2, tl + T_EL + 16 * hh + i / 2, z);
       }
+      st_split16<AB16>(tl + T_EH + 8 * hh, tl + T_EL + 8 * hh, x);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.e_ready);
       pipe_wait(&S_.f_full, ph, ab, err, 0x1000);
       tc_fence_after();
+      tmem_ld16(tl + T_Y + i0, x);
 #pragma unroll
-      for (int i = 0; i < 32; i += 16) {
-        float x[16], y[16];
-        tmem_ld16(tl + T_Y + i0 + i, x);
-        tmem_ld16(tl + T_Y + 64 + i0 + i, y);
+      for (int i = 0; i < 16; i += 8) {
+        float y[8];
+        tmem_ld8(tl + T_Y + 64 + i0 + i, y);
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
+        for (int j = 0; j < 8; j += 4) {
           const float4 b = *reinterpret_cast<const float4*>(ax + AX_G + i0 + i + j);
           const float bb[4] = {-b.x, -b.y, -b.z, -b.w};
-          add2f(x + j, x + j, y + j);
-          add2f(x + j + 2, x + j + 2, y + j + 2);
-          mul2f(x + j, x + j, bb);
-          mul2f(x + j + 2, x + j + 2, bb + 2);
+          float* z = x + i + j;
+          add2f(z, z, y + j);
+          add2f(z + 2, z + 2, y + j + 2);
+          mul2f(z, z, bb);
+          mul2f(z + 2, z + 2, bb + 2);
         }
-        st_split16<AB16>(tl + T_EH + 16 * hh + i / 2, tl + T_EL + 16 * hh + i / 2, x);
       }
+      st_split16<AB16>(tl + T_EH + 8 * hh, tl + T_EL + 8 * hh, x);
       const float gam[2] = {ax[AX_GC], ax[AX_GC]};
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.f_ready);
-      warp_arrive(&S_.empty[s]);
+      if (warp != W_CHAIN) warp_arrive(&S_.empty[s]);
       pipe_wait(&S_.d_full, ph, ab, err, 0x2000);
       tc_fence_after();
 #pragma unroll
       for (int i = 0; i < KH; i += 16) {
-        float x[16];
         tmem_ld16(tl + T_D + KH * hh + i, x);
 #pragma unroll
         for (int j = 0; j < 16; j += 2) fma2(S + i + j, gam, S + i + j, x + j);
       }
-      pipe_wait(&S_.h_read, ph, ab, err, 0x20000);  // the output warps have dS
-      tc_fence_after();
-      if (c > 0) put_state();
+      if (c > 0) put_state(sb + s * L_STAGE + L_KQ);  // every product with the K and Q rows is done: their space is the staging
+      fence_async_smem();
+      bar_sync<2, CHAIN_THREADS>();
+      if (threadIdx.x == 32 * W_CHAIN) {
+        if (c > 0)
+          for (int i = 0; i < NP; ++i)
+            if (64 * i < a.K)
+              store_panel(&tms, sm + s * L_STAGE + L_KQ + 2 * i * PANEL, 64 * i, v0, a.V, sh0 + (int64_t)(c - 1) * a.HV);
+        bulk_wait_read();  // then the stage may be loaded again
+        mbar_arrive(&S_.empty[s]);
+      }
       if (c > 0 && c % ANCHOR == 0) put_anchor(c / ANCHOR - 1, false);
     }
+    if (threadIdx.x == 32 * W_CHAIN) bulk_wait_all();
     if (a.dinitial_state && vin) {
 #pragma unroll
       for (int i = 0; i < KH; ++i) {
@@ -282,8 +306,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------------ output: scaled dO, dV, V . dV
-    const int vl = warp * 32 + lane;
-    const uint32_t tl = tb + ((uint32_t)(warp * 32) << 16);
+    const int quad = warp & 3, j0 = 32 * (warp >> 2);  // tokens j0 .. j0 + 31
+    const int vl = quad * 32 + lane;
+    const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
     const int64_t slots = gdr_slots(a, C);
     for (int t = 0; t < nch; ++t) {
       const int s = t & 1, ph = t & 1, c = nch - 1 - t;
@@ -294,8 +319,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       pipe_wait(&S_.full[s], (t >> 1) & 1, ab, err, 0x4000);
       if (valid < C) {
         // the rows past the document belong to another one: what a product sums over must be zero
-        for (int i = 0; i < 2 * NP; ++i) zero_rows(p + L_KQ + i * PANEL, 1, valid, threadIdx.x, 128);
-        zero_rows(p + L_DO, 2, valid, threadIdx.x, 128);
+        for (int i = 0; i < 2 * NP; ++i) zero_rows(p + L_KQ + i * PANEL, 1, valid, threadIdx.x, OUT_THREADS);
+        zero_rows(p + L_DO, 2, valid, threadIdx.x, OUT_THREADS);
         fence_async_smem();
         warp_arrive(&S_.kz);
       }
@@ -304,7 +329,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       {
         const Column D(p + L_DO, vl);
 #pragma unroll
-        for (int i = 0; i < 64; i += 16) {
+        for (int i = j0; i < j0 + 32; i += 16) {
           float x[16];
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
@@ -319,48 +344,31 @@ __global__ void __launch_bounds__(THREADS, 1)
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.g_ready);
-      float y[64];
-      // the hi part of dS, to the workspace
-      pipe_wait(&S_.y_full, ph, ab, err, 0x40000);
-      tc_fence_after();
-#pragma unroll
-      for (int i = 0; i < NP; ++i) tmem_ld32(tl + T_SH + 32 * i, y + 32 * i);
-      tc_fence_before();
-      warp_arrive(&S_.h_read);
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        if (threadIdx.x == 0) bulk_wait_read();
-        bar_sync<1, 128>();
-        stage_row(sb + L_OUT, vl, y + 32 * i);
-        fence_async_smem();
-        bar_sync<1, 128>();
-        if (threadIdx.x == 0 && 64 * i < a.K) store_panel(&tms, sm + L_OUT, 64 * i, v0, a.V, sh0 + (int64_t)c * a.HV);
-      }
+      float y[32];
       pipe_wait(&S_.f_full, ph, ab, err, 0x10000);
       tc_fence_after();
+      tmem_ld32(tl + T_Y + j0, y);
 #pragma unroll
-      for (int i = 0; i < 64; i += 16) {
+      for (int i = 0; i < 32; i += 16) {
         float x[16];
-        tmem_ld16(tl + T_Y + i, y + i);
-        tmem_ld16(tl + T_Y + 64 + i, x);
+        tmem_ld16(tl + T_Y + 64 + j0 + i, x);
 #pragma unroll
         for (int j = 0; j < 16; j += 2) add2f(y + i + j, y + i + j, x + j);
       }
       tc_fence_before();
       warp_arrive(&S_.f_read);
       if (threadIdx.x == 0) bulk_wait_read();  // the stores of the chunk before have read the tile
-      bar_sync<1, 128>();
+      bar_sync<1, OUT_THREADS>();
       const Column O(sb + L_OUT, vl), V(p + L_V, vl);
 #pragma unroll
-      for (int i = 0; i < 64; ++i) sts16(O.at(i), f2h<AB16>(y[i]));
+      for (int i = 0; i < 32; ++i) sts16(O.at(j0 + i), f2h<AB16>(y[i]));
 #pragma unroll
-      for (int i = 0; i < 64; ++i) y[i] = i < valid ? y[i] * h2f<AB16>(lds16(V.at(i))) : 0.f;
+      for (int i = 0; i < 32; ++i) y[i] = j0 + i < valid ? y[i] * h2f<AB16>(lds16(V.at(j0 + i))) : 0.f;
       warp_arrive(&S_.empty[s]);
-      lane_sums<64>(y, lane);
-      S_.red[warp][2 * lane] = y[0];
-      S_.red[warp][2 * lane + 1] = y[1];
+      lane_sums<32>(y, lane);
+      S_.red[quad][j0 + lane] = y[0];
       fence_async_smem();
-      bar_sync<1, 128>();
+      bar_sync<1, OUT_THREADS>();
       if (valid == C) {
         if (threadIdx.x == 0) {
           tma_store_3d(&tmdv, sm + L_OUT, v0, hv, (int)row0);
@@ -368,21 +376,21 @@ __global__ void __launch_bounds__(THREADS, 1)
           bulk_commit();
         }
       } else {
-        copy_rows(sb + L_OUT, reinterpret_cast<uint16_t*>(a.dv), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, 128);
+        copy_rows(sb + L_OUT, reinterpret_cast<uint16_t*>(a.dv), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, OUT_THREADS);
       }
       if (threadIdx.x < C) {
         const int i = threadIdx.x;
         w.dotV[((int64_t)blockIdx.y * slots * a.HV + sh0 + (int64_t)c * a.HV) * C + i] =
             S_.red[0][i] + S_.red[1][i] + S_.red[2][i] + S_.red[3][i];
       }
-      bar_sync<1, 128>();  // the sums are read before the next chunk's are written
+      bar_sync<1, OUT_THREADS>();  // the sums are read before the next chunk's are written
     }
     if (threadIdx.x == 0) bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 13) tmem_dealloc(tb, 512);
+  if (warp == W_MMA) tmem_dealloc(tb, 512);
 }
 
 template <int AB16, int KD>
@@ -397,7 +405,7 @@ cudaError_t launch(const GdrArgs& a, const Ws& w) {
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(rscan_kernel<AB16, KD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L_BYTES);
   if (e != cudaSuccess) return e;
-  rscan_kernel<AB16, KD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), THREADS, L_BYTES, a.stream>>>(q, k, v, o, dv, st, a, w);
+  rscan_kernel<AB16, KD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), SCAN_THREADS, L_BYTES, a.stream>>>(q, k, v, o, dv, st, a, w);
   return cudaGetLastError();
 }
 

@@ -19,8 +19,7 @@
 // BWD: instead of O it writes what the backward reads: S0 (16-bit, transposed), E (16-bit), dO . O and,
 // every ANCHOR chunks, S in fp32.
 //
-// Warps (448 threads): 0-3 output (one per TMEM quadrant), 4-11 chain (two per quadrant, each half of the
-// columns), 12 TMA, 13 MMA.  TMEM columns: S hi, S lo (64 each), X | Y, then dS (128), E, then E P^T
+// TMEM columns: S hi, S lo (64 each), X | Y, then dS (128), E, then E P^T
 // (128), Gam X / E as operands (64), w beta E as operand (64): all 512.  Every wait is bounded; see tc_common.cuh.
 #include "gdr_tc.cuh"
 
@@ -29,7 +28,6 @@ namespace gdrtc {
 namespace {
 using namespace tc;
 
-constexpr int THREADS = 448;
 constexpr uint32_t T_SH = 0, T_SL = 64, T_X = 128, T_D = 256, T_RH = 384, T_RL = 416, T_WH = 448, T_WL = 480;
 
 struct Small {
@@ -49,7 +47,7 @@ struct Lay {  // offsets of one stage, then of the rest
 static_assert(Lay<true>::BYTES <= 232448 && Lay<false>::BYTES <= 232448, "shared memory");
 
 template <int AB16, int KD, bool BWD>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(SCAN_THREADS, 1)
     scan_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                 const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmo,
                 const __grid_constant__ CUtensorMap tms, const __grid_constant__ CUtensorMap tme, GdrArgs a, Ws w) {
@@ -70,23 +68,23 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&S_.full[i], 1);
-      mbar_init(&S_.empty[i], 13);  // last commit, 8 chain warps, 4 output warps
+      mbar_init(&S_.empty[i], 1 + CHAIN_WARPS + OUT_WARPS);  // last commit, every chain and output warp
     }
-    mbar_init(&S_.s_ready, 8);
-    mbar_init(&S_.r_ready, 8);
-    mbar_init(&S_.u_ready, 8);
+    mbar_init(&S_.s_ready, CHAIN_WARPS);
+    mbar_init(&S_.r_ready, CHAIN_WARPS);
+    mbar_init(&S_.u_ready, CHAIN_WARPS);
     mbar_init(&S_.x_full, 1);
     mbar_init(&S_.u_full, 1);
     mbar_init(&S_.d_full, 1);
     mbar_init(&S_.o_full, 1);
-    mbar_init(&S_.o1_read, 4);
-    mbar_init(&S_.o2_free, 4);
-    mbar_init(&S_.kz, 4);
+    mbar_init(&S_.o1_read, OUT_WARPS);
+    mbar_init(&S_.o2_free, OUT_WARPS);
+    mbar_init(&S_.kz, OUT_WARPS);
     mbar_init(&S_.done, 1);
     S_.abort = 0;
     fence_barrier_init();
   }
-  if (warp == 13) tmem_alloc(&S_.tmem, 512);
+  if (warp == W_MMA) tmem_alloc(&S_.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -94,7 +92,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   volatile int* ab = &S_.abort;
   int* err = w.err;
 
-  if (warp == 12) {
+  if (warp == W_TMA) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
       int issued = 0;
@@ -122,7 +120,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // never leave the block with copies in flight
       for (int c = (issued > 2 ? issued - 2 : 0); c < issued; ++c) own_copy_wait(&S_.full[c & 1], (c >> 1) & 1, ab, err, 2);
     }
-  } else if (warp == 13) {
+  } else if (warp == W_MMA) {
     // ------------------------------------------------------------------ MMA issuer
     if (lane == 0) {
       const uint32_t id64 = idesc_f16(128, 64, AB16, 0, 0), id128 = idesc_f16(128, 128, AB16, 0, 0);
@@ -176,10 +174,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       umma_commit(&S_.done);  // TMEM is freed only after every issued MMA has completed
       mbar_wait(&S_.done, 0);
     }
-  } else if (warp >= 4) {
+  } else if (warp >= W_CHAIN) {
     // ------------------------------------------------------------------ chain: Gam X, E, S
-    constexpr int KH = KD / 2;  // columns of K this thread keeps
-    const int quad = warp & 3, hh = (warp - 4) >> 2;
+    constexpr int KH = KD / 4;  // columns of K this thread keeps
+    const int quad = warp & 3, hh = (warp - W_CHAIN) >> 2;
     const int vl = quad * 32 + lane;
     const bool vin = v0 + vl < a.V;
     const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
@@ -189,74 +187,115 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int k = KH * hh + i;
       S[i] = (a.initial_state && vin && k < a.K) ? a.initial_state[st + (int64_t)k * a.V + v0 + vl] : 0.f;
     }
-    // S as the operand of the next chunk
-    auto put_state = [&]() {
+    // S as the operand of the next chunk; for the backward its hi part also goes to `tile` (two panels of
+    // 128 rows), or straight to the workspace for the first chunk
+    auto put_state = [&](uint32_t tile) {
 #pragma unroll
-      for (int i = 0; i < KH; i += 16)
-        st_split16<AB16>(tl + T_SH + hh * (KH / 2) + i / 2, tl + T_SL + hh * (KH / 2) + i / 2, S + i);
+      for (int i = 0; i < KH; i += 16) {
+        uint32_t hi[8], lo[8];
+        split<AB16, 8>(S + i, hi, lo);
+        tmem_st8(tl + T_SH + hh * (KH / 2) + i / 2, hi);
+        tmem_st8(tl + T_SL + hh * (KH / 2) + i / 2, lo);
+        if (BWD) {
+          const int k = KH * hh + i;
+          const uint4 u = make_uint4(hi[0], hi[1], hi[2], hi[3]), v = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+          if (tile != 0) {
+            const uint32_t pan = tile + (k >> 6) * 2 * PANEL;
+            sts128(pan + sw128(vl, (k & 63) >> 3), u);
+            sts128(pan + sw128(vl, ((k & 63) >> 3) + 1), v);
+          } else if (vin) {
+            uint16_t* g = w.S0 + (sh0 * a.V + v0 + vl) * a.K + k;
+            if (k < a.K) *reinterpret_cast<uint4*>(g) = u;
+            if (k + 8 < a.K) *reinterpret_cast<uint4*>(g + 8) = v;
+          }
+        }
+      }
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.s_ready);
     };
-    if (nch > 0) put_state();
+    if (nch > 0) put_state(0);
     for (int c = 0; c < nch; ++c) {
       const int s = c & 1, ph = c & 1;
+      const uint32_t p = sb + s * L::STAGE;
       const float* ax = reinterpret_cast<const float*>(sm + s * L::STAGE + L::AX);
-      const int i0 = 32 * hh;
+      const int i0 = 16 * hh;
       pipe_wait(&S_.full[s], (c >> 1) & 1, ab, err, 0x400);
       pipe_wait(&S_.x_full, ph, ab, err, 0x800);
-      if (BWD && c > 0) pipe_wait(&S_.o2_free, (c - 1) & 1, ab, err, 0x40000);  // E of the chunk before is read
       tc_fence_after();
+      float x[16];
+      tmem_ld16(tl + T_X + i0, x);
 #pragma unroll
-      for (int i = 0; i < 32; i += 16) {
-        float x[16];
-        tmem_ld16(tl + T_X + i0 + i, x);
-#pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(ax + AX_G + i0 + i + j);
-          const float bb[4] = {-b.x, -b.y, -b.z, -b.w};
-          mul2f(x + j, x + j, bb);
-          mul2f(x + j + 2, x + j + 2, bb + 2);
-        }
-        st_split16<AB16>(tl + T_RH + 16 * hh + i / 2, tl + T_RL + 16 * hh + i / 2, x);
+      for (int j = 0; j < 16; j += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(ax + AX_G + i0 + j);
+        const float bb[4] = {-b.x, -b.y, -b.z, -b.w};
+        mul2f(x + j, x + j, bb);
+        mul2f(x + j + 2, x + j + 2, bb + 2);
       }
+      st_split16<AB16>(tl + T_RH + 8 * hh, tl + T_RL + 8 * hh, x);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.r_ready);
       pipe_wait(&S_.u_full, ph, ab, err, 0x1000);
       tc_fence_after();
       const float gam[2] = {ax[AX_GC], ax[AX_GC]};
+      tmem_ld16(tl + T_D + i0, x);
 #pragma unroll
-      for (int i = 0; i < 32; i += 16) {
-        float x[16], y[16];
-        tmem_ld16(tl + T_D + i0 + i, x);
-        tmem_ld16(tl + T_D + 64 + i0 + i, y);
+      for (int i = 0; i < 16; i += 8) {
+        float y[8];
+        tmem_ld8(tl + T_D + 64 + i0 + i, y);
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) add2f(x + j, x + j, y + j);
-        st_split16<AB16>(tl + T_RH + 16 * hh + i / 2, tl + T_RL + 16 * hh + i / 2, x);
-#pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + i + j);
-          const float bb[4] = {b.x, b.y, b.z, b.w};
-          mul2f(x + j, x + j, bb);
-          mul2f(x + j + 2, x + j + 2, bb + 2);
-        }
-        st_split16<AB16>(tl + T_WH + 16 * hh + i / 2, tl + T_WL + 16 * hh + i / 2, x);
+        for (int j = 0; j < 8; j += 2) add2f(x + i + j, x + i + j, y + j);
       }
+      {
+        uint32_t hi[8], lo[8];
+        split<AB16, 8>(x, hi, lo);
+        tmem_st8(tl + T_RH + 8 * hh, hi);
+        tmem_st8(tl + T_RL + 8 * hh, lo);
+        if (BWD) {  // E, transposed, to the staging panel
+          sts128(sb + L::OUT + sw128(vl, i0 >> 3), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+          sts128(sb + L::OUT + sw128(vl, (i0 >> 3) + 1), make_uint4(hi[4], hi[5], hi[6], hi[7]));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + j);
+        const float bb[4] = {b.x, b.y, b.z, b.w};
+        mul2f(x + j, x + j, bb);
+        mul2f(x + j + 2, x + j + 2, bb + 2);
+      }
+      st_split16<AB16>(tl + T_WH + 8 * hh, tl + T_WL + 8 * hh, x);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.u_ready);
-      warp_arrive(&S_.empty[s]);
+      if (!BWD || warp != W_CHAIN) warp_arrive(&S_.empty[s]);
+      if (BWD) {
+        fence_async_smem();
+        bar_sync<2, CHAIN_THREADS>();
+        if (threadIdx.x == 32 * W_CHAIN) store_panel(&tme, sm + L::OUT, 0, v0, a.V, sh0 + (int64_t)c * a.HV);
+      }
       pipe_wait(&S_.d_full, ph, ab, err, 0x2000);
       tc_fence_after();
 #pragma unroll
       for (int i = 0; i < KH; i += 16) {
-        float x[16];
         tmem_ld16(tl + T_X + KH * hh + i, x);
 #pragma unroll
         for (int j = 0; j < 16; j += 2) fma2(S + i + j, gam, S + i + j, x + j);
       }
-      if (c + 1 < nch) put_state();
+      if (c + 1 < nch) put_state(p + L::KQ);  // every product with the K and Q rows is done: their space is the staging
+      if (BWD) {
+        fence_async_smem();
+        bar_sync<2, CHAIN_THREADS>();
+        if (threadIdx.x == 32 * W_CHAIN) {
+          if (c + 1 < nch)
+            for (int i = 0; i < NP; ++i)
+              if (64 * i < a.K)
+                store_panel(&tms, sm + s * L::STAGE + L::KQ + 2 * i * PANEL, 64 * i, v0, a.V, sh0 + (int64_t)(c + 1) * a.HV);
+          bulk_wait_read();  // then the stage, and the panel of E, may be written again
+          mbar_arrive(&S_.empty[s]);
+        }
+        bar_sync<2, CHAIN_THREADS>();
+      }
       if (BWD && vin && ((c + 1) % ANCHOR == 0 || c + 1 == nch)) {
         float* g = w.Sf + ((gdr_slot0(a, n, sq, C * ANCHOR) + c / ANCHOR) * a.HV + hv) * a.K * a.V + v0 + vl;
 #pragma unroll
@@ -264,6 +303,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (KH * hh + i < a.K) g[(int64_t)(KH * hh + i) * a.V] = S[i];
       }
     }
+    if (BWD && threadIdx.x == 32 * W_CHAIN) bulk_wait_all();
     if (!BWD && a.final_state && vin) {
 #pragma unroll
       for (int i = 0; i < KH; ++i) {
@@ -273,8 +313,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------------ output
-    const int vl = warp * 32 + lane;
-    const uint32_t tl = tb + ((uint32_t)(warp * 32) << 16);
+    const int quad = warp & 3, j0 = 32 * (warp >> 2);  // tokens j0 .. j0 + 31
+    const int vl = quad * 32 + lane;
+    const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
     const int64_t slots = gdr_slots(a, C);
     for (int c = 0; c < nch; ++c) {
       const int s = c & 1, ph = c & 1;
@@ -285,33 +326,20 @@ __global__ void __launch_bounds__(THREADS, 1)
       pipe_wait(&S_.full[s], (c >> 1) & 1, ab, err, 0x4000);
       if (valid < C) {
         // the rows past the document belong to another one: what a product sums over must be zero
-        for (int i = 0; i < NP; ++i) zero_rows(p + L::KQ + 2 * i * PANEL, 1, valid, threadIdx.x, 128);
-        zero_rows(p + L::V, 2, valid, threadIdx.x, 128);
+        for (int i = 0; i < NP; ++i) zero_rows(p + L::KQ + 2 * i * PANEL, 1, valid, threadIdx.x, OUT_THREADS);
+        zero_rows(p + L::V, 2, valid, threadIdx.x, OUT_THREADS);
         fence_async_smem();
         warp_arrive(&S_.kz);
       }
-      float y[64];
+      float y[32];
       pipe_wait(&S_.x_full, ph, ab, err, 0x8000);
       tc_fence_after();
-      if (BWD) {
-        // the hi part of S, to the workspace: read before o1_read lets the state change
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          tmem_ld32(tl + T_SH + 32 * i, y);
-          if (threadIdx.x == 0) bulk_wait_read();
-          bar_sync<1, 128>();
-          stage_row(sb + L::OUT, vl, y);
-          fence_async_smem();
-          bar_sync<1, 128>();
-          if (threadIdx.x == 0 && 64 * i < a.K) store_panel(&tms, sm + L::OUT, 64 * i, v0, a.V, sh0 + (int64_t)c * a.HV);
-        }
-      }
-      tmem_ld64(tl + T_X + 64, y);
+      tmem_ld32(tl + T_X + 64 + j0, y);
       tc_fence_before();
       warp_arrive(&S_.o1_read);
 #pragma unroll
-      for (int i = 0; i < 64; i += 4) {
-        const float4 b = *reinterpret_cast<const float4*>(ax + AX_SG + i);
+      for (int i = 0; i < 32; i += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(ax + AX_SG + j0 + i);
         y[i] *= b.x;
         y[i + 1] *= b.y;
         y[i + 2] *= b.z;
@@ -321,65 +349,55 @@ __global__ void __launch_bounds__(THREADS, 1)
       tc_fence_after();
 #pragma unroll
       for (int i = 0; i < 64; i += 16) {
-        float x[16], z[16];
-        tmem_ld16(tl + T_D + i, x);
-        tmem_ld16(tl + T_D + 64 + i, z);
+        float x[16];
+        tmem_ld16(tl + T_D + 64 * (i >> 5) + j0 + (i & 16), x);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) y[i + j] += x[j] + z[j];
+        for (int j = 0; j < 16; j += 2) add2f(y + (i & 16) + j, y + (i & 16) + j, x + j);
       }
-      float e[32];
-      if (BWD) tmem_ld32(tl + T_RH, e);  // the hi part of E
       tc_fence_before();
       warp_arrive(&S_.o2_free);
       if (!BWD) {
         warp_arrive(&S_.empty[s]);
         const uint32_t out = sb + L::OUT;
         if (threadIdx.x == 0) bulk_wait_read();  // the stores of the chunk before have read the tile
-        bar_sync<1, 128>();
+        bar_sync<1, OUT_THREADS>();
         const Column O(out, vl);
 #pragma unroll
-        for (int i = 0; i < 64; ++i) sts16(O.at(i), f2h<AB16>(y[i]));
+        for (int i = 0; i < 32; ++i) sts16(O.at(j0 + i), f2h<AB16>(y[i]));
         if (valid == C) {
           fence_async_smem();
-          bar_sync<1, 128>();
+          bar_sync<1, OUT_THREADS>();
           if (threadIdx.x == 0) {
             tma_store_3d(&tmo, sm + L::OUT, v0, hv, (int)row0);
             if (v0 + 64 < a.V) tma_store_3d(&tmo, sm + L::OUT + PANEL, v0 + 64, hv, (int)row0);
             bulk_commit();
           }
         } else {
-          bar_sync<1, 128>();
-          copy_rows(out, reinterpret_cast<uint16_t*>(a.o), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, 128);
+          bar_sync<1, OUT_THREADS>();
+          copy_rows(out, reinterpret_cast<uint16_t*>(a.o), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, OUT_THREADS);
         }
       } else {
-        if (threadIdx.x == 0) bulk_wait_read();
-        bar_sync<1, 128>();
-        stage_row(sb + L::OUT, vl, e);
-        fence_async_smem();
-        bar_sync<1, 128>();
-        if (threadIdx.x == 0) store_panel(&tme, sm + L::OUT, 0, v0, a.V, sh0 + (int64_t)c * a.HV);
         const Column D(p + L::DO, vl);
 #pragma unroll
-        for (int i = 0; i < 64; ++i) y[i] = i < valid ? y[i] * h2f<AB16>(lds16(D.at(i))) : 0.f;
+        for (int i = 0; i < 32; ++i) y[i] = j0 + i < valid ? y[i] * h2f<AB16>(lds16(D.at(j0 + i))) : 0.f;
         warp_arrive(&S_.empty[s]);
-        lane_sums<64>(y, lane);
-        S_.red[warp][2 * lane] = y[0];
-        S_.red[warp][2 * lane + 1] = y[1];
-        bar_sync<1, 128>();
+        lane_sums<32>(y, lane);
+        S_.red[quad][j0 + lane] = y[0];
+        bar_sync<1, OUT_THREADS>();
         if (threadIdx.x < C) {
           const int i = threadIdx.x;
           w.dotO[((int64_t)blockIdx.y * slots * a.HV + sh0 + (int64_t)c * a.HV) * C + i] =
               S_.red[0][i] + S_.red[1][i] + S_.red[2][i] + S_.red[3][i];
         }
-        bar_sync<1, 128>();
+        bar_sync<1, OUT_THREADS>();
       }
     }
-    if (threadIdx.x == 0) bulk_wait_all();
+    if (!BWD && threadIdx.x == 0) bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 13) tmem_dealloc(tb, 512);
+  if (warp == W_MMA) tmem_dealloc(tb, 512);
 }
 
 template <int AB16, int KD, bool BWD>
@@ -397,7 +415,7 @@ cudaError_t launch(const GdrArgs& a, const Ws& w) {
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(scan_kernel<AB16, KD, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e != cudaSuccess) return e;
-  scan_kernel<AB16, KD, BWD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), THREADS, bytes, a.stream>>>(q, k, v, o, st, e16, a, w);
+  scan_kernel<AB16, KD, BWD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), SCAN_THREADS, bytes, a.stream>>>(q, k, v, o, st, e16, a, w);
   return cudaGetLastError();
 }
 
