@@ -5,12 +5,23 @@
 //   dbeta_j = sum_i scale D_ij (q_i.k_j) (dO E^T)_ij + w_j k_j.(E dS1^T)_j - sum_i D_ij (k_i.k_j) (dV E^T)_ij
 //   dg_t = sum_{i >= t} (dO_i . O_i - V_i . dV_i) + <dS, S>, over the tokens up to the next anchor and there
 //
-// summed over the value heads of the key head in registers.  The chunks are independent: persistent
-// blocks of 16 warps walk (chunk, key head) items; each item runs over (value head, 64 columns of V)
-// steps whose tiles are loaded by TMA two steps ahead, across items.  A warp holds a 16 x 32 tile of the
-// 64 x 128 products and a 16 x 16 tile of the 64 x 64 ones, on mma.sync: an item reads 144 KB for 29 MFLOP, so
-// HBM and mma.sync are about equally near; five products with 64-row operands would leave half of
-// each tcgen05 tile empty.  Operands are single 16-bit values: what is formed here is rounded to 16 bits next.
+// summed over the value heads of the key head in TMEM.  The chunks are independent: persistent blocks
+// walk (chunk, key head) items, and an item's (value head, 64 columns of V) steps are loaded by TMA two
+// ahead, across items.  The 64-token operands are stacked in pairs to fill the 128 lanes: rows 0-63 carry what
+// leads to dK, rows 64-127 what leads to dQ:
+//
+//   X  = [dV ; dO] S0^T    [128 x K]      P = [dV ; dO] E^T   [128 x 64]     B = [K ; Q] K^T  [128 x 64]
+//   X2 = E dS1^T           [64 x K] (its other 64 rows are not read)
+//   F  = [-Gam X + w beta X2 ; scale Gam X] + [N ; W] K + [N^T ; 0] K + [W^T ; 0] Q
+//
+// X, X2, P and B are read by the epilogue warps, which put the first term of F back into TMEM and [N ; W]
+// into shared memory; the transposed products read the same bytes MN-major, with a panel of zeros for
+// the other half.  44 MMAs an item; operands are single 16-bit values, since what is formed here is rounded to
+// 16 bits next.  An item moves 176 KB; the kernel is bound by that and by the serial epilogue between
+// its two groups of products, of which the next item's loads and the last item's stores run beside.
+//
+// Warps (576 threads): 0-7 epilogue A (P and B), 8-15 epilogue B (X and X2), all of them the output; 16 TMA,
+// 17 MMA.
 #include "gdr_tc.cuh"
 
 namespace ccq {
@@ -18,100 +29,38 @@ namespace gdrtc {
 namespace {
 using namespace tc;
 
-constexpr int THREADS = 512;
-constexpr uint32_t B_S = 0, B_DS = 2 * PANEL, B_DO = 4 * PANEL, B_E = 5 * PANEL, B_DV = 6 * PANEL, B_SIZE = 7 * PANEL;  // one step
-constexpr uint32_t L_QK = 0;                       // two buffers of Q (2 panels) and K (2 panels)
+constexpr int THREADS = 576, EPI = 512;
+constexpr uint32_t T_X = 0, T_X2 = 128, T_P = 256, T_B = 320, T_F = 384;
+// one step: [dV ; dO] (two panels), E, S0 and dS1 (two panels each)
+constexpr uint32_t B_DV = 0, B_DO = PANEL, B_E = 2 * PANEL, B_S = 3 * PANEL, B_DS = 5 * PANEL, B_SIZE = 7 * PANEL;
+constexpr uint32_t L_KQ = 0;                       // two buffers: K over Q in panels of 128 rows
 constexpr uint32_t L_B = 8 * PANEL;                // two steps
-constexpr uint32_t L_W = L_B + 2 * B_SIZE, L_N = L_W + PANEL;
-constexpr uint32_t L_AX = L_N + PANEL;             // two
+constexpr uint32_t L_W = L_B + 2 * B_SIZE;         // N over W, then zeros
+constexpr uint32_t L_Z = L_W + 2 * PANEL;
 constexpr uint32_t AX_BYTES = (AX_N * 4 + 127) & ~127u;
+constexpr uint32_t L_AX = L_Z + PANEL;             // four
+constexpr int RING = 4;
 
-__device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t* r, uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-template <int AB16>
-__device__ __forceinline__ void mma16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  if (AB16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// A [16 x 16] fragments of a row-major panel tile (rows r0.., 16-byte chunks c0, c0 + 1)
-__device__ __forceinline__ uint32_t a_addr(uint32_t panel, int r0, int c0, int lane) {
-  return panel + sw128(r0 + (lane & 15), c0 + (lane >> 4));
-}
-// the same of the transposed matrix: A[m][k] = P[k][m], rows k0.. of the panel, columns m from chunk c0
-__device__ __forceinline__ uint32_t at_addr(uint32_t panel, int k0, int c0, int lane) {
-  return panel + sw128(k0 + (lane & 7) + ((lane >> 4) << 3), c0 + ((lane >> 3) & 1));
-}
-// B fragments of two 8-column tiles, B[k][n] = P[n][k]: rows n0.., k from chunk c0 (non-transposed load)
-__device__ __forceinline__ uint32_t b_addr(uint32_t panel, int n0, int c0, int lane) {
-  return panel + sw128(n0 + (lane & 7) + ((lane >> 4) << 3), c0 + ((lane >> 3) & 1));
-}
-// B[k][n] = P[k][n]: rows k0.., n from chunk c0 (transposed load)
-__device__ __forceinline__ uint32_t bt_addr(uint32_t panel, int k0, int c0, int lane) {
-  return panel + sw128(k0 + (lane & 15), c0 + (lane >> 4));
-}
-
-// One step as the block's warps see it, written by thread 0 two steps ahead.
-struct Step {
-  int live, hv, h, row0, valid, first_v, last_v, first, last, qk, ax, more, zero_first;
+// One value head of an item, written by the TMA thread.  Four in a ring: the loads run at most two steps ahead
+// of the products, those one value head ahead of the epilogue.
+struct Rec {
+  int live, hv, h, row0, valid, first, last, qk, more, zero_first;
   int64_t sh, anchor;
 };
-
-__device__ __forceinline__ int nvt128(const GdrArgs& a) { return (a.V + VT - 1) / VT; }
-
-// The position of the next step to load (thread 0's; in shared memory to spare the others its registers).
-struct Walk {
-  int item, items, count, n, c, g, vt, loaded;  // item = slot * H + key head
-  Seq sq;
-  bool live;
-  __device__ __forceinline__ void find(const GdrArgs& a) {
-    for (; item < items; item += gridDim.x)
-      if (gdr_slot_find(a, item / a.H, C, &n, &c, &sq)) {
-        live = true;
-        g = vt = 0;
-        return;
-      }
-    live = false;
-  }
-  __device__ __forceinline__ void next(const GdrArgs& a, int group, int nvt) {
-    if (++vt < nvt) return;
-    vt = 0;
-    if (++g < group) return;
-    item += gridDim.x;
-    ++count;
-    find(a);
-  }
-};
-
 struct Small {
-  uint64_t full[2];
-  Step step[2];
-  Walk walk;
-  float ke[4][C], db[4][C], dg[17];
-  int abort;
+  uint64_t full[2], empty[2], qk_empty[2];
+  uint64_t rec_full[RING];  // the record and its per-token factors
+  uint64_t x_full, wn_ready, f_full, kz, done;
+  Rec rec[RING];
+  float ke[2][C], db[4][C], dg[17];
+  uint32_t tmem;
+  int go, abort;
 };
-constexpr uint32_t L_SMALL = L_AX + 2 * AX_BYTES;
+constexpr uint32_t L_SMALL = L_AX + RING * AX_BYTES;
 constexpr uint32_t BYTES = L_SMALL + sizeof(Small) + 1024;
 static_assert(BYTES <= 232448, "shared memory");
 
-// ONE: a key head serves one value head, so nothing is carried from one value head to the next
-template <int AB16, int KD, bool ONE>
+template <int AB16, int KD>
 __global__ void __launch_bounds__(THREADS, 1)
     grads_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                  const __grid_constant__ CUtensorMap tmo, const __grid_constant__ CUtensorMap tmdv,
@@ -123,314 +72,370 @@ __global__ void __launch_bounds__(THREADS, 1)
   Small& S_ = *reinterpret_cast<Small*>(sm + L_SMALL);
   const uint32_t sb = smem_u32(sm);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int mt = warp >> 2, nq = warp & 3;  // rows 16 mt.., columns KD / 4 nq.. of K (16 nq.. of the 64 x 64 products)
-  const int g = lane >> 2, tq = lane & 3;
-  constexpr int NP = KD / 64, NT = KD / 32;  // panels of K; 8-column tiles of K a warp holds
+  constexpr int NP = KD / 64;
   const int group = a.HV / a.H, nvt = (a.V + 63) / 64;
   if (tid == 0) {
-    mbar_init(&S_.full[0], 1);
-    mbar_init(&S_.full[1], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&S_.full[i], 1);
+      mbar_init(&S_.empty[i], 1);
+      mbar_init(&S_.qk_empty[i], 1);
+    }
+    for (int i = 0; i < RING; ++i) mbar_init(&S_.rec_full[i], 1);
+    mbar_init(&S_.x_full, 1);
+    mbar_init(&S_.wn_ready, EPI / 32);
+    mbar_init(&S_.f_full, 1);
+    mbar_init(&S_.kz, EPI / 32);
+    mbar_init(&S_.done, 1);
     S_.abort = 0;
     fence_barrier_init();
   }
+  if (tid < EPI) sts128(sb + L_Z + tid * 16, make_uint4(0, 0, 0, 0));
+  fence_async_smem();
+  if (warp == 17) tmem_alloc(&S_.tmem, 512);
+  tc_fence_before();
   __syncthreads();
-  Walk& pf = S_.walk;
-  // thread 0: describes and loads the next step
-  auto load = [&]() {
-    const int b = pf.loaded & 1;
-    Step& s = S_.step[b];
-    s.live = pf.live;
-    if (!pf.live) return;
-    {
-      uint64_t* bar = &S_.full[b];
-      uint8_t* p = sm + L_B + b * B_SIZE;
-      const int slot = pf.item / a.H, h = pf.item - slot * a.H, hv = h * group + pf.g;
-      const int64_t sh = (int64_t)slot * a.HV + hv;
-      const int row = (int)(pf.sq.bos + (int64_t)pf.c * C);
-      const int nch = (pf.sq.len + C - 1) / C;
-      s.hv = hv;
-      s.h = h;
-      s.row0 = row;
-      s.valid = min(C, pf.sq.len - pf.c * C);
-      s.first_v = pf.vt == 0;
-      s.last_v = pf.vt == nvt - 1;
-      s.first = s.first_v && pf.g == 0;
-      s.last = s.last_v && pf.g == group - 1;
-      s.qk = pf.count & 1;
-      s.ax = (pf.count * group + pf.g) & 1;
-      s.more = min(ANCHOR - 1 - pf.c % ANCHOR, nch - 1 - pf.c);
-      s.zero_first = pf.c == 0 && a.initial_state == nullptr;
-      s.sh = sh;
-      s.anchor = (gdr_slot0(a, pf.n, pf.sq, C * ANCHOR) + pf.c / ANCHOR) * a.HV + hv;
-      mbar_arrive_expect_tx(bar, 2 * NP * PANEL + 3 * PANEL + (s.first_v ? AX_N * 4 : 0) + (s.first ? 2 * NP * PANEL : 0));
-      if (s.first) {
-        uint8_t* d = sm + L_QK + s.qk * 4 * PANEL;
-        for (int i = 0; i < NP; ++i) {
-          tma_load_3d(d + i * PANEL, &tmq, bar, 64 * i, h, row);
-          tma_load_3d(d + (2 + i) * PANEL, &tmk, bar, 64 * i, h, row);
+  tc_fence_after();
+  const uint32_t tb = S_.tmem;
+  volatile int* ab = &S_.abort;
+  int* err = w.err;
+
+  if (warp == 16) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      const int items = (int)(gdr_slots(a, C) * a.H);
+      int step = 0, rec = 0, count = 0;
+      bool ok = true;
+      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        const int slot = item / a.H, h = item - slot * a.H;
+        int n, c;
+        Seq sq;
+        if (!gdr_slot_find(a, slot, C, &n, &c, &sq)) continue;
+        const int row = (int)(sq.bos + (int64_t)c * C), nch = (sq.len + C - 1) / C;
+        for (int g = 0; g < group && ok; ++g, ++rec) {
+          const int hv = h * group + g, r = rec % RING;
+          const int64_t sh = (int64_t)slot * a.HV + hv;
+          for (int vt = 0; vt < nvt; ++vt, ++step) {
+            const int b = step & 1;
+            if (step >= 2 && !pipe_wait(&S_.empty[b], ((step - 2) >> 1) & 1, ab, err, 1)) { ok = false; break; }
+            if (g == 0 && vt == 0 && count >= 2 && !pipe_wait(&S_.qk_empty[count & 1], ((count - 2) >> 1) & 1, ab, err, 2)) {
+              ok = false;
+              break;
+            }
+            if (*ab) { ok = false; break; }
+            uint64_t* bar = &S_.full[b];
+            uint8_t* p = sm + L_B + b * B_SIZE;
+            mbar_arrive_expect_tx(bar, 2 * NP * PANEL + 3 * PANEL + (g == 0 && vt == 0 ? 2 * NP * PANEL : 0));
+            if (vt == 0) {
+              Rec& R = S_.rec[r];
+              R.live = 1;
+              R.hv = hv;
+              R.h = h;
+              R.row0 = row;
+              R.valid = min(C, sq.len - c * C);
+              R.first = g == 0;
+              R.last = g == group - 1;
+              R.qk = count & 1;
+              R.more = min(ANCHOR - 1 - c % ANCHOR, nch - 1 - c);
+              R.zero_first = c == 0 && a.initial_state == nullptr;
+              R.sh = sh;
+              R.anchor = (gdr_slot0(a, n, sq, C * ANCHOR) + c / ANCHOR) * a.HV + hv;
+              mbar_arrive_expect_tx(&S_.rec_full[r], AX_N * 4);
+              bulk_load(sm + L_AX + r * AX_BYTES, w.aux + sh * AX_N, AX_N * 4, &S_.rec_full[r]);
+              if (g == 0) {
+                uint8_t* d = sm + L_KQ + (count & 1) * 4 * PANEL;
+                for (int i = 0; i < NP; ++i) {
+                  tma_load_3d(d + 2 * i * PANEL, &tmk, bar, 64 * i, h, row);
+                  tma_load_3d(d + (2 * i + 1) * PANEL, &tmq, bar, 64 * i, h, row);
+                }
+              }
+            }
+            tma_load_3d(p + B_DV, &tmdv, bar, 64 * vt, hv, row);
+            tma_load_3d(p + B_DO, &tmo, bar, 64 * vt, hv, row);
+            tma_load_3d(p + B_E, &tme, bar, 0, 64 * vt, (int)sh);
+            for (int i = 0; i < NP; ++i) {
+              tma_load_3d(p + B_S + i * PANEL, &tms, bar, 64 * i, 64 * vt, (int)sh);
+              tma_load_3d(p + B_DS + i * PANEL, &tmds, bar, 64 * i, 64 * vt, (int)sh);
+            }
+          }
         }
+        ++count;
       }
-      if (s.first_v) bulk_load(sm + L_AX + s.ax * AX_BYTES, w.aux + sh * AX_N, AX_N * 4, bar);
-      tma_load_3d(p + B_DO, &tmo, bar, 64 * pf.vt, hv, row);
-      tma_load_3d(p + B_DV, &tmdv, bar, 64 * pf.vt, hv, row);
-      tma_load_3d(p + B_E, &tme, bar, 0, 64 * pf.vt, (int)sh);
-      for (int i = 0; i < NP; ++i) {
-        tma_load_3d(p + B_S + i * PANEL, &tms, bar, 64 * i, 64 * pf.vt, (int)sh);
-        tma_load_3d(p + B_DS + i * PANEL, &tmds, bar, 64 * i, 64 * pf.vt, (int)sh);
+      // never leave the block with copies in flight; then the end, for the others
+      for (int i = (step > 2 ? step - 2 : 0); i < step; ++i) own_copy_wait(&S_.full[i & 1], (i >> 1) & 1, ab, err, 4);
+      for (int i = (rec > RING ? rec - RING : 0); i < rec; ++i)
+        own_copy_wait(&S_.rec_full[i % RING], (i / RING) & 1, ab, err, 4);
+      if (ok) {
+        S_.rec[rec % RING].live = 0;
+        mbar_arrive(&S_.rec_full[rec % RING]);
       }
     }
-    ++pf.loaded;
-    pf.next(a, group, nvt);
-  };
-  if (tid == 0) {
-    pf.loaded = 0;
-    pf.items = (int)(gdr_slots(a, C) * a.H);
-    pf.item = blockIdx.x;
-    pf.count = 0;
-    pf.find(a);
-    load();
-    load();
-  }
-  __syncthreads();
-  float dq[NT][4], dk[NT][4];  // ONE: dO S0^T and dV S0^T grow into them
-  float xq[NT][4], xv[NT][4], xe[NT][4], pe[2][4], ve[2][4];  // dO S0^T, dV S0^T, E dS1^T, dO E^T, dV E^T
-  float dot = 0.f, later = 0.f;
-  for (int step = 0;; ++step) {
-    const int b = step & 1;
-    const Step& s = S_.step[b];
-    if (!s.live) break;
-    // what is read after the step's last barrier, when thread 0 may already describe the step after the next
-    const int valid = s.valid, row0 = s.row0, head = s.h;
-    const bool last = s.last;
-    const uint32_t p = sb + L_B + b * B_SIZE;
-    const uint32_t Q = sb + L_QK + s.qk * 4 * PANEL, K = Q + 2 * PANEL;
-    const float* ax = reinterpret_cast<const float*>(sm + L_AX + s.ax * AX_BYTES);
-    if (s.first_v) {
+  } else if (warp == 17) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const uint32_t id_x = idesc_f16(128, KD, AB16, 0, 1), id_x2 = idesc_f16(128, KD, AB16, 1, 1);
+      const uint32_t id_p = idesc_f16(128, 64, AB16, 0, 1), id_b = idesc_f16(128, 64, AB16, 0, 0);
+      const uint32_t W = sb + L_W;
+      int step = 0, zeroed = 0;
+      for (int rec = 0;; ++rec) {
+        const int r = rec % RING;
+        if (!spin_wait(&S_.rec_full[r], (rec / RING) & 1, ab, err, 8)) break;
+        const Rec& R = S_.rec[r];
+        if (!R.live) break;
+        const uint32_t KQ = sb + L_KQ + R.qk * 4 * PANEL;
+        bool ok = true;
+        for (int vt = 0; vt < nvt; ++vt, ++step) {
+          const int b = step & 1;
+          const uint32_t p = sb + L_B + b * B_SIZE;
+          if (!spin_wait(&S_.full[b], (step >> 1) & 1, ab, err, 0x10)) { ok = false; break; }
+          if (vt == 0 && R.first && R.valid < C) {
+            if (!spin_wait(&S_.kz, zeroed & 1, ab, err, 0x20)) { ok = false; break; }
+            ++zeroed;
+          }
+          tc_fence_after();
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+          for (int ks = 0; ks < 4; ++ks)
+            umma(tb + T_P, sdesc(p + B_DV + ks * 32, 16, 1024), sdesc(p + B_E + ks * 2048, PANEL, 1024), id_p, vt + ks > 0);
+          if (vt == 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          xq[i][j] = xv[i][j] = xe[i][j] = 0.f;
-          if (!ONE && s.first) dq[i][j] = dk[i][j] = 0.f;
+            for (int ks = 0; ks < KD / 16; ++ks) {
+              const uint64_t d = sdesc(KQ + (ks >> 2) * 2 * PANEL + (ks & 3) * 32, 16, 1024);
+              umma(tb + T_B, d, d, id_b, ks > 0);
+            }
+          }
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma(tb + T_X, sdesc(p + B_DV + ks * 32, 16, 1024), sdesc(p + B_S + ks * 2048, PANEL, 1024), id_x, vt + ks > 0);
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma(tb + T_X2, sdesc(p + B_E + ks * 2048, PANEL, 1024), sdesc(p + B_DS + ks * 2048, PANEL, 1024), id_x2,
+                 vt + ks > 0);
+          umma_commit(&S_.empty[b]);
         }
+        if (!ok) break;
+        umma_commit(&S_.x_full);
+        if (!spin_wait(&S_.wn_ready, rec & 1, ab, err, 0x40)) break;
+        tc_fence_after();
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int ks = 0; ks < 4; ++ks)
+          umma(tb + T_F, sdesc(W + ks * 32, 16, 1024), sdesc(KQ + ks * 2048, 2 * PANEL, 1024), id_x, 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) pe[i][j] = ve[i][j] = 0.f;
+        for (int ks = 0; ks < 4; ++ks)
+          umma(tb + T_F, sdesc(W + ks * 2048, 2 * PANEL, 1024), sdesc(KQ + ks * 2048, 2 * PANEL, 1024), id_x2, 1);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+          umma(tb + T_F, sdesc(W + PANEL + ks * 2048, PANEL, 1024), sdesc(KQ + PANEL + ks * 2048, 2 * PANEL, 1024), id_x2, 1);
+        umma_commit(&S_.f_full);
+      }
+      umma_commit(&S_.done);  // TMEM is freed only after every issued MMA has completed
+      mbar_wait(&S_.done, 0);
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    const int quad = warp & 3;
+    const bool kside = quad < 2;          // rows 0-63: what leads to dK
+    const int i = (quad & 1) * 32 + lane; // token
+    const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
+    int first_step = 0;                   // step of this record's first loads
+    for (int rec = 0;; ++rec, first_step += nvt) {
+      const int r = rec % RING;
+      const Rec& R = S_.rec[r];
+      // one decision for all warps, so that a wait that gave up cannot leave some of them at a barrier
+      if (tid == 0) S_.go = pipe_wait(&S_.rec_full[r], (rec / RING) & 1, ab, err, 0x80) && R.live;
+      bar_sync<1, EPI>();
+      if (!S_.go) break;
+      const int valid = R.valid;
+      const uint32_t KQ = sb + L_KQ + R.qk * 4 * PANEL;
+      const float* ax = reinterpret_cast<const float*>(sm + L_AX + r * AX_BYTES);
       // dO . O - V . dV: of this chunk's tokens in warps 0 and 1, of the chunks up to the next anchor in the
       // others; and <dS, S> there
-      dot = later = 0.f;
-      const int64_t vs = gdr_slots(a, C) * a.HV, va = gdr_slots(a, C * ANCHOR) * a.HV;
-      for (int v = 0; v < nvt128(a); ++v) {
-        if ((tid >> 6) <= s.more) {
-          const int64_t at = (v * vs + s.sh + (int64_t)(tid >> 6) * a.HV) * C + (tid & 63);
-          dot += w.dotO[at] - w.dotV[at];
-        }
-        if (tid < CHAIN_WARPS) later += w.anchor[(v * va + s.anchor) * CHAIN_WARPS + tid];
-      }
-    }
-    pipe_wait(&S_.full[b], (step >> 1) & 1, &S_.abort, w.err, 0x200000);
-    if (valid < C && s.first) {
-      // the rows past the document belong to another one: what a product sums over must be zero
-      for (int i = 0; i < NP; ++i) {
-        zero_rows(Q + i * PANEL, 1, valid, tid, THREADS);
-        zero_rows(K + i * PANEL, 1, valid, tid, THREADS);
-      }
-      __syncthreads();
-    }
-#pragma unroll 1
-    for (int ks = 0; ks < 4; ++ks) {
-      uint32_t fo[4], fv[4], fe[4], be[4];
-      ldsm4(fo, a_addr(p + B_DO, 16 * mt, 2 * ks, lane));
-      ldsm4(fv, a_addr(p + B_DV, 16 * mt, 2 * ks, lane));
-      ldsm4t(fe, at_addr(p + B_E, 16 * ks, 2 * mt, lane));
-      ldsm4t(be, bt_addr(p + B_E, 16 * ks, 2 * nq, lane));
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        mma16<AB16>(pe[j], fo, be[2 * j], be[2 * j + 1]);
-        mma16<AB16>(ve[j], fv, be[2 * j], be[2 * j + 1]);
-      }
-#pragma unroll
-      for (int j = 0; j < NT / 2; ++j) {
-        const int col = (KD / 4) * nq + 16 * j;
-        uint32_t bs[4], bd[4];
-        ldsm4t(bs, bt_addr(p + B_S + (col >> 6) * PANEL, 16 * ks, (col & 63) >> 3, lane));
-        ldsm4t(bd, bt_addr(p + B_DS + (col >> 6) * PANEL, 16 * ks, (col & 63) >> 3, lane));
-        mma16<AB16>(xq[2 * j], fo, bs[0], bs[1]);
-        mma16<AB16>(xq[2 * j + 1], fo, bs[2], bs[3]);
-        mma16<AB16>(xv[2 * j], fv, bs[0], bs[1]);
-        mma16<AB16>(xv[2 * j + 1], fv, bs[2], bs[3]);
-        mma16<AB16>(xe[2 * j], fe, bd[0], bd[1]);
-        mma16<AB16>(xe[2 * j + 1], fe, bd[2], bd[3]);
-      }
-    }
-    if (s.last_v) {
-      // q k^T and k k^T of this warp's 16 x 16 tile, where it reaches the lower triangle
-      float qk[2][4] = {}, kk[2][4] = {};
-      if (nq <= mt) {
-#pragma unroll 1
-        for (int ks = 0; ks < KD / 16; ++ks) {
-          uint32_t fq[4], fk[4], bk[4];
-          const uint32_t pan = (ks >> 2) * PANEL;
-          ldsm4(fq, a_addr(Q + pan, 16 * mt, 2 * (ks & 3), lane));
-          ldsm4(fk, a_addr(K + pan, 16 * mt, 2 * (ks & 3), lane));
-          ldsm4(bk, b_addr(K + pan, 16 * nq, 2 * (ks & 3), lane));
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            mma16<AB16>(qk[j], fq, bk[2 * j], bk[2 * j + 1]);
-            mma16<AB16>(kk[j], fk, bk[2 * j], bk[2 * j + 1]);
+      float dot = 0.f, later = 0.f;
+      {
+        const int64_t vs = gdr_slots(a, C) * a.HV, va = gdr_slots(a, C * ANCHOR) * a.HV;
+        for (int v = 0; v < (a.V + VT - 1) / VT; ++v) {
+          if ((tid >> 6) <= R.more) {
+            const int64_t at = (v * vs + R.sh + (int64_t)(tid >> 6) * a.HV) * C + (tid & 63);
+            dot += w.dotO[at] - w.dotV[at];
           }
+          if (tid < CHAIN_WARPS) later += w.anchor[(v * va + R.anchor) * CHAIN_WARPS + tid];
         }
       }
-      const int i0 = 16 * mt + g;
-      const float gh[2] = {ax[AX_GH + i0], ax[AX_GH + i0 + 8]}, gl[2] = {ax[AX_GL + i0], ax[AX_GL + i0 + 8]};
+      if (valid < C && R.first) {
+        pipe_wait(&S_.full[first_step & 1], (first_step >> 1) & 1, ab, err, 0x100);
+        // the rows past the document belong to another one: what a product sums over must be zero
+        for (int p = 0; p < 2 * NP; ++p) zero_rows(KQ + p * PANEL, 1, valid, tid, EPI);
+        fence_async_smem();
+        warp_arrive(&S_.kz);
+      }
+      pipe_wait(&S_.x_full, rec & 1, ab, err, 0x200);
+      tc_fence_after();
+      if (warp < 8) {
+        // [N ; W] and the scores' part of dbeta, columns c0 .. c0 + 31
+        const int c0 = 32 * (warp >> 2);
+        float z[32];
+        const uint32_t row = sb + L_W + (kside ? 0 : PANEL);
+        if (c0 > (quad & 1) * 32) {  // the block above the diagonal
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int j0 = 16 * nq + 8 * j + 2 * tq;
-        float db[2] = {0.f, 0.f};
+          for (int cc = 0; cc < 4; ++cc) sts128(row + sw128(i, c0 / 8 + cc), make_uint4(0, 0, 0, 0));
+          S_.db[quad][c0 + lane] = 0.f;
+        } else {
+          const float gh = ax[AX_GH + i], gl = ax[AX_GL + i];
+          const float sx = kside ? -1.f : a.scale;
+          const int top = i < valid ? (kside ? i - 1 : i) : -1;  // last column of this row
 #pragma unroll
-        for (int hr = 0; hr < 2; ++hr) {
-          const int i = i0 + 8 * hr;
-          float W[2], N[2];
+          for (int cc = 0; cc < 4; ++cc) {
+            float x[8], y[8];
+            tmem_ld8(tl + T_P + c0 + 8 * cc, x);
+            tmem_ld8(tl + T_B + c0 + 8 * cc, y);
+            uint32_t u[4];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int jj = j0 + e;
-            const bool on = jj <= i && i < valid;
-            const float d = on ? exp2f((gh[hr] - ax[AX_GH + jj]) + (gl[hr] - ax[AX_GL + jj])) : 0.f;
-            const float x = on ? d * pe[j][2 * hr + e] : 0.f, y = on && jj < i ? d * ve[j][2 * hr + e] : 0.f;
-            const float be = ax[AX_B + jj];
-            W[e] = a.scale * be * x;
-            N[e] = -be * y;
-            db[e] += a.scale * x * qk[j][2 * hr + e] - y * kk[j][2 * hr + e];
+            for (int e = 0; e < 8; e += 4) {
+              const int j = c0 + 8 * cc + e;
+              const float4 hj = *reinterpret_cast<const float4*>(ax + AX_GH + j), lj = *reinterpret_cast<const float4*>(ax + AX_GL + j);
+              const float4 bj = *reinterpret_cast<const float4*>(ax + AX_B + j);
+              const float h4[4] = {hj.x, hj.y, hj.z, hj.w}, l4[4] = {lj.x, lj.y, lj.z, lj.w}, b4[4] = {bj.x, bj.y, bj.z, bj.w};
+#pragma unroll
+              for (int f = 0; f < 4; ++f) {
+                const float d = j + f <= top ? sx * exp2f((gh - h4[f]) + (gl - l4[f])) * x[e + f] : 0.f;
+                z[8 * cc + e + f] = d * y[e + f];
+                x[e + f] = d * b4[f];
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[e] = pack2<AB16>(x[2 * e], x[2 * e + 1]);
+            sts128(row + sw128(i, c0 / 8 + cc), make_uint4(u[0], u[1], u[2], u[3]));
           }
-          const uint32_t at = sw128(i, 2 * nq + j) + tq * 4;
-          *reinterpret_cast<uint32_t*>(sm + L_W + at) = pack2<AB16>(W[0], W[1]);
-          *reinterpret_cast<uint32_t*>(sm + L_N + at) = pack2<AB16>(N[0], N[1]);
+          lane_sums<32>(z, lane);
+          S_.db[quad][c0 + lane] = z[0];
         }
+      } else {
+        // the first term of F, half of its columns, and k_i . X2_i
+        constexpr int KH = KD / 2;
+        const int hf = (warp - 8) >> 2;
+        const float g0 = kside ? -ax[AX_G + i] : ax[AX_SG + i], g1 = ax[AX_WB + i];
+        float ke = 0.f;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int k0 = 0; k0 < KH; k0 += 16) {
+          const int k = KH * hf + k0;
+          float x[16];
+          tmem_ld16(tl + T_X + k, x);
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) db[e] += __shfl_xor_sync(0xffffffffu, db[e], o);
-          if (g == 0) S_.db[mt][j0 + e] = db[e];
-        }
-      }
-      // the state's part of dq and dk, and k_j . (E dS1^T)_j
-      float ke[2] = {0.f, 0.f};
+          for (int e = 0; e < 16; ++e) x[e] *= g0;
+          if (kside) {
+            float y[16];
+            tmem_ld16(tl + T_X2 + k, y);
+            const uint32_t p = KQ + (k >> 6) * 2 * PANEL;
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int col = (KD / 4) * nq + 8 * j;
+            for (int cc = 0; cc < 2; ++cc) {
+              const uint4 kv = lds128(p + sw128(i, ((k & 63) >> 3) + cc));
+              const uint32_t u[4] = {kv.x, kv.y, kv.z, kv.w};
 #pragma unroll
-        for (int hr = 0; hr < 2; ++hr) {
-          const int i = i0 + 8 * hr;
-          const float2 kf = unpack2<AB16>(*reinterpret_cast<const uint32_t*>(
-              sm + (K - sb) + (col >> 6) * PANEL + sw128(i, (col & 63) >> 3) + tq * 4));
-          ke[hr] = fmaf(kf.x, xe[j][2 * hr], fmaf(kf.y, xe[j][2 * hr + 1], ke[hr]));
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2<AB16>(u[e]);
+                ke = fmaf(f.x, y[8 * cc + 2 * e], fmaf(f.y, y[8 * cc + 2 * e + 1], ke));
+              }
+            }
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float x = ax[AX_SG + i] * xq[j][2 * hr + e];
-            const float y = ax[AX_WB + i] * xe[j][2 * hr + e] - ax[AX_G + i] * xv[j][2 * hr + e];
-            dq[j][2 * hr + e] = ONE ? x : dq[j][2 * hr + e] + x;
-            dk[j][2 * hr + e] = ONE ? y : dk[j][2 * hr + e] + y;
+            for (int e = 0; e < 16; ++e) x[e] = fmaf(g1, y[e], x[e]);
           }
-        }
-      }
+          if (!R.first) {
+            float y[16];
+            tmem_ld16(tl + T_F + k, y);
 #pragma unroll
-      for (int hr = 0; hr < 2; ++hr) {
-        ke[hr] += __shfl_xor_sync(0xffffffffu, ke[hr], 1);
-        ke[hr] += __shfl_xor_sync(0xffffffffu, ke[hr], 2);
-        if (tq == 0) S_.ke[nq][i0 + 8 * hr] = ke[hr];
+            for (int e = 0; e < 16; ++e) x[e] += y[e];
+          }
+          uint32_t u[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(x[e]);
+          tmem_st8(tl + T_F + k, u);
+          tmem_st8(tl + T_F + k + 8, u + 8);
+        }
+        if (kside) S_.ke[hf][i] = ke;
+        tmem_st_wait();
       }
       {
-        const float r = warp_sum(warp < 2 ? later : dot + later);
-        if (lane == 0) S_.dg[warp] = r;
+        const float x = warp_sum(warp < 2 ? later : dot + later);
+        if (lane == 0) S_.dg[warp] = x;
       }
-      __syncthreads();
-      // W K, W^T Q, N K, N^T K
-#pragma unroll 1
-      for (int ks = 0; ks < 4; ++ks) {
-        uint32_t fw[4], fwt[4], fn[4], fnt[4];
-        ldsm4(fw, a_addr(sb + L_W, 16 * mt, 2 * ks, lane));
-        ldsm4t(fwt, at_addr(sb + L_W, 16 * ks, 2 * mt, lane));
-        ldsm4(fn, a_addr(sb + L_N, 16 * mt, 2 * ks, lane));
-        ldsm4t(fnt, at_addr(sb + L_N, 16 * ks, 2 * mt, lane));
-#pragma unroll
-        for (int j = 0; j < NT / 2; ++j) {
-          const int col = (KD / 4) * nq + 16 * j;
-          uint32_t bk[4], bq[4];
-          ldsm4t(bk, bt_addr(K + (col >> 6) * PANEL, 16 * ks, (col & 63) >> 3, lane));
-          ldsm4t(bq, bt_addr(Q + (col >> 6) * PANEL, 16 * ks, (col & 63) >> 3, lane));
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            mma16<AB16>(dq[2 * j + e], fw, bk[2 * e], bk[2 * e + 1]);
-            mma16<AB16>(dk[2 * j + e], fwt, bq[2 * e], bq[2 * e + 1]);
-            mma16<AB16>(dk[2 * j + e], fn, bk[2 * e], bk[2 * e + 1]);
-            mma16<AB16>(dk[2 * j + e], fnt, bk[2 * e], bk[2 * e + 1]);
-          }
-        }
-      }
+      fence_async_smem();
+      tc_fence_before();
+      warp_arrive(&S_.wn_ready);
+      bar_sync<1, EPI>();
       if (warp < 2) {
         const int j = tid;
-        const float ke4 = S_.ke[0][j] + S_.ke[1][j] + S_.ke[2][j] + S_.ke[3][j];
+        const int64_t at = (int64_t)(R.row0 + j) * a.HV + R.hv;
         if (j < valid)
-          gate_store(a.dbeta, a.beta_dtype, (int64_t)(s.row0 + j) * a.HV + s.hv,
-                     S_.db[0][j] + S_.db[1][j] + S_.db[2][j] + S_.db[3][j] + ax[AX_W + j] * ke4);
+          gate_store(a.dbeta, a.beta_dtype, at,
+                     S_.db[0][j] + S_.db[1][j] + S_.db[2][j] + S_.db[3][j] + ax[AX_W + j] * (S_.ke[0][j] + S_.ke[1][j]));
         // dg: reverse running sum; warp 1 holds tokens 32..63, whose sum warp 0 adds
-        float r = dot;
+        float x = dot;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const float u = __shfl_down_sync(0xffffffffu, r, o);
-          if (lane + o < 32) r += u;
+          const float u = __shfl_down_sync(0xffffffffu, x, o);
+          if (lane + o < 32) x += u;
         }
-        if (lane == 0 && warp == 1) S_.dg[16] = r;
+        if (lane == 0 && warp == 1) S_.dg[16] = x;
         bar_sync<2, 64>();
         float rest = S_.dg[lane & 15];
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
-        r += rest + (warp == 0 ? S_.dg[16] : 0.f);
+        x += rest + (warp == 0 ? S_.dg[16] : 0.f);
         // nothing decays at the first token of a document that starts from a zero state
-        if (j == 0 && s.zero_first) r = 0.f;
-        if (j < valid) gate_store(a.dg, a.g_dtype, (int64_t)(s.row0 + j) * a.HV + s.hv, r);
+        if (j == 0 && R.zero_first) x = 0.f;
+        if (j < valid) gate_store(a.dg, a.g_dtype, at, x);
       }
-    }
-    __syncthreads();  // the step's tiles, W, N and, after the last step, Q and K have been read
-    if (last) {
-      // dq over Q and dk over K, then out
+      pipe_wait(&S_.f_full, rec & 1, ab, err, 0x400);
+      tc_fence_after();
+      if (!R.last) bar_sync<1, EPI>();  // the sums are read before the next value head's are written
+      if (R.last) {
+        // dK over the K rows and dQ over the Q rows, then out
+        constexpr int KQTR = KD / 4;
+        const int k0 = KQTR * (warp >> 2);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int col = (KD / 4) * nq + 8 * j;
+        for (int k = k0; k < k0 + KQTR; k += 16) {
+          float x[16];
+          tmem_ld16(tl + T_F + k, x);
+          uint32_t u[8];
 #pragma unroll
-        for (int hr = 0; hr < 2; ++hr) {
-          const uint32_t at = (col >> 6) * PANEL + sw128(16 * mt + g + 8 * hr, (col & 63) >> 3) + tq * 4;
-          *reinterpret_cast<uint32_t*>(sm + (Q - sb) + at) = pack2<AB16>(dq[j][2 * hr], dq[j][2 * hr + 1]);
-          *reinterpret_cast<uint32_t*>(sm + (K - sb) + at) = pack2<AB16>(dk[j][2 * hr], dk[j][2 * hr + 1]);
+          for (int e = 0; e < 8; ++e) u[e] = pack2<AB16>(x[2 * e], x[2 * e + 1]);
+          const uint32_t p = KQ + (k >> 6) * 2 * PANEL;
+          sts128(p + sw128(quad * 32 + lane, (k & 63) >> 3), make_uint4(u[0], u[1], u[2], u[3]));
+          sts128(p + sw128(quad * 32 + lane, ((k & 63) >> 3) + 1), make_uint4(u[4], u[5], u[6], u[7]));
+        }
+        fence_async_smem();
+        bar_sync<1, EPI>();
+        if (valid == C) {
+          if (tid == 0) {
+            for (int p = 0; p < NP; ++p)
+              if (64 * p < a.K) {
+                tma_store_3d(&tmdk, sm + (KQ - sb) + 2 * p * PANEL, 64 * p, R.h, R.row0);
+                tma_store_3d(&tmdq, sm + (KQ - sb) + (2 * p + 1) * PANEL, 64 * p, R.h, R.row0);
+              }
+            bulk_commit();
+            bulk_wait_read();
+            mbar_arrive(&S_.qk_empty[R.qk]);
+          }
+        } else {
+          for (int e = tid; e < valid * 2 * NP * 8; e += EPI) {
+            const int t = e / (2 * NP * 8), x = e % (2 * NP * 8), which = x & 1, ch = x >> 1;
+            if (ch * 8 < a.K)
+              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(which ? a.dq : a.dk) +
+                                        ((int64_t)(R.row0 + t) * a.H + R.h) * a.K + ch * 8) =
+                  lds128(KQ + ((ch >> 3) * 2 + which) * PANEL + sw128(t, ch & 7));
+          }
+          bar_sync<1, EPI>();
+          if (tid == 0) mbar_arrive(&S_.qk_empty[R.qk]);
         }
       }
-      fence_async_smem();
-      __syncthreads();
-      if (valid == C) {
-        if (tid == 0) {
-          for (int i = 0; i < NP; ++i)
-            if (64 * i < a.K) {
-              tma_store_3d(&tmdq, sm + (Q - sb) + i * PANEL, 64 * i, head, row0);
-              tma_store_3d(&tmdk, sm + (K - sb) + i * PANEL, 64 * i, head, row0);
-            }
-          bulk_commit();
-          bulk_wait_read();
-        }
-      } else {
-        copy_rows(Q, reinterpret_cast<uint16_t*>(a.dq), row0, a.H, head, a.K, 0, valid, tid, THREADS);
-        copy_rows(K, reinterpret_cast<uint16_t*>(a.dk), row0, a.H, head, a.K, 0, valid, tid, THREADS);
-        __syncthreads();
-      }
     }
-    // the step is done: its description and buffers go to the one after the next.  A last step's dq and dk
-    // have left Q and K (thread 0 waited); the barrier at the end of the next step publishes the description.
-    if (tid == 0) load();
+    if (tid == 0) bulk_wait_all();
   }
-  if (tid == 0) bulk_wait_all();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 17) tmem_dealloc(tb, 512);
 }
 
-template <int AB16, int KD, bool ONE>
+template <int AB16, int KD>
 cudaError_t launch(const GdrArgs& a, const Ws& w) {
   const int64_t slots = gdr_slots(a, C), sh = slots * a.HV;
   CUtensorMap q, k, o, dv, e, s, ds, dq, dk;
@@ -443,26 +448,21 @@ cudaError_t launch(const GdrArgs& a, const Ws& w) {
   if (r == cudaSuccess) r = matrix_map(&ds, a, w.dS1, a.K, sh);
   if (r == cudaSuccess) r = token_map(&dq, a, a.dq, a.H, a.K);
   if (r == cudaSuccess) r = token_map(&dk, a, a.dk, a.H, a.K);
-  if (r == cudaSuccess) r = cudaFuncSetAttribute(grads_kernel<AB16, KD, ONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BYTES);
+  if (r == cudaSuccess) r = cudaFuncSetAttribute(grads_kernel<AB16, KD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)BYTES);
   if (r != cudaSuccess) return r;
   const int64_t items = slots * a.H;
   const unsigned grid = (unsigned)(items < 148 ? items : 148);  // one persistent block per SM
-  grads_kernel<AB16, KD, ONE><<<grid, THREADS, BYTES, a.stream>>>(q, k, o, dv, e, s, ds, dq, dk, a, w);
+  grads_kernel<AB16, KD><<<grid, THREADS, BYTES, a.stream>>>(q, k, o, dv, e, s, ds, dq, dk, a, w);
   return cudaGetLastError();
-}
-
-template <int AB16>
-cudaError_t pick(const GdrArgs& a, const Ws& w) {
-  const bool one = a.H == a.HV;
-  if (a.K <= 64) return one ? launch<AB16, 64, true>(a, w) : launch<AB16, 64, false>(a, w);
-  return one ? launch<AB16, 128, true>(a, w) : launch<AB16, 128, false>(a, w);
 }
 
 }  // namespace
 
 cudaError_t grads(const GdrArgs& a, const Ws& w, int* launches) {
   ++*launches;
-  return a.dtype == DT_BF16 ? pick<1>(a, w) : pick<0>(a, w);
+  const bool small = a.K <= 64;
+  if (a.dtype == DT_BF16) return small ? launch<1, 64>(a, w) : launch<1, 128>(a, w);
+  return small ? launch<0, 64>(a, w) : launch<0, 128>(a, w);
 }
 
 }  // namespace gdrtc
