@@ -31,7 +31,7 @@ size_t carve(const GdrArgs& a, bool bwd, Ws* w) {
     t.dotV = reinterpret_cast<float*>(take(nvt * sh * C * 4));
     const size_t ah = (size_t)gdr_slots(a, C * ANCHOR) * a.HV;
     t.Sf = reinterpret_cast<float*>(take(ah * a.K * a.V * 4));
-    t.anchor = reinterpret_cast<float*>(take(nvt * ah * CHAIN_WARPS * 4));
+    t.anchor = reinterpret_cast<float*>(take(nvt * ah * ANCHOR_PARTS * 4));
   }
   if (w) *w = t;
   return off;

@@ -198,12 +198,31 @@ __device__ __forceinline__ void copy_rows(uint32_t tile, uint16_t* dst, int64_t 
   }
 }
 
-// Warps of the scans (832 threads): 0-7 output (two per TMEM quadrant, half the tokens each), 8-23 chain (four
-// per quadrant, a quarter of the tokens and of K each), 24 TMA, 25 MMA.  A phase of the chain is bound by how
-// fast one warp's instructions go, not by the SM's issue rate (eight chain and four output warps took
-// 6.7 k cycles a chunk forward, 10-10.8 k in the backward's two scans).
-constexpr int SCAN_THREADS = 832, W_CHAIN = 8, W_TMA = 24, W_MMA = 25;
-constexpr int OUT_THREADS = 256, CHAIN_THREADS = 512, OUT_WARPS = 8, CHAIN_WARPS = 16;
+// Warps of a scan: OW for the output (a share of the tokens of one TMEM quadrant each), CW for the chain (a share
+// of the tokens and of K each), then a warpgroup of which the first warp loads and the second issues MMAs.
+// RC, RO, RX: registers of a thread by role, redistributed from an even share.
+template <int CW, int OW, int RC, int RO, int RX>
+struct ScanWarps {
+  static constexpr int CHAIN = OW, TMA = OW + CW, MMA = TMA + 1, THREADS = 32 * (TMA + 4);
+  static constexpr int CHAIN_WARPS = CW, OUT_WARPS = OW, CHAIN_THREADS = 32 * CW, OUT_THREADS = 32 * OW;
+  static constexpr int CT = 256 / CW, OT = 256 / OW;  // tokens of a chain and of an output thread
+  static constexpr int EVEN = 65536 / THREADS / 8 * 8;
+  static_assert(32 * CW * RC + 32 * OW * RO + 128 * RX <= THREADS * EVEN, "registers");
+  template <int R>
+  static __device__ __forceinline__ void set_regs() {
+    if (R > EVEN) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+    if (R < EVEN) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
+  }
+  static __device__ __forceinline__ void chain_regs() { set_regs<RC>(); }
+  static __device__ __forceinline__ void out_regs() { set_regs<RO>(); }
+  static __device__ __forceinline__ void rest_regs() { set_regs<RX>(); }
+};
+// Measured at B=8, T=4096, H=16, K=V=128, bf16 (prep and scan; whole backward): 8 and 4 warps 367 us and
+// 1190 us, 16 and 8 warps 400 us and 1127 us.  The backward's scans also stage the states and form a dot
+// product per token, which four output warps do not finish within a chunk.
+using FwdWarps = ScanWarps<8, 4, 144, 128, 96>;
+using BwdWarps = ScanWarps<16, 8, 72, 72, 72>;
+constexpr int ANCHOR_PARTS = BwdWarps::CHAIN_WARPS;
 
 // pipe_wait for the MMA thread: polls without suspending (a suspended try_wait wakes a few hundred cycles
 // late, and this thread's waits are all on the chunk's critical path), bounded like the others.

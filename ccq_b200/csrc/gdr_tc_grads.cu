@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int64_t at = (v * vs + R.sh + (int64_t)(tid >> 6) * a.HV) * C + (tid & 63);
             dot += w.dotO[at] - w.dotV[at];
           }
-          if (tid < CHAIN_WARPS) later += w.anchor[(v * va + R.anchor) * CHAIN_WARPS + tid];
+          if (tid < ANCHOR_PARTS) later += w.anchor[(v * va + R.anchor) * ANCHOR_PARTS + tid];
         }
       }
       if (valid < C && R.first) {

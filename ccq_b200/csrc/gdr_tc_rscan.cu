@@ -37,10 +37,11 @@ constexpr uint32_t L_BYTES = L_SMALL + sizeof(Small) + 1024;
 static_assert(L_BYTES <= 232448, "shared memory");
 
 template <int AB16, int KD>
-__global__ void __launch_bounds__(SCAN_THREADS, 1)
+__global__ void __launch_bounds__(BwdWarps::THREADS, 1)
     rscan_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                  const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmo,
                  const __grid_constant__ CUtensorMap tmdv, const __grid_constant__ CUtensorMap tms, GdrArgs a, Ws w) {
+  using G = BwdWarps;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Small& S_ = *reinterpret_cast<Small*>(sm + L_SMALL);
@@ -53,18 +54,19 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   const int64_t sh0 = gdr_slot0(a, n, sq, C) * a.HV + hv;  // chunk c is at sh0 + c * HV
   const int64_t st = ((int64_t)n * a.HV + hv) * a.K * a.V;
   constexpr int NP = KD / 64;  // panels of K and Q
+  constexpr int CT = G::CT, OT = G::OT;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&S_.full[i], 1);
-      mbar_init(&S_.empty[i], 1 + CHAIN_WARPS + OUT_WARPS);  // last commit, every chain and output warp
+      mbar_init(&S_.empty[i], 1 + G::CHAIN_WARPS + G::OUT_WARPS);  // last commit, every chain and output warp
     }
-    mbar_init(&S_.s_ready, CHAIN_WARPS);
-    mbar_init(&S_.e_ready, CHAIN_WARPS);
-    mbar_init(&S_.f_ready, CHAIN_WARPS);
-    mbar_init(&S_.f_read, OUT_WARPS);
-    mbar_init(&S_.g_ready, OUT_WARPS);
-    mbar_init(&S_.kz, OUT_WARPS);
+    mbar_init(&S_.s_ready, G::CHAIN_WARPS);
+    mbar_init(&S_.e_ready, G::CHAIN_WARPS);
+    mbar_init(&S_.f_ready, G::CHAIN_WARPS);
+    mbar_init(&S_.f_read, G::OUT_WARPS);
+    mbar_init(&S_.g_ready, G::OUT_WARPS);
+    mbar_init(&S_.kz, G::OUT_WARPS);
     mbar_init(&S_.y_full, 1);
     mbar_init(&S_.f_full, 1);
     mbar_init(&S_.d_full, 1);
@@ -72,7 +74,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
     S_.abort = 0;
     fence_barrier_init();
   }
-  if (warp == W_MMA) tmem_alloc(&S_.tmem, 512);
+  if (warp == G::MMA) tmem_alloc(&S_.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -81,7 +83,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   int* err = w.err;
   const bool part = sq.len % C != 0;  // the last chunk, the first one here, is partial
 
-  if (warp == W_TMA) {
+  if (warp >= G::TMA) G::rest_regs();
+  if (warp == G::TMA) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
       int issued = 0;
@@ -107,7 +110,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       // never leave the block with copies in flight
       for (int t = (issued > 2 ? issued - 2 : 0); t < issued; ++t) own_copy_wait(&S_.full[t & 1], (t >> 1) & 1, ab, err, 2);
     }
-  } else if (warp == W_MMA) {
+  } else if (warp == G::MMA) {
     // ------------------------------------------------------------------ MMA issuer
     if (lane == 0) {
       const uint32_t id_y = idesc_f16(128, 64, AB16, 0, 0), id_z = idesc_f16(128, 64, AB16, 1, 1);
@@ -170,10 +173,13 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       umma_commit(&S_.done);  // TMEM is freed only after every issued MMA has completed
       mbar_wait(&S_.done, 0);
     }
-  } else if (warp >= W_CHAIN) {
+  } else if (warp > G::MMA) {
+    // completes the warpgroup
+  } else if (warp >= G::CHAIN) {
     // ------------------------------------------------------------------ chain: dE, Gam dV, dS
-    constexpr int KH = KD / 4;  // columns of K this thread keeps
-    const int quad = warp & 3, hh = (warp - W_CHAIN) >> 2;
+    G::chain_regs();
+    constexpr int KH = 4 * KD / G::CHAIN_WARPS;  // columns of K this thread keeps
+    const int quad = warp & 3, hh = (warp - G::CHAIN) >> 2;
     const int vl = quad * 32 + lane;
     const bool vin = v0 + vl < a.V;
     const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
@@ -220,73 +226,82 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
           if (KH * hh + i < a.K) d = fmaf(S[i], g[(int64_t)(KH * hh + i) * a.V], d);
       }
       d = warp_sum(d);
-      if (lane == 0) w.anchor[((int64_t)blockIdx.y * anchors * a.HV + at) * CHAIN_WARPS + warp - W_CHAIN] = d;
+      if (lane == 0) w.anchor[((int64_t)blockIdx.y * anchors * a.HV + at) * G::CHAIN_WARPS + warp - G::CHAIN] = d;
     };
     if (nch > 0) {
       put_state(0);
       put_anchor((nch - 1) / ANCHOR, a.dfinal_state == nullptr);
     }
-    const int i0 = 16 * hh;
+    const int i0 = CT * hh;
     for (int t = 0; t < nch; ++t) {
       const int s = t & 1, ph = t & 1, c = nch - 1 - t;
       const float* ax = reinterpret_cast<const float*>(sm + s * L_STAGE + L_AX);
       pipe_wait(&S_.full[s], (t >> 1) & 1, ab, err, 0x400);
       pipe_wait(&S_.y_full, ph, ab, err, 0x800);
       tc_fence_after();
-      float x[16];
-      tmem_ld16(tl + T_Z + i0, x);
 #pragma unroll
-      for (int i = 0; i < 16; i += 8) {
-        float y[8];
-        tmem_ld8(tl + T_Y + i0 + i, y);
+      for (int i = 0; i < CT; i += 16) {
+        float x[16];
+        tmem_ld16(tl + T_Z + i0 + i, x);
 #pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + i + j);
-          const float bb[4] = {b.x, b.y, b.z, b.w};
-          fma2(x + i + j, bb, y + j, x + i + j);
-          fma2(x + i + j + 2, bb + 2, y + j + 2, x + i + j + 2);
+        for (int k = 0; k < 16; k += 8) {
+          float y[8];
+          tmem_ld8(tl + T_Y + i0 + i + k, y);
+#pragma unroll
+          for (int j = 0; j < 8; j += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + i + k + j);
+            const float bb[4] = {b.x, b.y, b.z, b.w};
+            float* z = x + k + j;
+            fma2(z, bb, y + j, z);
+            fma2(z + 2, bb + 2, y + j + 2, z + 2);
+          }
         }
+        st_split16<AB16>(tl + T_EH + (i0 + i) / 2, tl + T_EL + (i0 + i) / 2, x);
       }
-      st_split16<AB16>(tl + T_EH + 8 * hh, tl + T_EL + 8 * hh, x);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.e_ready);
       pipe_wait(&S_.f_full, ph, ab, err, 0x1000);
       tc_fence_after();
-      tmem_ld16(tl + T_Y + i0, x);
 #pragma unroll
-      for (int i = 0; i < 16; i += 8) {
-        float y[8];
-        tmem_ld8(tl + T_Y + 64 + i0 + i, y);
+      for (int i = 0; i < CT; i += 16) {
+        float x[16];
+        tmem_ld16(tl + T_Y + i0 + i, x);
 #pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(ax + AX_G + i0 + i + j);
-          const float bb[4] = {-b.x, -b.y, -b.z, -b.w};
-          float* z = x + i + j;
-          add2f(z, z, y + j);
-          add2f(z + 2, z + 2, y + j + 2);
-          mul2f(z, z, bb);
-          mul2f(z + 2, z + 2, bb + 2);
+        for (int k = 0; k < 16; k += 8) {
+          float y[8];
+          tmem_ld8(tl + T_Y + 64 + i0 + i + k, y);
+#pragma unroll
+          for (int j = 0; j < 8; j += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(ax + AX_G + i0 + i + k + j);
+            const float bb[4] = {-b.x, -b.y, -b.z, -b.w};
+            float* z = x + k + j;
+            add2f(z, z, y + j);
+            add2f(z + 2, z + 2, y + j + 2);
+            mul2f(z, z, bb);
+            mul2f(z + 2, z + 2, bb + 2);
+          }
         }
+        st_split16<AB16>(tl + T_EH + (i0 + i) / 2, tl + T_EL + (i0 + i) / 2, x);
       }
-      st_split16<AB16>(tl + T_EH + 8 * hh, tl + T_EL + 8 * hh, x);
       const float gam[2] = {ax[AX_GC], ax[AX_GC]};
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.f_ready);
-      if (warp != W_CHAIN) warp_arrive(&S_.empty[s]);
+      if (warp != G::CHAIN) warp_arrive(&S_.empty[s]);
       pipe_wait(&S_.d_full, ph, ab, err, 0x2000);
       tc_fence_after();
 #pragma unroll
       for (int i = 0; i < KH; i += 16) {
+        float x[16];
         tmem_ld16(tl + T_D + KH * hh + i, x);
 #pragma unroll
         for (int j = 0; j < 16; j += 2) fma2(S + i + j, gam, S + i + j, x + j);
       }
       if (c > 0) put_state(sb + s * L_STAGE + L_KQ);  // every product with the K and Q rows is done: their space is the staging
       fence_async_smem();
-      bar_sync<2, CHAIN_THREADS>();
-      if (threadIdx.x == 32 * W_CHAIN) {
+      bar_sync<2, G::CHAIN_THREADS>();
+      if (threadIdx.x == 32 * G::CHAIN) {
         if (c > 0)
           for (int i = 0; i < NP; ++i)
             if (64 * i < a.K)
@@ -296,7 +311,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       }
       if (c > 0 && c % ANCHOR == 0) put_anchor(c / ANCHOR - 1, false);
     }
-    if (threadIdx.x == 32 * W_CHAIN) bulk_wait_all();
+    if (threadIdx.x == 32 * G::CHAIN) bulk_wait_all();
     if (a.dinitial_state && vin) {
 #pragma unroll
       for (int i = 0; i < KH; ++i) {
@@ -306,7 +321,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------------ output: scaled dO, dV, V . dV
-    const int quad = warp & 3, j0 = 32 * (warp >> 2);  // tokens j0 .. j0 + 31
+    G::out_regs();
+    const int quad = warp & 3, j0 = OT * (warp >> 2);  // tokens j0 .. j0 + OT - 1
     const int vl = quad * 32 + lane;
     const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
     const int64_t slots = gdr_slots(a, C);
@@ -319,8 +335,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       pipe_wait(&S_.full[s], (t >> 1) & 1, ab, err, 0x4000);
       if (valid < C) {
         // the rows past the document belong to another one: what a product sums over must be zero
-        for (int i = 0; i < 2 * NP; ++i) zero_rows(p + L_KQ + i * PANEL, 1, valid, threadIdx.x, OUT_THREADS);
-        zero_rows(p + L_DO, 2, valid, threadIdx.x, OUT_THREADS);
+        for (int i = 0; i < 2 * NP; ++i) zero_rows(p + L_KQ + i * PANEL, 1, valid, threadIdx.x, G::OUT_THREADS);
+        zero_rows(p + L_DO, 2, valid, threadIdx.x, G::OUT_THREADS);
         fence_async_smem();
         warp_arrive(&S_.kz);
       }
@@ -329,7 +345,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       {
         const Column D(p + L_DO, vl);
 #pragma unroll
-        for (int i = j0; i < j0 + 32; i += 16) {
+        for (int i = j0; i < j0 + OT; i += 16) {
           float x[16];
 #pragma unroll
           for (int j = 0; j < 16; j += 4) {
@@ -344,13 +360,13 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.g_ready);
-      float y[32];
+      float y[OT];
       pipe_wait(&S_.f_full, ph, ab, err, 0x10000);
       tc_fence_after();
-      tmem_ld32(tl + T_Y + j0, y);
 #pragma unroll
-      for (int i = 0; i < 32; i += 16) {
+      for (int i = 0; i < OT; i += 16) {
         float x[16];
+        tmem_ld16(tl + T_Y + j0 + i, y + i);
         tmem_ld16(tl + T_Y + 64 + j0 + i, x);
 #pragma unroll
         for (int j = 0; j < 16; j += 2) add2f(y + i + j, y + i + j, x + j);
@@ -358,17 +374,18 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       tc_fence_before();
       warp_arrive(&S_.f_read);
       if (threadIdx.x == 0) bulk_wait_read();  // the stores of the chunk before have read the tile
-      bar_sync<1, OUT_THREADS>();
+      bar_sync<1, G::OUT_THREADS>();
       const Column O(sb + L_OUT, vl), V(p + L_V, vl);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) sts16(O.at(j0 + i), f2h<AB16>(y[i]));
+      for (int i = 0; i < OT; ++i) sts16(O.at(j0 + i), f2h<AB16>(y[i]));
 #pragma unroll
-      for (int i = 0; i < 32; ++i) y[i] = j0 + i < valid ? y[i] * h2f<AB16>(lds16(V.at(j0 + i))) : 0.f;
+      for (int i = 0; i < OT; ++i) y[i] = j0 + i < valid ? y[i] * h2f<AB16>(lds16(V.at(j0 + i))) : 0.f;
       warp_arrive(&S_.empty[s]);
-      lane_sums<32>(y, lane);
-      S_.red[quad][j0 + lane] = y[0];
+      lane_sums<OT>(y, lane);
+#pragma unroll
+      for (int i = 0; i < OT / 32; ++i) S_.red[quad][j0 + lane * (OT / 32) + i] = y[i];
       fence_async_smem();
-      bar_sync<1, OUT_THREADS>();
+      bar_sync<1, G::OUT_THREADS>();
       if (valid == C) {
         if (threadIdx.x == 0) {
           tma_store_3d(&tmdv, sm + L_OUT, v0, hv, (int)row0);
@@ -376,21 +393,21 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
           bulk_commit();
         }
       } else {
-        copy_rows(sb + L_OUT, reinterpret_cast<uint16_t*>(a.dv), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, OUT_THREADS);
+        copy_rows(sb + L_OUT, reinterpret_cast<uint16_t*>(a.dv), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, G::OUT_THREADS);
       }
       if (threadIdx.x < C) {
         const int i = threadIdx.x;
         w.dotV[((int64_t)blockIdx.y * slots * a.HV + sh0 + (int64_t)c * a.HV) * C + i] =
             S_.red[0][i] + S_.red[1][i] + S_.red[2][i] + S_.red[3][i];
       }
-      bar_sync<1, OUT_THREADS>();  // the sums are read before the next chunk's are written
+      bar_sync<1, G::OUT_THREADS>();  // the sums are read before the next chunk's are written
     }
     if (threadIdx.x == 0) bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == W_MMA) tmem_dealloc(tb, 512);
+  if (warp == G::MMA) tmem_dealloc(tb, 512);
 }
 
 template <int AB16, int KD>
@@ -405,7 +422,7 @@ cudaError_t launch(const GdrArgs& a, const Ws& w) {
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(rscan_kernel<AB16, KD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L_BYTES);
   if (e != cudaSuccess) return e;
-  rscan_kernel<AB16, KD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), SCAN_THREADS, L_BYTES, a.stream>>>(q, k, v, o, dv, st, a, w);
+  rscan_kernel<AB16, KD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), BwdWarps::THREADS, L_BYTES, a.stream>>>(q, k, v, o, dv, st, a, w);
   return cudaGetLastError();
 }
 

@@ -21,6 +21,8 @@
 //
 // TMEM columns: S hi, S lo (64 each), X | Y, then dS (128), E, then E P^T
 // (128), Gam X / E as operands (64), w beta E as operand (64): all 512.  Every wait is bounded; see tc_common.cuh.
+#include <type_traits>
+
 #include "gdr_tc.cuh"
 
 namespace ccq {
@@ -38,6 +40,9 @@ struct Small {
 };
 
 template <bool BWD>
+using Warps = std::conditional_t<BWD, BwdWarps, FwdWarps>;
+
+template <bool BWD>
 struct Lay {  // offsets of one stage, then of the rest
   static constexpr uint32_t KQ = 0, V = 2 * TILE, DO = 3 * TILE, M = (BWD ? 4 : 3) * TILE, AX = M + MATS;
   static constexpr uint32_t STAGE = (AX + AX_N * 4 + 1023) & ~1023u;
@@ -47,11 +52,12 @@ struct Lay {  // offsets of one stage, then of the rest
 static_assert(Lay<true>::BYTES <= 232448 && Lay<false>::BYTES <= 232448, "shared memory");
 
 template <int AB16, int KD, bool BWD>
-__global__ void __launch_bounds__(SCAN_THREADS, 1)
+__global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
     scan_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                 const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmo,
                 const __grid_constant__ CUtensorMap tms, const __grid_constant__ CUtensorMap tme, GdrArgs a, Ws w) {
   using L = Lay<BWD>;
+  using G = Warps<BWD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Small& S_ = *reinterpret_cast<Small*>(sm + L::SMALL);
@@ -64,27 +70,28 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   const int64_t sh0 = gdr_slot0(a, n, sq, C) * a.HV + hv;  // chunk c is at sh0 + c * HV
   const int64_t st = ((int64_t)n * a.HV + hv) * a.K * a.V;
   constexpr int NP = KD / 64;  // panels of K and Q
+  constexpr int CT = G::CT, OT = G::OT;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&S_.full[i], 1);
-      mbar_init(&S_.empty[i], 1 + CHAIN_WARPS + OUT_WARPS);  // last commit, every chain and output warp
+      mbar_init(&S_.empty[i], 1 + G::CHAIN_WARPS + G::OUT_WARPS);  // last commit, every chain and output warp
     }
-    mbar_init(&S_.s_ready, CHAIN_WARPS);
-    mbar_init(&S_.r_ready, CHAIN_WARPS);
-    mbar_init(&S_.u_ready, CHAIN_WARPS);
+    mbar_init(&S_.s_ready, G::CHAIN_WARPS);
+    mbar_init(&S_.r_ready, G::CHAIN_WARPS);
+    mbar_init(&S_.u_ready, G::CHAIN_WARPS);
     mbar_init(&S_.x_full, 1);
     mbar_init(&S_.u_full, 1);
     mbar_init(&S_.d_full, 1);
     mbar_init(&S_.o_full, 1);
-    mbar_init(&S_.o1_read, OUT_WARPS);
-    mbar_init(&S_.o2_free, OUT_WARPS);
-    mbar_init(&S_.kz, OUT_WARPS);
+    mbar_init(&S_.o1_read, G::OUT_WARPS);
+    mbar_init(&S_.o2_free, G::OUT_WARPS);
+    mbar_init(&S_.kz, G::OUT_WARPS);
     mbar_init(&S_.done, 1);
     S_.abort = 0;
     fence_barrier_init();
   }
-  if (warp == W_MMA) tmem_alloc(&S_.tmem, 512);
+  if (warp == G::MMA) tmem_alloc(&S_.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -92,7 +99,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   volatile int* ab = &S_.abort;
   int* err = w.err;
 
-  if (warp == W_TMA) {
+  if (warp >= G::TMA) G::rest_regs();
+  if (warp == G::TMA) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
       int issued = 0;
@@ -120,7 +128,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       // never leave the block with copies in flight
       for (int c = (issued > 2 ? issued - 2 : 0); c < issued; ++c) own_copy_wait(&S_.full[c & 1], (c >> 1) & 1, ab, err, 2);
     }
-  } else if (warp == W_MMA) {
+  } else if (warp == G::MMA) {
     // ------------------------------------------------------------------ MMA issuer
     if (lane == 0) {
       const uint32_t id64 = idesc_f16(128, 64, AB16, 0, 0), id128 = idesc_f16(128, 128, AB16, 0, 0);
@@ -174,10 +182,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       umma_commit(&S_.done);  // TMEM is freed only after every issued MMA has completed
       mbar_wait(&S_.done, 0);
     }
-  } else if (warp >= W_CHAIN) {
+  } else if (warp > G::MMA) {
+    // completes the warpgroup
+  } else if (warp >= G::CHAIN) {
     // ------------------------------------------------------------------ chain: Gam X, E, S
-    constexpr int KH = KD / 4;  // columns of K this thread keeps
-    const int quad = warp & 3, hh = (warp - W_CHAIN) >> 2;
+    G::chain_regs();
+    constexpr int KH = 4 * KD / G::CHAIN_WARPS;  // columns of K this thread keeps
+    constexpr int NY = G::CT >= 32 ? 16 : 8;  // columns per load where registers are short
+    const int quad = warp & 3, hh = (warp - G::CHAIN) >> 2;
     const int vl = quad * 32 + lane;
     const bool vin = v0 + vl < a.V;
     const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
@@ -219,65 +231,72 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       const int s = c & 1, ph = c & 1;
       const uint32_t p = sb + s * L::STAGE;
       const float* ax = reinterpret_cast<const float*>(sm + s * L::STAGE + L::AX);
-      const int i0 = 16 * hh;
+      const int i0 = CT * hh;
       pipe_wait(&S_.full[s], (c >> 1) & 1, ab, err, 0x400);
       pipe_wait(&S_.x_full, ph, ab, err, 0x800);
       tc_fence_after();
-      float x[16];
-      tmem_ld16(tl + T_X + i0, x);
 #pragma unroll
-      for (int j = 0; j < 16; j += 4) {
-        const float4 b = *reinterpret_cast<const float4*>(ax + AX_G + i0 + j);
-        const float bb[4] = {-b.x, -b.y, -b.z, -b.w};
-        mul2f(x + j, x + j, bb);
-        mul2f(x + j + 2, x + j + 2, bb + 2);
+      for (int i = 0; i < CT; i += 16) {
+        float x[16];
+        tmem_ld16(tl + T_X + i0 + i, x);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(ax + AX_G + i0 + i + j);
+          const float bb[4] = {-b.x, -b.y, -b.z, -b.w};
+          mul2f(x + j, x + j, bb);
+          mul2f(x + j + 2, x + j + 2, bb + 2);
+        }
+        st_split16<AB16>(tl + T_RH + (i0 + i) / 2, tl + T_RL + (i0 + i) / 2, x);
       }
-      st_split16<AB16>(tl + T_RH + 8 * hh, tl + T_RL + 8 * hh, x);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.r_ready);
       pipe_wait(&S_.u_full, ph, ab, err, 0x1000);
       tc_fence_after();
       const float gam[2] = {ax[AX_GC], ax[AX_GC]};
-      tmem_ld16(tl + T_D + i0, x);
 #pragma unroll
-      for (int i = 0; i < 16; i += 8) {
-        float y[8];
-        tmem_ld8(tl + T_D + 64 + i0 + i, y);
+      for (int i = 0; i < CT; i += 16) {
+        float x[16];
+        tmem_ld16(tl + T_D + i0 + i, x);
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) add2f(x + i + j, x + i + j, y + j);
-      }
-      {
+        for (int k = 0; k < 16; k += NY) {
+          float y[NY];
+          if (NY == 16) tmem_ld16(tl + T_D + 64 + i0 + i + k, y);
+          else tmem_ld8(tl + T_D + 64 + i0 + i + k, y);
+#pragma unroll
+          for (int j = 0; j < NY; j += 2) add2f(x + k + j, x + k + j, y + j);
+        }
         uint32_t hi[8], lo[8];
         split<AB16, 8>(x, hi, lo);
-        tmem_st8(tl + T_RH + 8 * hh, hi);
-        tmem_st8(tl + T_RL + 8 * hh, lo);
+        tmem_st8(tl + T_RH + (i0 + i) / 2, hi);
+        tmem_st8(tl + T_RL + (i0 + i) / 2, lo);
         if (BWD) {  // E, transposed, to the staging panel
-          sts128(sb + L::OUT + sw128(vl, i0 >> 3), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-          sts128(sb + L::OUT + sw128(vl, (i0 >> 3) + 1), make_uint4(hi[4], hi[5], hi[6], hi[7]));
+          sts128(sb + L::OUT + sw128(vl, (i0 + i) >> 3), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+          sts128(sb + L::OUT + sw128(vl, ((i0 + i) >> 3) + 1), make_uint4(hi[4], hi[5], hi[6], hi[7]));
         }
-      }
 #pragma unroll
-      for (int j = 0; j < 16; j += 4) {
-        const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + j);
-        const float bb[4] = {b.x, b.y, b.z, b.w};
-        mul2f(x + j, x + j, bb);
-        mul2f(x + j + 2, x + j + 2, bb + 2);
+        for (int j = 0; j < 16; j += 4) {
+          const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + i + j);
+          const float bb[4] = {b.x, b.y, b.z, b.w};
+          mul2f(x + j, x + j, bb);
+          mul2f(x + j + 2, x + j + 2, bb + 2);
+        }
+        st_split16<AB16>(tl + T_WH + (i0 + i) / 2, tl + T_WL + (i0 + i) / 2, x);
       }
-      st_split16<AB16>(tl + T_WH + 8 * hh, tl + T_WL + 8 * hh, x);
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.u_ready);
-      if (!BWD || warp != W_CHAIN) warp_arrive(&S_.empty[s]);
+      if (!BWD || warp != G::CHAIN) warp_arrive(&S_.empty[s]);
       if (BWD) {
         fence_async_smem();
-        bar_sync<2, CHAIN_THREADS>();
-        if (threadIdx.x == 32 * W_CHAIN) store_panel(&tme, sm + L::OUT, 0, v0, a.V, sh0 + (int64_t)c * a.HV);
+        bar_sync<2, G::CHAIN_THREADS>();
+        if (threadIdx.x == 32 * G::CHAIN) store_panel(&tme, sm + L::OUT, 0, v0, a.V, sh0 + (int64_t)c * a.HV);
       }
       pipe_wait(&S_.d_full, ph, ab, err, 0x2000);
       tc_fence_after();
 #pragma unroll
       for (int i = 0; i < KH; i += 16) {
+        float x[16];
         tmem_ld16(tl + T_X + KH * hh + i, x);
 #pragma unroll
         for (int j = 0; j < 16; j += 2) fma2(S + i + j, gam, S + i + j, x + j);
@@ -285,8 +304,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       if (c + 1 < nch) put_state(p + L::KQ);  // every product with the K and Q rows is done: their space is the staging
       if (BWD) {
         fence_async_smem();
-        bar_sync<2, CHAIN_THREADS>();
-        if (threadIdx.x == 32 * W_CHAIN) {
+        bar_sync<2, G::CHAIN_THREADS>();
+        if (threadIdx.x == 32 * G::CHAIN) {
           if (c + 1 < nch)
             for (int i = 0; i < NP; ++i)
               if (64 * i < a.K)
@@ -294,7 +313,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
           bulk_wait_read();  // then the stage, and the panel of E, may be written again
           mbar_arrive(&S_.empty[s]);
         }
-        bar_sync<2, CHAIN_THREADS>();
+        bar_sync<2, G::CHAIN_THREADS>();
       }
       if (BWD && vin && ((c + 1) % ANCHOR == 0 || c + 1 == nch)) {
         float* g = w.Sf + ((gdr_slot0(a, n, sq, C * ANCHOR) + c / ANCHOR) * a.HV + hv) * a.K * a.V + v0 + vl;
@@ -303,7 +322,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
           if (KH * hh + i < a.K) g[(int64_t)(KH * hh + i) * a.V] = S[i];
       }
     }
-    if (BWD && threadIdx.x == 32 * W_CHAIN) bulk_wait_all();
+    if (BWD && threadIdx.x == 32 * G::CHAIN) bulk_wait_all();
     if (!BWD && a.final_state && vin) {
 #pragma unroll
       for (int i = 0; i < KH; ++i) {
@@ -313,7 +332,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
     }
   } else {
     // ------------------------------------------------------------------ output
-    const int quad = warp & 3, j0 = 32 * (warp >> 2);  // tokens j0 .. j0 + 31
+    G::out_regs();
+    const int quad = warp & 3, j0 = OT * (warp >> 2);  // tokens j0 .. j0 + OT - 1
     const int vl = quad * 32 + lane;
     const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
     const int64_t slots = gdr_slots(a, C);
@@ -326,19 +346,20 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       pipe_wait(&S_.full[s], (c >> 1) & 1, ab, err, 0x4000);
       if (valid < C) {
         // the rows past the document belong to another one: what a product sums over must be zero
-        for (int i = 0; i < NP; ++i) zero_rows(p + L::KQ + 2 * i * PANEL, 1, valid, threadIdx.x, OUT_THREADS);
-        zero_rows(p + L::V, 2, valid, threadIdx.x, OUT_THREADS);
+        for (int i = 0; i < NP; ++i) zero_rows(p + L::KQ + 2 * i * PANEL, 1, valid, threadIdx.x, G::OUT_THREADS);
+        zero_rows(p + L::V, 2, valid, threadIdx.x, G::OUT_THREADS);
         fence_async_smem();
         warp_arrive(&S_.kz);
       }
-      float y[32];
+      float y[OT];
       pipe_wait(&S_.x_full, ph, ab, err, 0x8000);
       tc_fence_after();
-      tmem_ld32(tl + T_X + 64 + j0, y);
+#pragma unroll
+      for (int i = 0; i < OT; i += 32) tmem_ld32(tl + T_X + 64 + j0 + i, y + i);
       tc_fence_before();
       warp_arrive(&S_.o1_read);
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) {
+      for (int i = 0; i < OT; i += 4) {
         const float4 b = *reinterpret_cast<const float4*>(ax + AX_SG + j0 + i);
         y[i] *= b.x;
         y[i + 1] *= b.y;
@@ -348,11 +369,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
       pipe_wait(&S_.o_full, ph, ab, err, 0x10000);
       tc_fence_after();
 #pragma unroll
-      for (int i = 0; i < 64; i += 16) {
+      for (int i = 0; i < OT; i += 16) {
         float x[16];
-        tmem_ld16(tl + T_D + 64 * (i >> 5) + j0 + (i & 16), x);
+        tmem_ld16(tl + T_D + j0 + i, x);
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) add2f(y + (i & 16) + j, y + (i & 16) + j, x + j);
+        for (int j = 0; j < 16; j += 2) add2f(y + i + j, y + i + j, x + j);
+        tmem_ld16(tl + T_D + 64 + j0 + i, x);
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) add2f(y + i + j, y + i + j, x + j);
       }
       tc_fence_before();
       warp_arrive(&S_.o2_free);
@@ -360,36 +384,37 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
         warp_arrive(&S_.empty[s]);
         const uint32_t out = sb + L::OUT;
         if (threadIdx.x == 0) bulk_wait_read();  // the stores of the chunk before have read the tile
-        bar_sync<1, OUT_THREADS>();
+        bar_sync<1, G::OUT_THREADS>();
         const Column O(out, vl);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) sts16(O.at(j0 + i), f2h<AB16>(y[i]));
+        for (int i = 0; i < OT; ++i) sts16(O.at(j0 + i), f2h<AB16>(y[i]));
         if (valid == C) {
           fence_async_smem();
-          bar_sync<1, OUT_THREADS>();
+          bar_sync<1, G::OUT_THREADS>();
           if (threadIdx.x == 0) {
             tma_store_3d(&tmo, sm + L::OUT, v0, hv, (int)row0);
             if (v0 + 64 < a.V) tma_store_3d(&tmo, sm + L::OUT + PANEL, v0 + 64, hv, (int)row0);
             bulk_commit();
           }
         } else {
-          bar_sync<1, OUT_THREADS>();
-          copy_rows(out, reinterpret_cast<uint16_t*>(a.o), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, OUT_THREADS);
+          bar_sync<1, G::OUT_THREADS>();
+          copy_rows(out, reinterpret_cast<uint16_t*>(a.o), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, G::OUT_THREADS);
         }
       } else {
         const Column D(p + L::DO, vl);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) y[i] = j0 + i < valid ? y[i] * h2f<AB16>(lds16(D.at(j0 + i))) : 0.f;
+        for (int i = 0; i < OT; ++i) y[i] = j0 + i < valid ? y[i] * h2f<AB16>(lds16(D.at(j0 + i))) : 0.f;
         warp_arrive(&S_.empty[s]);
-        lane_sums<32>(y, lane);
-        S_.red[quad][j0 + lane] = y[0];
-        bar_sync<1, OUT_THREADS>();
+        lane_sums<OT>(y, lane);
+#pragma unroll
+        for (int i = 0; i < OT / 32; ++i) S_.red[quad][j0 + lane * (OT / 32) + i] = y[i];
+        bar_sync<1, G::OUT_THREADS>();
         if (threadIdx.x < C) {
           const int i = threadIdx.x;
           w.dotO[((int64_t)blockIdx.y * slots * a.HV + sh0 + (int64_t)c * a.HV) * C + i] =
               S_.red[0][i] + S_.red[1][i] + S_.red[2][i] + S_.red[3][i];
         }
-        bar_sync<1, OUT_THREADS>();
+        bar_sync<1, G::OUT_THREADS>();
       }
     }
     if (!BWD && threadIdx.x == 0) bulk_wait_all();
@@ -397,7 +422,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == W_MMA) tmem_dealloc(tb, 512);
+  if (warp == G::MMA) tmem_dealloc(tb, 512);
 }
 
 template <int AB16, int KD, bool BWD>
@@ -415,7 +440,7 @@ cudaError_t launch(const GdrArgs& a, const Ws& w) {
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(scan_kernel<AB16, KD, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e != cudaSuccess) return e;
-  scan_kernel<AB16, KD, BWD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), SCAN_THREADS, bytes, a.stream>>>(q, k, v, o, st, e16, a, w);
+  scan_kernel<AB16, KD, BWD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), Warps<BWD>::THREADS, bytes, a.stream>>>(q, k, v, o, st, e16, a, w);
   return cudaGetLastError();
 }
 
