@@ -22,9 +22,10 @@ EXPORTS = ('ccq_last_error', 'ccq_last_path', 'ccq_version', 'ccq_last_launch_co
            'ccq_workspace_size', 'ccq_workspace_size_for', 'ccq_device_status', 'ccq_clean_fwd', 'ccq_clean_bwd',
            'ccq_decode_step', 'ccq_clean_bwd_noalloc', 'ccq_noalloc_status', 'ccq_clean_l2norm_fwd',
            'ccq_clean_l2norm_bwd', 'ccq_decode_step_l2norm', 'ccq_gdr_workspace_size', 'ccq_gdr_fwd', 'ccq_gdr_bwd',
-           'ccq_gdr_step', 'ccq_layer_norm_workspace_size', 'ccq_layer_norm_fwd', 'ccq_layer_norm_bwd')
+           'ccq_gdr_bwd_from', 'ccq_gdr_step', 'ccq_layer_norm_workspace_size', 'ccq_layer_norm_fwd', 'ccq_layer_norm_bwd')
 CCQ_WS_HAVE_FWD_OUTPUTS, CCQ_WS_L2NORM = 1, 2
 CCQ_NORM_LAYER, CCQ_NORM_RMS = 0, 1
+CCQ_GDR_VARLEN, CCQ_GDR_HAVE_FWD, CCQ_GDR_UNALIGNED = 1, 2, 4
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -60,6 +61,7 @@ _SIGS = {
     'ccq_gdr_workspace_size': (_SZ, [_I] * 10),
     'ccq_gdr_fwd': (_I, _GDR + [_P, _P, _P, _SZ, _P]),
     'ccq_gdr_bwd': (_I, _GDR + [_P] * 8 + [_P, _SZ, _P]),
+    'ccq_gdr_bwd_from': (_I, _GDR + [_P] * 9 + [_P, _SZ, _P]),
     'ccq_gdr_step': (_I, _GDR + [_P, _P, _P]),
     'ccq_layer_norm_workspace_size': (_SZ, [_I, _L, _I]),
     'ccq_layer_norm_fwd': (_I, [_I, _I, _L, _I, _F] + [_P] * 9),

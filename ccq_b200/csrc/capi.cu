@@ -520,17 +520,16 @@ int need_workspace(const char* who, size_t need, const void* ws, size_t got) {
 
 extern "C" {
 
-size_t ccq_gdr_workspace_size(int op, int dtype, int B, int T, int H, int HV, int K, int V, int n_seqs, int varlen) {
+size_t ccq_gdr_workspace_size(int op, int dtype, int B, int T, int H, int HV, int K, int V, int n_seqs, int flags) {
   if (B < 1 || T < 0 || H < 1 || HV < 1 || K < 1 || K > 256 || V < 1 || n_seqs < 1) return 0;
   ccq::GdrArgs a;
   memset(&a, 0, sizeof(a));
   a.dtype = dtype; a.B = B; a.T = T; a.H = H; a.HV = HV; a.K = K; a.V = V; a.n_seqs = n_seqs;
-  static const int64_t some_offsets = 0;
-  a.cu_seqlens = varlen ? &some_offsets : nullptr;  // only whether it is given counts
-  // a 16-bit call takes the exact path when a tensor is not 16-byte aligned: room for either
-  const size_t simt = ccq::gdr_simt_workspace(a, op == CCQ_OP_BWD);
-  const size_t tc = ccq::gdr_tc_supported(a) ? ccq::gdr_tc_workspace(a, op == CCQ_OP_BWD) : 0;
-  return tc > simt ? tc : simt;
+  alignas(16) static const int64_t given[2] = {0, 0};  // only whether a pointer is given counts
+  a.cu_seqlens = (flags & CCQ_GDR_VARLEN) ? given : nullptr;
+  a.fwd_workspace = (flags & CCQ_GDR_HAVE_FWD) ? given : nullptr;
+  if ((flags & CCQ_GDR_UNALIGNED) || !ccq::gdr_tc_supported(a)) return ccq::gdr_simt_workspace(a, op == CCQ_OP_BWD);
+  return ccq::gdr_tc_workspace(a, op == CCQ_OP_BWD);
 }
 
 int ccq_gdr_fwd(int dtype, int B, int T, int H, int HV, int K, int V, const void* q, const void* k, const void* v,
@@ -562,6 +561,17 @@ int ccq_gdr_bwd(int dtype, int B, int T, int H, int HV, int K, int V, const void
                 int n_seqs, const float* initial_state, const void* d_o, const float* dfinal_state, void* dq, void* dk,
                 void* dv, void* dg, void* dbeta, float* dinitial_state, void* workspace, size_t workspace_bytes,
                 void* stream) {
+  return ccq_gdr_bwd_from(dtype, B, T, H, HV, K, V, q, k, v, g_dtype, g, beta_dtype, beta, scale, cu_seqlens, n_seqs,
+                          initial_state, d_o, dfinal_state, dq, dk, dv, dg, dbeta, dinitial_state, nullptr, workspace,
+                          workspace_bytes, stream);
+}
+
+int ccq_gdr_bwd_from(int dtype, int B, int T, int H, int HV, int K, int V, const void* q, const void* k, const void* v,
+                     int g_dtype, const void* g, int beta_dtype, const void* beta, float scale,
+                     const int64_t* cu_seqlens, int n_seqs, const float* initial_state, const void* d_o,
+                     const float* dfinal_state, void* dq, void* dk, void* dv, void* dg, void* dbeta,
+                     float* dinitial_state, const void* fwd_workspace, void* workspace, size_t workspace_bytes,
+                     void* stream) {
   g_err[0] = 0;
   ccq::GdrArgs a;
   int st = gdr_args(&a, dtype, B, T, H, HV, K, V, q, k, v, g_dtype, g, beta_dtype, beta, scale, cu_seqlens, n_seqs,
@@ -573,6 +583,7 @@ int ccq_gdr_bwd(int dtype, int B, int T, int H, int HV, int K, int V, const void
   a.dfinal_state = dfinal_state;
   a.dq = dq; a.dk = dk; a.dv = dv; a.dg = dg; a.dbeta = dbeta;
   a.dinitial_state = dinitial_state;
+  a.fwd_workspace = fwd_workspace;
   const bool tc = ccq::gdr_tc_supported(a);
   st = need_workspace("ccq_gdr_bwd", tc ? ccq::gdr_tc_workspace(a, true) : ccq::gdr_simt_workspace(a, true), workspace,
                       workspace_bytes);

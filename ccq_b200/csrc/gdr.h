@@ -56,6 +56,7 @@ struct GdrArgs {
   void* dg;             // g's type
   void* dbeta;          // beta's type
   float* dinitial_state;  // or nullptr
+  const void* fwd_workspace;  // of the forward on the same inputs, or nullptr (tensor-core path only)
   void* workspace;
   size_t workspace_bytes;
   cudaStream_t stream;

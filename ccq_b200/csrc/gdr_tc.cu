@@ -21,12 +21,18 @@ size_t carve(const GdrArgs& a, bool bwd, Ws* w) {
   Ws t;
   memset(&t, 0, sizeof(t));
   t.err = reinterpret_cast<int*>(take(256));
-  t.mats = take(sh * MATS);
-  t.aux = reinterpret_cast<float*>(take(sh * AX_N * 4));
+  if (a.fwd_workspace == nullptr) {
+    t.mats = take(sh * MATS);
+    t.aux = reinterpret_cast<float*>(take(sh * AX_N * 4));
+  } else {  // as the forward left them: the same carving of its workspace
+    uint8_t* f = reinterpret_cast<uint8_t*>(const_cast<void*>(a.fwd_workspace)) + ws_align(256);
+    t.mats = f;
+    t.aux = reinterpret_cast<float*>(f + ws_align(sh * MATS));
+  }
   if (bwd) {
     t.S0 = reinterpret_cast<uint16_t*>(take(sh * a.K * a.V * 2));
     t.dS1 = reinterpret_cast<uint16_t*>(take(sh * a.K * a.V * 2));
-    t.E = reinterpret_cast<uint16_t*>(take(sh * C * a.V * 2));
+    t.E = reinterpret_cast<uint16_t*>(take(sh * 2 * C * a.V * 2));
     t.dotO = reinterpret_cast<float*>(take(nvt * sh * C * 4));
     t.dotV = reinterpret_cast<float*>(take(nvt * sh * C * 4));
     const size_t ah = (size_t)gdr_slots(a, C * ANCHOR) * a.HV;
@@ -44,7 +50,8 @@ bool gdr_tc_supported(const GdrArgs& a) {
   if (a.T < 1 || a.K > 128 || a.K % 8 != 0 || a.V % 8 != 0) return false;
   if (gdr_slots(a, C) * a.HV >= (1ll << 31)) return false;  // the kernels count (chunk, head) pairs in 32 bits
   const uintptr_t p = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o | (uintptr_t)a.d_o |
-                      (uintptr_t)a.dq | (uintptr_t)a.dk | (uintptr_t)a.dv | (uintptr_t)a.workspace;
+                      (uintptr_t)a.dq | (uintptr_t)a.dk | (uintptr_t)a.dv | (uintptr_t)a.workspace |
+                      (uintptr_t)a.fwd_workspace;
   return (p & 15) == 0 && tc::encode_fn() != nullptr;
 }
 
@@ -67,7 +74,7 @@ cudaError_t gdr_tc_bwd(const GdrArgs& a, int* launches) {
   Ws w;
   carve(a, true, &w);
   cudaError_t e = cudaMemsetAsync(w.err, 0, 8, a.stream);
-  if (e == cudaSuccess) e = prep(a, w, launches);
+  if (e == cudaSuccess && a.fwd_workspace == nullptr) e = prep(a, w, launches);
   if (e == cudaSuccess) e = scan(a, w, true, launches);
   if (e == cudaSuccess) e = rscan(a, w, launches);
   if (e == cudaSuccess) e = grads(a, w, launches);

@@ -11,8 +11,10 @@
 // hi + lo, which keeps 2^-17 of it: the state and its gradient then stay at fp32 accuracy over any number
 // of chunks (measured 4e-6 against 64 bits), as they would not with one rounding each (2.4e-3).  The
 // products cost two or three MMAs instead of one; the scans are bound by the latency of one chunk's
-// chain of three products, not by the MMA rate.  The gradient kernel, whose outputs are rounded to 16
-// bits next and feed no recurrence, uses single 16-bit operands.
+// chain of three products, not by the MMA rate.  The gradient kernel, whose outputs are
+// rounded to 16 bits next and feed no recurrence, uses single 16-bit operands but for E, which enters
+// every one of its products but two: its rounding alone left 1.6e-3 in dq, dk and dbeta, as much as the
+// outputs' own.
 #pragma once
 
 #include "gdr.h"
@@ -42,7 +44,7 @@ struct Ws {
   // backward only
   uint16_t* S0;        // [slots * HV][V][K] state before the chunk, transposed, 16-bit
   uint16_t* dS1;       // [slots * HV][V][K] gradient of the state after it
-  uint16_t* E;         // [slots * HV][V][C] E transposed, 16-bit
+  uint16_t* E;         // [slots * HV][V][2 C] E transposed: hi part, then lo part
   float* dotO;         // [V tiles][slots * HV][C]: dO . O
   float* dotV;         // [V tiles][slots * HV][C]: V . dV
   float* Sf;           // [slots of 512 * HV][K][V] fp32 state after every ANCHOR chunks and after the last one

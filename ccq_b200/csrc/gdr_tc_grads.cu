@@ -16,8 +16,8 @@
 //
 // X, X2, P and B are read by the epilogue warps, which put the first term of F back into TMEM and [N ; W]
 // into shared memory; the transposed products read the same bytes MN-major, with a panel of zeros for
-// the other half.  44 MMAs an item; operands are single 16-bit values, since what is formed here is rounded to
-// 16 bits next.  An item moves 176 KB; the kernel is bound by that and by the serial epilogue between
+// the other half.  60 MMAs an item at V = 128.  Operands are single 16-bit values but for E (see
+// gdr_tc.cuh).  An item moves 192 KB; the kernel is bound by that and by the serial epilogue between
 // its two groups of products, of which the next item's loads and the last item's stores run beside.
 //
 // Warps (576 threads): 0-7 epilogue A (P and B), 8-15 epilogue B (X and X2), all of them the output; 16 TMA,
@@ -31,8 +31,8 @@ using namespace tc;
 
 constexpr int THREADS = 576, EPI = 512;
 constexpr uint32_t T_X = 0, T_X2 = 128, T_P = 256, T_B = 320, T_F = 384;
-// one step: [dV ; dO] (two panels), E, S0 and dS1 (two panels each)
-constexpr uint32_t B_DV = 0, B_DO = PANEL, B_E = 2 * PANEL, B_S = 3 * PANEL, B_DS = 5 * PANEL, B_SIZE = 7 * PANEL;
+// one step: [dV ; dO] (two panels), E hi and lo, S0 and dS1 (two panels each)
+constexpr uint32_t B_DV = 0, B_DO = PANEL, B_E = 2 * PANEL, B_S = 4 * PANEL, B_DS = 6 * PANEL, B_SIZE = 8 * PANEL;
 constexpr uint32_t L_KQ = 0;                       // two buffers: K over Q in panels of 128 rows
 constexpr uint32_t L_B = 8 * PANEL;                // two steps
 constexpr uint32_t L_W = L_B + 2 * B_SIZE;         // N over W, then zeros
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (*ab) { ok = false; break; }
             uint64_t* bar = &S_.full[b];
             uint8_t* p = sm + L_B + b * B_SIZE;
-            mbar_arrive_expect_tx(bar, 2 * NP * PANEL + 3 * PANEL + (g == 0 && vt == 0 ? 2 * NP * PANEL : 0));
+            mbar_arrive_expect_tx(bar, 2 * NP * PANEL + 4 * PANEL + (g == 0 && vt == 0 ? 2 * NP * PANEL : 0));
             if (vt == 0) {
               Rec& R = S_.rec[r];
               R.live = 1;
@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             tma_load_3d(p + B_DV, &tmdv, bar, 64 * vt, hv, row);
             tma_load_3d(p + B_DO, &tmo, bar, 64 * vt, hv, row);
             tma_load_3d(p + B_E, &tme, bar, 0, 64 * vt, (int)sh);
+            tma_load_3d(p + B_E + PANEL, &tme, bar, C, 64 * vt, (int)sh);
             for (int i = 0; i < NP; ++i) {
               tma_load_3d(p + B_S + i * PANEL, &tms, bar, 64 * i, 64 * vt, (int)sh);
               tma_load_3d(p + B_DS + i * PANEL, &tmds, bar, 64 * i, 64 * vt, (int)sh);
@@ -193,8 +194,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           tc_fence_after();
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            umma(tb + T_P, sdesc(p + B_DV + ks * 32, 16, 1024), sdesc(p + B_E + ks * 2048, PANEL, 1024), id_p, vt + ks > 0);
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              umma(tb + T_P, sdesc(p + B_DV + ks * 32, 16, 1024), sdesc(p + B_E + x * PANEL + ks * 2048, PANEL, 1024), id_p,
+                   vt + x + ks > 0);
           if (vt == 0) {
 #pragma unroll
             for (int ks = 0; ks < KD / 16; ++ks) {
@@ -206,9 +210,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int ks = 0; ks < 4; ++ks)
             umma(tb + T_X, sdesc(p + B_DV + ks * 32, 16, 1024), sdesc(p + B_S + ks * 2048, PANEL, 1024), id_x, vt + ks > 0);
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            umma(tb + T_X2, sdesc(p + B_E + ks * 2048, PANEL, 1024), sdesc(p + B_DS + ks * 2048, PANEL, 1024), id_x2,
-                 vt + ks > 0);
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              umma(tb + T_X2, sdesc(p + B_E + x * PANEL + ks * 2048, PANEL, 1024), sdesc(p + B_DS + ks * 2048, PANEL, 1024),
+                   id_x2, vt + x + ks > 0);
           umma_commit(&S_.empty[b]);
         }
         if (!ok) break;
@@ -443,7 +449,7 @@ cudaError_t launch(const GdrArgs& a, const Ws& w) {
   if (r == cudaSuccess) r = token_map(&k, a, a.k, a.H, a.K);
   if (r == cudaSuccess) r = token_map(&o, a, a.d_o, a.HV, a.V);
   if (r == cudaSuccess) r = token_map(&dv, a, a.dv, a.HV, a.V);
-  if (r == cudaSuccess) r = matrix_map(&e, a, w.E, C, sh);
+  if (r == cudaSuccess) r = matrix_map(&e, a, w.E, 2 * C, sh);
   if (r == cudaSuccess) r = matrix_map(&s, a, w.S0, a.K, sh);
   if (r == cudaSuccess) r = matrix_map(&ds, a, w.dS1, a.K, sh);
   if (r == cudaSuccess) r = token_map(&dq, a, a.dq, a.H, a.K);

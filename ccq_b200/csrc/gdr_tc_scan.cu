@@ -16,7 +16,7 @@
 // The rest of a chunk's period is instructions of the chain warps between the products, so V enters by an MMA
 // of its own (beside the chain) and the factors by packed two-value arithmetic.
 //
-// BWD: instead of O it writes what the backward reads: S0 (16-bit, transposed), E (16-bit), dO . O and,
+// BWD: instead of O it writes what the backward reads: S0 (16-bit, transposed), E (hi + lo), dO . O and,
 // every ANCHOR chunks, S in fp32.
 //
 // TMEM columns: S hi, S lo (64 each), X | Y, then dS (128), E, then E P^T
@@ -270,9 +270,11 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
         split<AB16, 8>(x, hi, lo);
         tmem_st8(tl + T_RH + (i0 + i) / 2, hi);
         tmem_st8(tl + T_RL + (i0 + i) / 2, lo);
-        if (BWD) {  // E, transposed, to the staging panel
+        if (BWD) {  // E, transposed, to the staging panel (hi) and over the V tile, whose product is done (lo)
           sts128(sb + L::OUT + sw128(vl, (i0 + i) >> 3), make_uint4(hi[0], hi[1], hi[2], hi[3]));
           sts128(sb + L::OUT + sw128(vl, ((i0 + i) >> 3) + 1), make_uint4(hi[4], hi[5], hi[6], hi[7]));
+          sts128(p + L::V + sw128(vl, (i0 + i) >> 3), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+          sts128(p + L::V + sw128(vl, ((i0 + i) >> 3) + 1), make_uint4(lo[4], lo[5], lo[6], lo[7]));
         }
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
@@ -290,7 +292,10 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
       if (BWD) {
         fence_async_smem();
         bar_sync<2, G::CHAIN_THREADS>();
-        if (threadIdx.x == 32 * G::CHAIN) store_panel(&tme, sm + L::OUT, 0, v0, a.V, sh0 + (int64_t)c * a.HV);
+        if (threadIdx.x == 32 * G::CHAIN) {
+          store_panel(&tme, sm + L::OUT, 0, v0, a.V, sh0 + (int64_t)c * a.HV);
+          store_panel(&tme, sm + s * L::STAGE + L::V, C, v0, a.V, sh0 + (int64_t)c * a.HV);
+        }
       }
       pipe_wait(&S_.d_full, ph, ab, err, 0x2000);
       tc_fence_after();
@@ -435,7 +440,7 @@ cudaError_t launch(const GdrArgs& a, const Ws& w) {
   st = e16 = o;  // unused by the forward
   const int64_t sh = gdr_slots(a, C) * a.HV;
   if (BWD && e == cudaSuccess) e = matrix_map(&st, a, w.S0, a.K, sh);
-  if (BWD && e == cudaSuccess) e = matrix_map(&e16, a, w.E, C, sh);
+  if (BWD && e == cudaSuccess) e = matrix_map(&e16, a, w.E, 2 * C, sh);
   constexpr uint32_t bytes = Lay<BWD>::BYTES;
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(scan_kernel<AB16, KD, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);

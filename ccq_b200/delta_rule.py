@@ -34,14 +34,20 @@ def _inputs(q, k, v, g, beta):
     if HV % H != 0:
         raise ValueError(f'the number of value heads ({HV}) must be a multiple of the number of key heads ({H})')
     q, k, v, g, beta = (t.detach() for t in (q, k, v, g, beta))
-    return (q.contiguous(), k.to(q.dtype).contiguous(), v.to(q.dtype).contiguous(), g.contiguous(),
-            beta.contiguous())
+    return _aligned(q), _aligned(k.to(q.dtype)), _aligned(v.to(q.dtype)), g.contiguous(), beta.contiguous()
 
 
-def _workspace(op, q, v, N, cu):
+def _aligned(t):
+    """t contiguous and on a 16-byte boundary, as the tensor-core path reads it (a copy of a view that is not)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _workspace(op, q, v, N, cu, have_fwd=False):
     B, T, H, K = q.shape
     HV, V = v.shape[2:]
-    nbytes = _lib.load().ccq_gdr_workspace_size(op, _dtype_code(q), B, T, H, HV, K, V, N, int(cu is not None))
+    flags = (_lib.CCQ_GDR_VARLEN if cu is not None else 0) | (_lib.CCQ_GDR_HAVE_FWD if have_fwd else 0)
+    nbytes = _lib.load().ccq_gdr_workspace_size(op, _dtype_code(q), B, T, H, HV, K, V, N, flags)
     return (torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None), nbytes
 
 
@@ -62,11 +68,12 @@ def _fwd_raw(q, k, v, g, beta, scale, h0, want_state, cu, N):
         st = _lib.load().ccq_gdr_fwd(*_head(q, k, v, g, beta, scale, cu, N, h0), _p(o), _p(state), _p(ws), nbytes,
                                      _stream(q.device))
     _lib.check(st)
-    return o, state
+    return o, state, ws
 
 
 class GatedDeltaRule(torch.autograd.Function):
-    """``gated_delta_rule`` as an autograd function; the backward recomputes the chunk states."""
+    """``gated_delta_rule`` as an autograd function.  A call that needs gradients keeps the forward's workspace
+    (540 bytes per token and value head on the tensor-core path); the backward recomputes the chunk states."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, scale, initial_state, output_final_state, cu_seqlens):
@@ -75,8 +82,8 @@ class GatedDeltaRule(torch.autograd.Function):
         q, k, v, g, beta = _inputs(q, k, v, g, beta)
         cu, N = _seqs(q.shape[0], cu_seqlens, q.shape[1])
         h0 = _state(initial_state, (N, v.shape[2], q.shape[3], v.shape[3]))
-        o, state = _fwd_raw(q, k, v, g, beta, scale, h0, output_final_state, cu, N)
-        ctx.save_for_backward(q, k, v, g, beta, h0, cu)
+        o, state, ws = _fwd_raw(q, k, v, g, beta, scale, h0, output_final_state, cu, N)
+        ctx.save_for_backward(q, k, v, g, beta, h0, cu, ws if any(ctx.needs_input_grad) else None)
         ctx.scale, ctx.N, ctx.types = scale, N, types
         ctx.state_dtype = initial_state.dtype if initial_state is not None else None
         ctx.set_materialize_grads(False)
@@ -84,16 +91,16 @@ class GatedDeltaRule(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, do, dstate):
-        q, k, v, g, beta, h0, cu = ctx.saved_tensors
-        do = torch.zeros_like(v) if do is None else do.to(v.dtype).contiguous()
+        q, k, v, g, beta, h0, cu, fwd_ws = ctx.saved_tensors
+        do = torch.zeros_like(v) if do is None else _aligned(do.to(v.dtype))
         dstate = dstate.float().contiguous() if dstate is not None else None
         dq, dk, dv, dg, dbeta = (torch.empty_like(t) for t in (q, k, v, g, beta))
         dh0 = torch.empty_like(h0) if h0 is not None else None
-        ws, nbytes = _workspace(_lib.CCQ_OP_BWD, q, v, ctx.N, cu)
+        ws, nbytes = _workspace(_lib.CCQ_OP_BWD, q, v, ctx.N, cu, fwd_ws is not None)
         with torch.cuda.device(q.device):
-            st = _lib.load().ccq_gdr_bwd(*_head(q, k, v, g, beta, ctx.scale, cu, ctx.N, h0), _p(do), _p(dstate), _p(dq),
-                                         _p(dk), _p(dv), _p(dg), _p(dbeta), _p(dh0), _p(ws), nbytes,
-                                         _stream(q.device))
+            st = _lib.load().ccq_gdr_bwd_from(*_head(q, k, v, g, beta, ctx.scale, cu, ctx.N, h0), _p(do), _p(dstate),
+                                              _p(dq), _p(dk), _p(dv), _p(dg), _p(dbeta), _p(dh0), _p(fwd_ws), _p(ws),
+                                              nbytes, _stream(q.device))
         _lib.check(st)
         if dh0 is not None:
             dh0 = dh0.to(ctx.state_dtype)

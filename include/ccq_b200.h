@@ -283,8 +283,14 @@ int ccq_decode_step_l2norm(int dtype, int B, int T, int H, int K,
  *   final_state may be NULL.  Documents of length zero return their initial state.
  * All sums, the state and the running sums of g are fp32 or wider.
  */
+typedef enum {
+  CCQ_GDR_VARLEN = 1,    /* cu_seqlens is given */
+  CCQ_GDR_HAVE_FWD = 2,  /* backward: the forward's workspace is given (ccq_gdr_bwd_from) */
+  CCQ_GDR_UNALIGNED = 4  /* a 16-bit tensor is not 16-byte aligned: the call takes the exact path */
+} ccq_gdr_flags;
+
 size_t ccq_gdr_workspace_size(int op /* CCQ_OP_FWD or CCQ_OP_BWD */, int dtype, int B, int T, int H, int HV,
-                              int K, int V, int n_seqs, int varlen);
+                              int K, int V, int n_seqs, int flags);
 
 int ccq_gdr_fwd(int dtype, int B, int T, int H, int HV, int K, int V,
                 const void* q, const void* k, const void* v,
@@ -305,6 +311,19 @@ int ccq_gdr_bwd(int dtype, int B, int T, int H, int HV, int K, int V,
                 const void* d_o, const float* dfinal_state,
                 void* dq, void* dk, void* dv, void* dg, void* dbeta, float* dinitial_state,
                 void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The same with the workspace of the ccq_gdr_fwd call on the same inputs, unmodified since (it holds the
+ * chunks' inverses and scores: on the tensor-core path the backward then starts from them instead of forming
+ * them again; the exact path does not read it).  NULL: as ccq_gdr_bwd.
+ */
+int ccq_gdr_bwd_from(int dtype, int B, int T, int H, int HV, int K, int V,
+                     const void* q, const void* k, const void* v,
+                     int g_dtype, const void* g, int beta_dtype, const void* beta, float scale,
+                     const int64_t* cu_seqlens, int n_seqs, const float* initial_state,
+                     const void* d_o, const float* dfinal_state,
+                     void* dq, void* dk, void* dv, void* dg, void* dbeta, float* dinitial_state,
+                     const void* fwd_workspace, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * The same recurrence token by token over a cache (generation: one token or a few per document).
