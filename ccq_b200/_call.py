@@ -1,0 +1,46 @@
+"""Calls of the C entry points with little host work: a generated token or a short prompt is bound by the
+host, so pointers go as plain integers, the device is switched only when it is another one, and the
+stream handle is read without a stream object."""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+_current_device = torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def invoke(fn, index, *args):
+    """fn(*args, current stream of device ``index``) with that device current; raises on a status."""
+    if _current_device() == index:
+        st = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            st = fn(*args, _raw_stream(index))
+    if st:
+        _lib.check(st)
+
+
+def cuda_index(*tensors):
+    """The device index of the given tensors (None among them is skipped); raises unless all are on one."""
+    index = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError('ccq_b200 operators run on CUDA tensors only (got a CPU tensor)')
+        i = t.device.index
+        if index is None:
+            index = i
+        elif i != index:
+            raise RuntimeError(f'tensors on different devices: cuda:{index} and cuda:{i}')
+    return index
+
+
+def wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

@@ -14,27 +14,31 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .ops import _check_cuda, _dtype_code, _p, _seqs, _state, _stream
+from ._call import cuda_index, invoke, ptr, wants_grad
+from .ops import _dtype_code, _seqs, _state
 
 
 def _inputs(q, k, v, g, beta):
-    """The five inputs detached, contiguous and checked; k and v in q's dtype, g and beta in their own
+    """The five inputs checked, contiguous and aligned; k and v in q's dtype, g and beta in their own
     (another type than float32, bfloat16 or float16 is an error)."""
     if q.ndim != 4 or v.ndim != 4:
         raise ValueError(f'q, k must be [B, T, H, K] and v [B, T, HV, V], got {tuple(q.shape)} and {tuple(v.shape)}')
     B, T, H, K = q.shape
-    HV, V = v.shape[2:]
-    if tuple(k.shape) != (B, T, H, K):
+    HV = v.shape[2]
+    if k.shape != q.shape:
         raise ValueError(f'k has shape {tuple(k.shape)}, expected {(B, T, H, K)}')
-    if tuple(v.shape[:2]) != (B, T):
+    if v.shape[0] != B or v.shape[1] != T:
         raise ValueError(f'v has shape {tuple(v.shape)}, expected {(B, T)} + (HV, V)')
-    for name, t in (('g', g), ('beta', beta)):
-        if tuple(t.shape) != (B, T, HV):
-            raise ValueError(f'{name} has shape {tuple(t.shape)}, expected {(B, T, HV)}')
+    gates = (B, T, HV)
+    if g.shape != gates:
+        raise ValueError(f'g has shape {tuple(g.shape)}, expected {gates}')
+    if beta.shape != gates:
+        raise ValueError(f'beta has shape {tuple(beta.shape)}, expected {gates}')
     if HV % H != 0:
         raise ValueError(f'the number of value heads ({HV}) must be a multiple of the number of key heads ({H})')
-    q, k, v, g, beta = (t.detach() for t in (q, k, v, g, beta))
-    return _aligned(q), _aligned(k.to(q.dtype)), _aligned(v.to(q.dtype)), g.contiguous(), beta.contiguous()
+    dt = q.dtype
+    return (_aligned(q), _aligned(k if k.dtype == dt else k.to(dt)), _aligned(v if v.dtype == dt else v.to(dt)),
+            g.contiguous(), beta.contiguous())
 
 
 def _aligned(t):
@@ -55,20 +59,23 @@ def _head(q, k, v, g, beta, scale, cu, N, h0):
     """The arguments the C entry points share."""
     B, T, H, K = q.shape
     HV, V = v.shape[2:]
-    return (_dtype_code(q), B, T, H, HV, K, V, _p(q), _p(k), _p(v), _dtype_code(g), _p(g), _dtype_code(beta), _p(beta),
-            float(scale), _p(cu), N, _p(h0))
+    return (_dtype_code(q), B, T, H, HV, K, V, q.data_ptr(), k.data_ptr(), v.data_ptr(), _dtype_code(g), g.data_ptr(),
+            _dtype_code(beta), beta.data_ptr(), scale, ptr(cu), N, ptr(h0))
 
 
-def _fwd_raw(q, k, v, g, beta, scale, h0, want_state, cu, N):
+def _forward(q, k, v, g, beta, scale, initial_state, output_final_state, cu_seqlens):
+    """One ccq_gdr_fwd call; returns (o, final state or None, what a backward needs)."""
+    index = cuda_index(q, k, v, g, beta, initial_state, cu_seqlens)
+    q, k, v, g, beta = _inputs(q, k, v, g, beta)
+    cu, N = _seqs(q.shape[0], cu_seqlens, q.shape[1])
+    shape = (N, v.shape[2], q.shape[3], v.shape[3])
+    h0 = _state(initial_state, shape)
     o = torch.empty_like(v)
-    state = torch.empty(N, *v.shape[2:3], q.shape[3], v.shape[3], device=q.device,
-                        dtype=torch.float32) if want_state else None
+    state = torch.empty(shape, device=q.device, dtype=torch.float32) if output_final_state else None
     ws, nbytes = _workspace(_lib.CCQ_OP_FWD, q, v, N, cu)
-    with torch.cuda.device(q.device):
-        st = _lib.load().ccq_gdr_fwd(*_head(q, k, v, g, beta, scale, cu, N, h0), _p(o), _p(state), _p(ws), nbytes,
-                                     _stream(q.device))
-    _lib.check(st)
-    return o, state, ws
+    invoke(_lib.load().ccq_gdr_fwd, index, *_head(q, k, v, g, beta, scale, cu, N, h0), o.data_ptr(), ptr(state), ptr(ws),
+           nbytes)
+    return o, state, (q, k, v, g, beta, h0, cu, ws)
 
 
 class GatedDeltaRule(torch.autograd.Function):
@@ -77,31 +84,26 @@ class GatedDeltaRule(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, scale, initial_state, output_final_state, cu_seqlens):
-        _check_cuda(q, k, v, g, beta, initial_state, cu_seqlens)
-        types = (k.dtype, v.dtype)
-        q, k, v, g, beta = _inputs(q, k, v, g, beta)
-        cu, N = _seqs(q.shape[0], cu_seqlens, q.shape[1])
-        h0 = _state(initial_state, (N, v.shape[2], q.shape[3], v.shape[3]))
-        o, state, ws = _fwd_raw(q, k, v, g, beta, scale, h0, output_final_state, cu, N)
-        ctx.save_for_backward(q, k, v, g, beta, h0, cu, ws if any(ctx.needs_input_grad) else None)
-        ctx.scale, ctx.N, ctx.types = scale, N, types
+        ctx.types = (k.dtype, v.dtype)
         ctx.state_dtype = initial_state.dtype if initial_state is not None else None
+        o, state, kept = _forward(q, k, v, g, beta, scale, initial_state, output_final_state, cu_seqlens)
+        ctx.save_for_backward(*kept)
+        ctx.scale = scale
         ctx.set_materialize_grads(False)
         return o, state
 
     @staticmethod
     def backward(ctx, do, dstate):
         q, k, v, g, beta, h0, cu, fwd_ws = ctx.saved_tensors
-        do = torch.zeros_like(v) if do is None else _aligned(do.to(v.dtype))
+        do = torch.zeros_like(v) if do is None else _aligned(do if do.dtype == v.dtype else do.to(v.dtype))
         dstate = dstate.float().contiguous() if dstate is not None else None
         dq, dk, dv, dg, dbeta = (torch.empty_like(t) for t in (q, k, v, g, beta))
         dh0 = torch.empty_like(h0) if h0 is not None else None
-        ws, nbytes = _workspace(_lib.CCQ_OP_BWD, q, v, ctx.N, cu, fwd_ws is not None)
-        with torch.cuda.device(q.device):
-            st = _lib.load().ccq_gdr_bwd_from(*_head(q, k, v, g, beta, ctx.scale, cu, ctx.N, h0), _p(do), _p(dstate),
-                                              _p(dq), _p(dk), _p(dv), _p(dg), _p(dbeta), _p(dh0), _p(fwd_ws), _p(ws),
-                                              nbytes, _stream(q.device))
-        _lib.check(st)
+        N = cu.numel() - 1 if cu is not None else q.shape[0]
+        ws, nbytes = _workspace(_lib.CCQ_OP_BWD, q, v, N, cu, fwd_ws is not None)
+        invoke(_lib.load().ccq_gdr_bwd_from, q.device.index, *_head(q, k, v, g, beta, ctx.scale, cu, N, h0), do.data_ptr(),
+               ptr(dstate), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(), ptr(dh0),
+               ptr(fwd_ws), ptr(ws), nbytes)
         if dh0 is not None:
             dh0 = dh0.to(ctx.state_dtype)
         return dq, dk.to(ctx.types[0]), dv.to(ctx.types[1]), dg, dbeta, None, dh0, None, None
@@ -117,9 +119,15 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, output
 
     g and beta may be float32, bfloat16 or float16; their gradients come in the same types.  Inputs must be
     finite, except that g = -inf empties the state before its token.
+
+    16-bit inputs with K a multiple of 8 up to 128 and V a multiple of 8 run on the tensor cores, where the
+    state and its gradient keep fp32 accuracy (about 4e-6) and dq, dk and dbeta that of the 16-bit type;
+    everything else, fp32 inputs among it, runs in fp32 on the CUDA cores.
     """
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    return GatedDeltaRule.apply(q, k, v, g, beta, scale, initial_state, bool(output_final_state), cu_seqlens)
+    if wants_grad(q, k, v, g, beta, initial_state):
+        return GatedDeltaRule.apply(q, k, v, g, beta, scale, initial_state, bool(output_final_state), cu_seqlens)
+    return _forward(q, k, v, g, beta, scale, initial_state, output_final_state, cu_seqlens)[:2]
 
 
 def gated_delta_step(q, k, v, g, beta, state=None, *, scale=None, cu_seqlens=None, inplace=False):
@@ -129,17 +137,15 @@ def gated_delta_step(q, k, v, g, beta, state=None, *, scale=None, cu_seqlens=Non
     Returns (o, state after [N, HV, K, V] fp32).  ``inplace=True`` updates the given state, which must
     then be a contiguous float32 tensor.
     """
-    _check_cuda(q, k, v, g, beta, state, cu_seqlens)
+    index = cuda_index(q, k, v, g, beta, state, cu_seqlens)
     q, k, v, g, beta = _inputs(q, k, v, g, beta)
     cu, N = _seqs(q.shape[0], cu_seqlens, q.shape[1])
     shape = (N, v.shape[2], q.shape[3], v.shape[3])
     if inplace and (state is None or state.dtype != torch.float32 or not state.is_contiguous()):
         raise ValueError('inplace needs a contiguous float32 state')
     h0 = _state(state, shape)
-    out = h0 if inplace else torch.empty(shape, device=q.device, dtype=torch.float32)
-    o = torch.empty_like(v)
+    out = state if inplace else torch.empty(shape, device=q.device, dtype=torch.float32)
+    o = torch.empty_like(v, requires_grad=False)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    with torch.cuda.device(q.device):
-        st = _lib.load().ccq_gdr_step(*_head(q, k, v, g, beta, scale, cu, N, h0), _p(out), _p(o), _stream(q.device))
-    _lib.check(st)
-    return o, (state if inplace else out)
+    invoke(_lib.load().ccq_gdr_step, index, *_head(q, k, v, g, beta, scale, cu, N, h0), out.data_ptr(), o.data_ptr())
+    return o, out
