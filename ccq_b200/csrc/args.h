@@ -86,6 +86,7 @@ cudaError_t l2norm_rows_bwd(int dtype, void* d, const void* d_ext, const void* y
 // Layer norm (layer_norm.cu): rows of D elements, D <= LN_MAX_D
 enum { LN_LAYER = 0, LN_RMS = 1 };
 constexpr int LN_MAX_D = 16384;
+constexpr int LN_BWD_BLOCKS = 148 * 16;  // most blocks (and partial sums) of the backward
 struct LayerNormArgs {
   int dtype, form, D;
   int64_t rows;

@@ -633,6 +633,9 @@ int ln_args(ccq::LayerNormArgs* out, int dtype, int form, int64_t rows, int D, f
   if (D > ccq::LN_MAX_D) return fail(CCQ_ERR_UNSUPPORTED, "row size D=%d > %d is not supported", D, ccq::LN_MAX_D);
   if (rows > 0x7FFFFFFF) return fail(CCQ_ERR_UNSUPPORTED, "rows=%lld is too large", (long long)rows);
   if (!(eps >= 0.f)) return fail(CCQ_ERR_INVALID, "eps must not be negative");
+  if (form == CCQ_NORM_RMS && bias != nullptr) return fail(CCQ_ERR_UNSUPPORTED, "the RMS form takes no bias");
+  if (gate != nullptr && (form != CCQ_NORM_RMS || residual != nullptr))
+    return fail(CCQ_ERR_UNSUPPORTED, "a gate goes with the RMS form without residual");
   if (rows > 0 && x == nullptr) return fail(CCQ_ERR_INVALID, "x is required");
   ccq::LayerNormArgs a;
   memset(&a, 0, sizeof(a));

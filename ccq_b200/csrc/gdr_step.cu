@@ -1,14 +1,18 @@
 // Gated delta rule token by token over a cache: the state update and read of gdr.h, fp32 throughout.
 //
-// A block owns VT columns of one (document, value head) state and keeps them in registers for all its
+// A block owns 4 LV columns of one (document, value head) state and keeps them in registers for all its
 // tokens: LV lanes of a warp take four neighbouring columns each (one 16-byte access a row), the other
-// 32 / LV lane groups and the warps split the K rows.  Both products of a token, S^T k and S^T q, are
-// formed in the same pass over the decayed state, since the read after the update is
+// 32 / LV lane groups and the warps split the K rows, neighbouring rows to a thread, whose k and q it then
+// loads eight at a time.  Both products of a token, S^T k and S^T q, are formed in the same pass over the
+// decayed state, since the read after the update is
 //   S_new^T q = S^T q + (k . q) u,
 // so a token costs one reduction over the block.  A state row is read once and written once: with one
-// token the kernel is bound by HBM (8 K V bytes a head).  With few heads it is bound by latency, so the
-// launcher narrows VT (128, 32 or 16 columns) until the grid covers the SMs.  Each element is read
-// and written by one thread, so the state may be updated in place.
+// token the kernel is bound by HBM (8 K V bytes a head).  Small blocks with many rows a thread keep most
+// of an SM's registers in flight as loads while others compute and store (256 requests, 16 heads,
+// K = V = 128, 537 MB of state: 2 warps of 32 rows 102 us, 4 of 16 109 us, 8 of 8 111 us; 128 columns a
+// block instead of 64: 106 us).  With few heads the kernel is bound by latency, so the launcher narrows
+// the block to 32 or 16 columns until the grid covers the SMs.  Each element is read and written by one
+// thread, so the state may be updated in place.
 #include "gdr.h"
 
 namespace ccq {
@@ -51,22 +55,42 @@ __device__ __forceinline__ void store_state(float* row, int v0, int V, const flo
   if (v0 + 3 < V) row[v0 + 3] = x.w;
 }
 
-// WARPS * (32 / LV) row groups of up to ROWS rows
+// ROWS values from r0 of a row of K; VEC: K is a multiple of 8 and the row starts on a 16-byte boundary
+template <typename TI, int ROWS, bool VEC>
+__device__ __forceinline__ void load_values(const TI* p, int r0, int K, float* x) {
+  if (VEC && ROWS % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < ROWS; i += 8) {
+      uint4 u[sizeof(TI) / 2] = {};
+      if (r0 + i < K) {
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(TI) / 2; ++j) u[j] = reinterpret_cast<const uint4*>(p + r0 + i)[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[i + j] = Act<TI>::load(reinterpret_cast<const TI*>(u) + j);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) x[i] = r0 + i < K ? Act<TI>::load(p + r0 + i) : 0.f;
+}
+
+// WARPS * (32 / LV) groups of ROWS neighbouring rows
 template <typename TI, int LV, int WARPS, int ROWS, bool VEC4>
 __global__ void __launch_bounds__(WARPS * 32) step_kernel(GdrArgs a) {
-  constexpr int GROUPS = 32 / LV, STRIDE = WARPS * GROUPS, VT = 4 * LV;
+  constexpr int GROUPS = 32 / LV, VT = 4 * LV;
   __shared__ float4 part[2][2][WARPS][LV];  // token parity; S^T k, S^T q; warp; columns
   __shared__ float kq[2][WARPS];
   const int n = blockIdx.x / a.HV, hv = blockIdx.x % a.HV, h = hv / (a.HV / a.H);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int lv = lane % LV, row0 = warp * GROUPS + lane / LV;
+  const int lv = lane % LV, row0 = (warp * GROUPS + lane / LV) * ROWS;
   const int v0 = blockIdx.y * VT + 4 * lv;
   const Seq sq = seq_of(n, a.T, a.cu_seqlens);
   const int64_t st = ((int64_t)n * a.HV + hv) * a.K * a.V;
   float4 S[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const int r = row0 + i * STRIDE;
+    const int r = row0 + i;
     S[i] = (a.initial_state && r < a.K) ? load_state<VEC4>(a.initial_state + st + (int64_t)r * a.V, v0, a.V)
                                         : make_float4(0.f, 0.f, 0.f, 0.f);
   }
@@ -80,19 +104,18 @@ __global__ void __launch_bounds__(WARPS * 32) step_kernel(GdrArgs a) {
     float vv[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) vv[c] = v0 + c < a.V ? Act<TI>::load(vp + v0 + c) : 0.f;
-    float k[ROWS];
+    float k[ROWS], q[ROWS];
+    load_values<TI, ROWS, VEC4>(kp, row0, a.K, k);
+    load_values<TI, ROWS, VEC4>(qp, row0, a.K, q);
     float4 sk = make_float4(0.f, 0.f, 0.f, 0.f), sqv = sk;
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      const int r = row0 + i * STRIDE;
-      k[i] = r < a.K ? Act<TI>::load(kp + r) : 0.f;
-      const float q = r < a.K ? Act<TI>::load(qp + r) : 0.f;
       // a zero decay empties the state whatever it holds
       S[i] = decay == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : scale4(S[i], decay);
       fma4(sk, S[i], k[i]);
-      fma4(sqv, S[i], q);
-      dot = fmaf(k[i], q, dot);
+      fma4(sqv, S[i], q[i]);
+      dot = fmaf(k[i], q[i], dot);
     }
 #pragma unroll
     for (int o = LV; o < 32; o <<= 1) {
@@ -130,7 +153,7 @@ __global__ void __launch_bounds__(WARPS * 32) step_kernel(GdrArgs a) {
   }
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const int r = row0 + i * STRIDE;
+    const int r = row0 + i;
     if (r < a.K) store_state<VEC4>(a.final_state + st + (int64_t)r * a.V, v0, a.V, S[i]);
   }
 }
@@ -138,28 +161,28 @@ __global__ void __launch_bounds__(WARPS * 32) step_kernel(GdrArgs a) {
 template <typename TI, int LV, int WARPS, int ROWS>
 void launch(const GdrArgs& a) {
   const dim3 grid(a.n_seqs * a.HV, (a.V + 4 * LV - 1) / (4 * LV));
-  const bool vec = a.V % 4 == 0 && (((uintptr_t)a.initial_state | (uintptr_t)a.final_state) & 15) == 0;
+  const bool vec = a.V % 4 == 0 && a.K % 8 == 0 &&
+                   (((uintptr_t)a.initial_state | (uintptr_t)a.final_state | (uintptr_t)a.q | (uintptr_t)a.k) & 15) == 0;
   if (vec) step_kernel<TI, LV, WARPS, ROWS, true><<<grid, WARPS * 32, 0, a.stream>>>(a);
   else step_kernel<TI, LV, WARPS, ROWS, false><<<grid, WARPS * 32, 0, a.stream>>>(a);
 }
 
-template <typename TI, int LV>
+// W64, W128, W256: warps of a block for K up to 64, 128 and 256
+template <typename TI, int LV, int W64, int W128, int W256>
 void pick_rows(const GdrArgs& a) {
   constexpr int G = 32 / LV;
-  if (a.K <= 64) launch<TI, LV, 8, (64 + 8 * G - 1) / (8 * G)>(a);
-  else if (a.K <= 128) launch<TI, LV, 8, (128 + 8 * G - 1) / (8 * G)>(a);
-  // 16 rows of four columns a thread no longer fit 128 registers: half the columns
-  else launch<TI, (LV > 16 ? 16 : LV), 16, (256 + 16 * (LV > 16 ? 2 : G) - 1) / (16 * (LV > 16 ? 2 : G))>(a);
+  if (a.K <= 64) launch<TI, LV, W64, 64 / (W64 * G)>(a);
+  else if (a.K <= 128) launch<TI, LV, W128, 128 / (W128 * G)>(a);
+  else launch<TI, LV, W256, 256 / (W256 * G)>(a);
 }
 
 template <typename TI>
 void pick_columns(const GdrArgs& a) {
-  // 128 columns a block give full 512-byte rows; narrower blocks only while the grid would leave
-  // SMs idle (148 on B200)
+  // narrower blocks, with more warps to a column, only while the grid would leave SMs idle (148)
   const int64_t heads = (int64_t)a.n_seqs * a.HV;
-  if (a.V > 32 && heads * ((a.V + 127) / 128) >= 148) pick_rows<TI, 32>(a);
-  else if (a.V > 16 && heads * ((a.V + 31) / 32) >= 148) pick_rows<TI, 8>(a);
-  else pick_rows<TI, 4>(a);
+  if (a.V > 32 && heads * ((a.V + 63) / 64) >= 2 * 148) pick_rows<TI, 16, 2, 2, 4>(a);
+  else if (a.V > 16 && heads * ((a.V + 31) / 32) >= 148) pick_rows<TI, 8, 2, 4, 8>(a);
+  else pick_rows<TI, 4, 2, 4, 8>(a);
 }
 
 }  // namespace

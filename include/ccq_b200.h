@@ -338,7 +338,8 @@ int ccq_gdr_step(int dtype, int B, int T, int H, int HV, int K, int V,
 /*
  * Layer norm over the last axis of [rows, D] (1 <= D <= 16384), forward and backward:
  *   h = x (+ residual);  n = (h - mean) / sqrt(var + eps)  (CCQ_NORM_RMS: mean = 0, var = mean of h^2)
- *   y = n weight (+ bias);  with gate: y *= gate sigmoid(gate)
+ *   y = n weight (+ bias, CCQ_NORM_LAYER only);  with gate (CCQ_NORM_RMS without residual only):
+ *   y = n weight gate sigmoid(gate)
  *   weight and bias: fp32 [D] or NULL;  residual and gate: [rows, D] in x's dtype or NULL;
  *   h: written when residual is given (the sum in x's dtype; the norm reads the unrounded sum);
  *   stats: fp32 [rows, 2] mean and 1 / sqrt(var + eps), NULL when no backward follows.
