@@ -15,6 +15,7 @@ from .ops import (  # noqa: F401
     reshape_lambda_3d,
 )
 from .delta_rule import GatedDeltaRule, gated_delta_rule, gated_delta_step  # noqa: F401
+from .mixer import ccq_gated_delta_rule, ccq_gated_delta_step  # noqa: F401
 from .norm import LayerNorm, gated_rms_norm, layer_norm, rms_norm  # noqa: F401
 from ._lib import CCQError, last_launch_count, last_path  # noqa: F401
 

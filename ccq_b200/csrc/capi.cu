@@ -633,9 +633,6 @@ int ln_args(ccq::LayerNormArgs* out, int dtype, int form, int64_t rows, int D, f
   if (D > ccq::LN_MAX_D) return fail(CCQ_ERR_UNSUPPORTED, "row size D=%d > %d is not supported", D, ccq::LN_MAX_D);
   if (rows > 0x7FFFFFFF) return fail(CCQ_ERR_UNSUPPORTED, "rows=%lld is too large", (long long)rows);
   if (!(eps >= 0.f)) return fail(CCQ_ERR_INVALID, "eps must not be negative");
-  if (form == CCQ_NORM_RMS && bias != nullptr) return fail(CCQ_ERR_UNSUPPORTED, "the RMS form takes no bias");
-  if (gate != nullptr && (form != CCQ_NORM_RMS || residual != nullptr))
-    return fail(CCQ_ERR_UNSUPPORTED, "a gate goes with the RMS form without residual");
   if (rows > 0 && x == nullptr) return fail(CCQ_ERR_INVALID, "x is required");
   ccq::LayerNormArgs a;
   memset(&a, 0, sizeof(a));
@@ -654,6 +651,13 @@ int ln_args(ccq::LayerNormArgs* out, int dtype, int form, int64_t rows, int D, f
   return CCQ_OK;
 }
 
+int ln_combination(const ccq::LayerNormArgs& a) {
+  if (a.form == CCQ_NORM_RMS && a.bias != nullptr) return fail(CCQ_ERR_UNSUPPORTED, "the RMS form takes no bias");
+  if (a.gate != nullptr && (a.form != CCQ_NORM_RMS || a.residual != nullptr))
+    return fail(CCQ_ERR_UNSUPPORTED, "a gate goes with the RMS form without residual");
+  return CCQ_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -668,6 +672,8 @@ int ccq_layer_norm_fwd(int dtype, int form, int64_t rows, int D, float eps, cons
   if (rows > 0 && y == nullptr) return fail(CCQ_ERR_INVALID, "the output y is required");
   if (rows > 0 && residual != nullptr && h == nullptr) return fail(CCQ_ERR_INVALID, "h is required with residual");
   if ((uintptr_t)stats & 7) return fail(CCQ_ERR_INVALID, "stats must be 8-byte aligned");
+  st = ln_combination(a);
+  if (st != CCQ_OK) return st;
   a.y = y;
   a.h = h;
   a.stats = reinterpret_cast<float2*>(stats);
@@ -691,6 +697,8 @@ int ccq_layer_norm_bwd(int dtype, int form, int64_t rows, int D, const void* x, 
     return fail(CCQ_ERR_INVALID, "stats, dy and dx are required");
   if (rows > 0 && gate != nullptr && dgate == nullptr) return fail(CCQ_ERR_INVALID, "dgate is required with gate");
   if ((uintptr_t)stats & 7) return fail(CCQ_ERR_INVALID, "stats must be 8-byte aligned");
+  st = ln_combination(a);
+  if (st != CCQ_OK) return st;
   a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
   a.dy = dy;
   a.dh = dh;

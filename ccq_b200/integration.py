@@ -23,16 +23,19 @@ for this path, so the unchanged layers run the B200 kernels:
   rebuilt here around the B200 decode step and fla's ``fused_recurrent_gla`` backbone, and its
   imported copy in ``ccq.gla.layer``.
 
-The backbones (fla's chunk_gated_delta_rule, chunk_gla, fused_recurrent_*) are untouched.
-``uninstall()`` restores the reference's own functions.
+The backbones (fla's chunk_gated_delta_rule, chunk_gla, fused_recurrent_*) are untouched by default;
+``install(backbone='b200')`` makes the two GDN orchestrators read ``delta_rule.gated_delta_rule`` instead of
+fla's chunk_gated_delta_rule.  ``uninstall()`` restores the reference's own functions.
 """
 from __future__ import annotations
 
 import importlib
 
 from . import ops
+from .delta_rule import gated_delta_rule
 
 _saved = {}
+_backbone = 'fla'
 
 
 def _set(module_name, attr, value):
@@ -62,14 +65,35 @@ def fused_recurrent_ccq_gla(q, k, v, lambda_h, gk=None, gv=None, scale=None, ini
     return o, final_state, final_cov_state, final_mean_state
 
 
+def _b200_gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, output_final_state=False,
+                           use_qk_l2norm_in_kernel=False, cu_seqlens=None, cp_context=None, transpose_state_layout=False,
+                           **kwargs):
+    """fla's chunk_gated_delta_rule call on this framework's operator."""
+    if cp_context is not None or transpose_state_layout or kwargs:
+        raise ValueError('the B200 gated delta rule takes no cp_context, transpose_state_layout or '
+                         f'{", ".join(kwargs) or "other options"}; use install(backbone="fla") for these')
+    if use_qk_l2norm_in_kernel:
+        q, k = ops.l2norm(q), ops.l2norm(k)
+    return gated_delta_rule(q, k, v, g, beta, scale=scale, initial_state=initial_state,
+                            output_final_state=output_final_state, cu_seqlens=cu_seqlens)
+
+
+def _gated_delta_rule():
+    if _backbone == 'b200':
+        return _b200_gated_delta_rule
+    from fla.ops.gated_delta_rule import chunk_gated_delta_rule
+    return chunk_gated_delta_rule
+
+
 def fused_chunk_ccq_gdn(q, k, v, lambda_h, g, beta, scale=None, initial_state=None, initial_cov_state=None,
                         initial_mean_state=None, output_final_state=False, use_qk_l2norm_in_kernel=False,
                         cu_seqlens=None, position_offset=0, subtract_mean=True, enable_ccq=True, **kwargs):
     """CCQ-GDN, attn_mode "fused_chunk" (ccq/ops/ccq_gdn/fused_chunk.py:16-59): the B200 cleaning, with
-    the l2norm of q and k fused into it, then fla's chunk_gated_delta_rule on (q_clean, k_norm).
+    the l2norm of q and k fused into it, then the gated delta rule (fla's chunk_gated_delta_rule, or this framework's: see
+    ``install``) on (q_clean, k_norm).
 
     Same arguments and returns: (o, final_state, final_cov_state, final_mean_state)."""
-    from fla.ops.gated_delta_rule import chunk_gated_delta_rule
+    chunk_gated_delta_rule = _gated_delta_rule()
     if not enable_ccq:
         o, final_state = chunk_gated_delta_rule(q=q, k=k, v=v, g=g, beta=beta, scale=scale, initial_state=initial_state,
                                                 output_final_state=output_final_state,
@@ -109,7 +133,7 @@ def chunk_ccq_gdn(q, k, v, lambda_h, g, beta, scale=None, initial_state=None, in
     context-parallel ``cp_context`` the cleaning carries its (C, m) state across the ranks
     (``distributed.cp_clean_read``), which the reference's chunk path does not do.
     Same arguments and returns: (o, final_state, final_cov_state, final_mean_state)."""
-    from fla.ops.gated_delta_rule import chunk_gated_delta_rule
+    chunk_gated_delta_rule = _gated_delta_rule()
     if not enable_ccq:
         o, final_state = chunk_gated_delta_rule(q=q, k=k, v=v, g=g, beta=beta, scale=scale, initial_state=initial_state,
                                                 output_final_state=output_final_state,
@@ -160,9 +184,14 @@ def _clean(q, k, lambda_h, l2norm_qk, position_offset, initial_cov_state, initia
     return qc, k, fc, fm
 
 
-def install():
+def install(backbone='fla'):
     """Route the reference package's cleaning operator, its attn_mode orchestrators and decode step to
-    the B200 kernels."""
+    the B200 kernels.  ``backbone``: whose gated delta rule the GDN orchestrators call after the cleaning,
+    'fla' (the reference's own) or 'b200'."""
+    global _backbone
+    if backbone not in ('fla', 'b200'):
+        raise ValueError(f"backbone must be 'fla' or 'b200', got {backbone!r}")
+    _backbone = backbone
     _set('ccq.ops.common.fused_read', 'fused_ccq_clean_read', ops.fused_ccq_clean_read)
     _set('ccq.ops.common.fused_read', 'FusedCCQCleanRead', ops.FusedCCQCleanRead)
     _set('ccq.ops.ccq_gdn.fused_chunk', 'fused_ccq_clean_read', ops.fused_ccq_clean_read)
@@ -190,7 +219,9 @@ def install():
 
 
 def uninstall():
-    """Restore every name install() replaced."""
+    """Restore every name install() replaced, and fla's backbone."""
+    global _backbone
+    _backbone = 'fla'
     for (module_name, attr), value in list(_saved.items()):
         setattr(importlib.import_module(module_name), attr, value)
     _saved.clear()

@@ -82,3 +82,19 @@ def test_layer_norm_bwd_refusals(lib):
     assert lib.ccq_layer_norm_bwd(*args(gate=16)) == 1 and 'dgate' in lib.ccq_last_error().decode()
     assert lib.ccq_layer_norm_bwd(*args(n=need - 1)) == 4
     assert lib.ccq_layer_norm_bwd(*args(ws=None)) == 4
+
+
+def test_layer_norm_combinations(lib):
+    need = lib.ccq_layer_norm_workspace_size(1, 4, 64)
+    for form, residual, bias, gate in ((1, None, 16, None), (0, None, None, 16), (1, 16, None, 16)):
+        st = lib.ccq_layer_norm_fwd(1, form, 4, 64, 1e-5, P(16), P(residual), None, P(bias), P(gate), P(16), P(16), None, None)
+        assert st == 2 and lib.ccq_last_error()
+        st = lib.ccq_layer_norm_bwd(1, form, 4, 64, P(16), P(residual), None, P(bias), P(gate), P(16), P(16), None, P(16), P(16),
+                                    None, None, P(16), need, None)
+        assert st == 2 and lib.ccq_last_error()
+
+
+def test_gdr_workspace_flags(lib):
+    size = lambda op, flags: lib.ccq_gdr_workspace_size(op, 1, 1, 1000, 2, 4, 128, 128, 1, flags)  # noqa: E731
+    assert size(0, 1) > 0 and size(1, 0) > size(1, 2) > 0       # without the forward's workspace the backward needs more
+    assert size(1, 4) > 0 and size(0, 4) != size(0, 0)          # an unaligned call takes the exact path
