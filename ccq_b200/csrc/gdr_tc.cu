@@ -52,7 +52,7 @@ bool gdr_tc_supported(const GdrArgs& a) {
   const uintptr_t p = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o | (uintptr_t)a.d_o |
                       (uintptr_t)a.dq | (uintptr_t)a.dk | (uintptr_t)a.dv | (uintptr_t)a.workspace |
                       (uintptr_t)a.fwd_workspace;
-  return (p & 15) == 0 && tc::encode_fn() != nullptr;
+  return (p & 15) == 0;
 }
 
 size_t gdr_tc_workspace(const GdrArgs& a, bool bwd) {
