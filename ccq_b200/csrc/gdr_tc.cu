@@ -1,4 +1,5 @@
 // Tensor-core path of the gated delta rule: when it applies, its workspace and its launches.
+#include <stdlib.h>
 #include <string.h>
 
 #include "gdr_tc.cuh"
@@ -21,11 +22,15 @@ size_t carve(const GdrArgs& a, bool bwd, Ws* w) {
   Ws t;
   memset(&t, 0, sizeof(t));
   t.err = reinterpret_cast<int*>(take(256));
+  const size_t order = lpt_order_bytes(a.n_seqs, a.cu_seqlens != nullptr);
   if (a.fwd_workspace == nullptr) {
+    t.order = order ? reinterpret_cast<int*>(take(order)) : nullptr;
     t.mats = take(sh * MATS);
     t.aux = reinterpret_cast<float*>(take(sh * AX_N * 4));
   } else {  // as the forward left them: the same carving of its workspace
     uint8_t* f = reinterpret_cast<uint8_t*>(const_cast<void*>(a.fwd_workspace)) + ws_align(256);
+    t.order = order ? reinterpret_cast<int*>(f) : nullptr;
+    f += order;
     t.mats = f;
     t.aux = reinterpret_cast<float*>(f + ws_align(sh * MATS));
   }
@@ -43,9 +48,26 @@ size_t carve(const GdrArgs& a, bool bwd, Ws* w) {
   return off;
 }
 
+// What the scans start from: the launch order of packed documents, the chunks' inverses, scores and factors.
+cudaError_t start(const GdrArgs& a, const Ws& w, int* launches) {
+  cudaError_t e = cudaSuccess;
+  if (w.order) {
+    CleanArgs c;
+    memset(&c, 0, sizeof(c));
+    c.T = a.T;
+    c.n_seqs = a.n_seqs;
+    c.cu_seqlens = a.cu_seqlens;
+    c.stream = a.stream;
+    e = lpt_order(c, const_cast<int*>(w.order), launches);
+  }
+  return e == cudaSuccess ? prep(a, w, launches) : e;
+}
+
 }  // namespace
 
 bool gdr_tc_supported(const GdrArgs& a) {
+  const char* env = getenv("CCQ_B200_FORCE_SIMT");
+  if (env && env[0] == '1') return false;
   if (a.dtype != DT_BF16 && a.dtype != DT_F16) return false;
   if (a.T < 1 || a.K > 128 || a.K % 8 != 0 || a.V % 8 != 0) return false;
   if (gdr_slots(a, C) * a.HV >= (1ll << 31)) return false;  // the kernels count (chunk, head) pairs in 32 bits
@@ -65,7 +87,7 @@ cudaError_t gdr_tc_fwd(const GdrArgs& a, int* launches) {
   Ws w;
   carve(a, false, &w);
   cudaError_t e = cudaMemsetAsync(w.err, 0, 8, a.stream);
-  if (e == cudaSuccess) e = prep(a, w, launches);
+  if (e == cudaSuccess) e = start(a, w, launches);
   if (e == cudaSuccess) e = scan(a, w, false, launches);
   return e;
 }
@@ -74,7 +96,7 @@ cudaError_t gdr_tc_bwd(const GdrArgs& a, int* launches) {
   Ws w;
   carve(a, true, &w);
   cudaError_t e = cudaMemsetAsync(w.err, 0, 8, a.stream);
-  if (e == cudaSuccess && a.fwd_workspace == nullptr) e = prep(a, w, launches);
+  if (e == cudaSuccess && a.fwd_workspace == nullptr) e = start(a, w, launches);
   if (e == cudaSuccess) e = scan(a, w, true, launches);
   if (e == cudaSuccess) e = rscan(a, w, launches);
   if (e == cudaSuccess) e = grads(a, w, launches);

@@ -39,6 +39,7 @@ constexpr int ANCHOR = 8;
 // Workspace regions; every kernel indexes them by sh = slot * HV + value head.
 struct Ws {
   int* err;            // word 0: device error code of the scans
+  const int* order;    // launch slot -> document of a packed batch, longest first; nullptr: as they come
   uint8_t* mats;       // [slots * HV][MATS]
   float* aux;          // [slots * HV][AX_N]
   // backward only
@@ -66,6 +67,12 @@ cudaError_t grads(const GdrArgs& a, const Ws& w, int* launches);
 namespace ccq {
 namespace gdrtc {
 
+// 2^x by the hardware's approximation (2 ulp; below 2^-126 it is zero, as it may be for a decay)
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // two fp32 operations in one instruction
 __device__ __forceinline__ uint64_t pair(float x, float y) {
   uint64_t r;

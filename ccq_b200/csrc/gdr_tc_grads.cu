@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               const float h4[4] = {hj.x, hj.y, hj.z, hj.w}, l4[4] = {lj.x, lj.y, lj.z, lj.w}, b4[4] = {bj.x, bj.y, bj.z, bj.w};
 #pragma unroll
               for (int f = 0; f < 4; ++f) {
-                const float d = j + f <= top ? sx * exp2f((gh - h4[f]) + (gl - l4[f])) * x[e + f] : 0.f;
+                const float d = j + f <= top ? sx * ex2((gh - h4[f]) + (gl - l4[f])) * x[e + f] : 0.f;
                 z[8 * cc + e + f] = d * y[e + f];
                 x[e + f] = d * b4[f];
               }

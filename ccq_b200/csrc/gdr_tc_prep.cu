@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(128)
     for (int j = 0; j < 2; ++j) {
       const int t = 2 * lane + j;
       const double x = Gs[j];
-      const float gam = exp2f((float)x), wt = exp2f((float)(last - x));
+      const float gam = ex2((float)x), wt = ex2((float)(last - x));
       S.gh[t] = ax[AX_GH + t] = (float)x;
       S.gl[t] = ax[AX_GL + t] = (float)(x - (double)(float)x);
       S.beta[t] = ax[AX_B + t] = b[j];
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(128)
       ax[AX_WB + t] = wt * b[j];
       ax[AX_W + t] = wt;
     }
-    if (lane < AX_N - AX_GC) ax[AX_GC + lane] = lane == 0 ? exp2f((float)last) : 0.f;
+    if (lane < AX_N - AX_GC) ax[AX_GC + lane] = lane == 0 ? ex2((float)last) : 0.f;
   }
   __syncthreads();
   // the copy's bytes always arrive; the bound only keeps a broken launch from hanging
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(128)
       for (int hr = 0; hr < 2; ++hr) {
         const int i = i0 + 8 * hr;
         const bool in = i < valid;
-        const float d0 = exp2f((gh[hr] - hj.x) + (gl[hr] - lj.x)) * bj.x, d1 = exp2f((gh[hr] - hj.y) + (gl[hr] - lj.y)) * bj.y;
+        const float d0 = ex2((gh[hr] - hj.x) + (gl[hr] - lj.x)) * bj.x, d1 = ex2((gh[hr] - hj.y) + (gl[hr] - lj.y)) * bj.y;
         const float a0 = in && j0 < i ? d0 * kk[nt][2 * hr] : 0.f, a1 = in && j0 + 1 < i ? d1 * kk[nt][2 * hr + 1] : 0.f;
         const float p0 = in && j0 <= i ? a.scale * d0 * qk[nt][2 * hr] : 0.f;
         const float p1 = in && j0 + 1 <= i ? a.scale * d1 * qk[nt][2 * hr + 1] : 0.f;

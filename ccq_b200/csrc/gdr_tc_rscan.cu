@@ -47,8 +47,10 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
   Small& S_ = *reinterpret_cast<Small*>(sm + L_SMALL);
   const uint32_t sb = smem_u32(sm);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = blockIdx.x / a.HV, hv = blockIdx.x % a.HV, h = hv / (a.HV / a.H);
-  const int v0 = blockIdx.y * VT;
+  // the V tiles of a head are neighbours, which read the same K, Q, T and P
+  const int nvt = (a.V + VT - 1) / VT, vt = blockIdx.x % nvt, head = blockIdx.x / nvt;
+  const int n = doc_of_slot(head / a.HV, w.order), hv = head % a.HV, h = hv / (a.HV / a.H);
+  const int v0 = vt * VT;
   const Seq sq = seq_of(n, a.T, a.cu_seqlens);
   const int nch = (sq.len + C - 1) / C;
   const int64_t sh0 = gdr_slot0(a, n, sq, C) * a.HV + hv;  // chunk c is at sh0 + c * HV
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
           if (KH * hh + i < a.K) d = fmaf(S[i], g[(int64_t)(KH * hh + i) * a.V], d);
       }
       d = warp_sum(d);
-      if (lane == 0) w.anchor[((int64_t)blockIdx.y * anchors * a.HV + at) * G::CHAIN_WARPS + warp - G::CHAIN] = d;
+      if (lane == 0) w.anchor[((int64_t)vt * anchors * a.HV + at) * G::CHAIN_WARPS + warp - G::CHAIN] = d;
     };
     if (nch > 0) {
       put_state(0);
@@ -397,7 +399,7 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
       }
       if (threadIdx.x < C) {
         const int i = threadIdx.x;
-        w.dotV[((int64_t)blockIdx.y * slots * a.HV + sh0 + (int64_t)c * a.HV) * C + i] =
+        w.dotV[((int64_t)vt * slots * a.HV + sh0 + (int64_t)c * a.HV) * C + i] =
             S_.red[0][i] + S_.red[1][i] + S_.red[2][i] + S_.red[3][i];
       }
       bar_sync<1, G::OUT_THREADS>();  // the sums are read before the next chunk's are written
@@ -422,7 +424,7 @@ cudaError_t launch(const GdrArgs& a, const Ws& w) {
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(rscan_kernel<AB16, KD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L_BYTES);
   if (e != cudaSuccess) return e;
-  rscan_kernel<AB16, KD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), BwdWarps::THREADS, L_BYTES, a.stream>>>(q, k, v, o, dv, st, a, w);
+  rscan_kernel<AB16, KD><<<a.n_seqs * a.HV * ((a.V + VT - 1) / VT), BwdWarps::THREADS, L_BYTES, a.stream>>>(q, k, v, o, dv, st, a, w);
   return cudaGetLastError();
 }
 

@@ -63,8 +63,10 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
   Small& S_ = *reinterpret_cast<Small*>(sm + L::SMALL);
   const uint32_t sb = smem_u32(sm);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = blockIdx.x / a.HV, hv = blockIdx.x % a.HV, h = hv / (a.HV / a.H);
-  const int v0 = blockIdx.y * VT;
+  // the V tiles of a head are neighbours, which read the same K, Q, T and P
+  const int nvt = (a.V + VT - 1) / VT, vt = blockIdx.x % nvt, head = blockIdx.x / nvt;
+  const int n = doc_of_slot(head / a.HV, w.order), hv = head % a.HV, h = hv / (a.HV / a.H);
+  const int v0 = vt * VT;
   const Seq sq = seq_of(n, a.T, a.cu_seqlens);
   const int nch = (sq.len + C - 1) / C;
   const int64_t sh0 = gdr_slot0(a, n, sq, C) * a.HV + hv;  // chunk c is at sh0 + c * HV
@@ -416,7 +418,7 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
         bar_sync<1, G::OUT_THREADS>();
         if (threadIdx.x < C) {
           const int i = threadIdx.x;
-          w.dotO[((int64_t)blockIdx.y * slots * a.HV + sh0 + (int64_t)c * a.HV) * C + i] =
+          w.dotO[((int64_t)vt * slots * a.HV + sh0 + (int64_t)c * a.HV) * C + i] =
               S_.red[0][i] + S_.red[1][i] + S_.red[2][i] + S_.red[3][i];
         }
         bar_sync<1, G::OUT_THREADS>();
@@ -445,7 +447,7 @@ cudaError_t launch(const GdrArgs& a, const Ws& w) {
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(scan_kernel<AB16, KD, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e != cudaSuccess) return e;
-  scan_kernel<AB16, KD, BWD><<<dim3(a.n_seqs * a.HV, (a.V + VT - 1) / VT), Warps<BWD>::THREADS, bytes, a.stream>>>(q, k, v, o, st, e16, a, w);
+  scan_kernel<AB16, KD, BWD><<<a.n_seqs * a.HV * ((a.V + VT - 1) / VT), Warps<BWD>::THREADS, bytes, a.stream>>>(q, k, v, o, st, e16, a, w);
   return cudaGetLastError();
 }
 
