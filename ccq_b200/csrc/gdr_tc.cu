@@ -22,18 +22,29 @@ size_t carve(const GdrArgs& a, bool bwd, Ws* w) {
   Ws t;
   memset(&t, 0, sizeof(t));
   t.err = reinterpret_cast<int*>(take(256));
-  const size_t order = lpt_order_bytes(a.n_seqs, a.cu_seqlens != nullptr);
-  if (a.fwd_workspace == nullptr) {
-    t.order = order ? reinterpret_cast<int*>(take(order)) : nullptr;
-    t.mats = take(sh * MATS);
-    t.aux = reinterpret_cast<float*>(take(sh * AX_N * 4));
-  } else {  // as the forward left them: the same carving of its workspace
-    uint8_t* f = reinterpret_cast<uint8_t*>(const_cast<void*>(a.fwd_workspace)) + ws_align(256);
-    t.order = order ? reinterpret_cast<int*>(f) : nullptr;
-    f += order;
-    t.mats = f;
-    t.aux = reinterpret_cast<float*>(f + ws_align(sh * MATS));
+  // what the forward leaves for the backward: in its workspace, here if that is not given
+  uint8_t* here = base;
+  const size_t at = off;
+  if (a.fwd_workspace != nullptr) {
+    base = reinterpret_cast<uint8_t*>(const_cast<void*>(a.fwd_workspace));
+    off = ws_align(256);
   }
+  const size_t order = lpt_order_bytes(a.n_seqs, a.cu_seqlens != nullptr);
+  const size_t heads = (size_t)a.n_seqs * a.HV, states = heads * a.K * a.V * 4;
+  t.nseg = plan_segments(a, &t.seg_chunks);
+  t.order = order ? reinterpret_cast<int*>(take(order)) : nullptr;
+  t.mats = take(sh * MATS);
+  t.aux = reinterpret_cast<float*>(take(sh * AX_N * 4));
+  if (t.nseg > 1) {
+    t.Sin = reinterpret_cast<float*>(take(t.nseg * states));
+    t.Ms = reinterpret_cast<float*>(take(t.nseg * heads * a.K * a.K * 4));
+  }
+  if (a.fwd_workspace != nullptr) {
+    base = here;
+    off = at;
+  }
+  if (t.nseg > 1) t.Bs = reinterpret_cast<float*>(take(t.nseg * states));
+  if (t.nseg > 1 && bwd) t.dSend = reinterpret_cast<float*>(take(t.nseg * states));
   if (bwd) {
     t.S0 = reinterpret_cast<uint16_t*>(take(sh * a.K * a.V * 2));
     t.dS1 = reinterpret_cast<uint16_t*>(take(sh * a.K * a.V * 2));
@@ -48,7 +59,8 @@ size_t carve(const GdrArgs& a, bool bwd, Ws* w) {
   return off;
 }
 
-// What the scans start from: the launch order of packed documents, the chunks' inverses, scores and factors.
+// What the scans start from: the launch order of packed documents, the chunks' inverses, scores and factors, the
+// states at the starts of segments.
 cudaError_t start(const GdrArgs& a, const Ws& w, int* launches) {
   cudaError_t e = cudaSuccess;
   if (w.order) {
@@ -60,7 +72,10 @@ cudaError_t start(const GdrArgs& a, const Ws& w, int* launches) {
     c.stream = a.stream;
     e = lpt_order(c, const_cast<int*>(w.order), launches);
   }
-  return e == cudaSuccess ? prep(a, w, launches) : e;
+  if (e == cudaSuccess) e = prep(a, w, launches);
+  if (e == cudaSuccess && w.nseg > 1) e = scan(a, w, SCAN_SUM, launches);
+  if (e == cudaSuccess && w.nseg > 1) e = join(a, w, false, launches);
+  return e;
 }
 
 }  // namespace
@@ -88,7 +103,7 @@ cudaError_t gdr_tc_fwd(const GdrArgs& a, int* launches) {
   carve(a, false, &w);
   cudaError_t e = cudaMemsetAsync(w.err, 0, 8, a.stream);
   if (e == cudaSuccess) e = start(a, w, launches);
-  if (e == cudaSuccess) e = scan(a, w, false, launches);
+  if (e == cudaSuccess) e = scan(a, w, SCAN_FWD, launches);
   return e;
 }
 
@@ -97,8 +112,10 @@ cudaError_t gdr_tc_bwd(const GdrArgs& a, int* launches) {
   carve(a, true, &w);
   cudaError_t e = cudaMemsetAsync(w.err, 0, 8, a.stream);
   if (e == cudaSuccess && a.fwd_workspace == nullptr) e = start(a, w, launches);
-  if (e == cudaSuccess) e = scan(a, w, true, launches);
-  if (e == cudaSuccess) e = rscan(a, w, launches);
+  if (e == cudaSuccess) e = scan(a, w, SCAN_BWD, launches);
+  if (e == cudaSuccess && w.nseg > 1) e = rscan(a, w, true, launches);
+  if (e == cudaSuccess && w.nseg > 1) e = join(a, w, true, launches);
+  if (e == cudaSuccess) e = rscan(a, w, false, launches);
   if (e == cudaSuccess) e = grads(a, w, launches);
   return e;
 }

@@ -42,6 +42,14 @@ struct Ws {
   const int* order;    // launch slot -> document of a packed batch, longest first; nullptr: as they come
   uint8_t* mats;       // [slots * HV][MATS]
   float* aux;          // [slots * HV][AX_N]
+  // Few heads, a long axis: documents are cut into nseg segments of seg_chunks chunks (a multiple of ANCHOR),
+  // which run side by side once the states at their starts are known (gdr_tc_seg.cu).  Index s * heads + head,
+  // heads = n_seqs * HV.
+  int nseg, seg_chunks;
+  float* Sin;          // [nseg][heads][K][V] state at a segment's start
+  float* Bs;           // [nseg][heads][K][V] its end from a zero (first: the given) state; backwards: its start's gradient
+  float* Ms;           // [nseg][heads][K][K] its end as a linear map of its start
+  float* dSend;        // [nseg][heads][K][V] gradient of the state at a segment's end (backward)
   // backward only
   uint16_t* S0;        // [slots * HV][V][K] state before the chunk, transposed, 16-bit
   uint16_t* dS1;       // [slots * HV][V][K] gradient of the state after it
@@ -53,8 +61,12 @@ struct Ws {
 };
 
 cudaError_t prep(const GdrArgs& a, const Ws& w, int* launches);
-cudaError_t scan(const GdrArgs& a, const Ws& w, bool bwd, int* launches);
-cudaError_t rscan(const GdrArgs& a, const Ws& w, int* launches);
+enum ScanMode { SCAN_FWD, SCAN_BWD, SCAN_SUM };  // output; for the backward; a segment's end state only
+cudaError_t scan(const GdrArgs& a, const Ws& w, ScanMode mode, int* launches);
+cudaError_t rscan(const GdrArgs& a, const Ws& w, bool sum, int* launches);
+// the states at the segments' starts from their summaries; backwards, the gradients at their ends
+cudaError_t join(const GdrArgs& a, const Ws& w, bool reverse, int* launches);
+int plan_segments(const GdrArgs& a, int* seg_chunks);
 cudaError_t grads(const GdrArgs& a, const Ws& w, int* launches);
 
 }  // namespace gdrtc
@@ -155,6 +167,23 @@ __device__ __forceinline__ uint16_t f2h(float x) {
   if (AB16) return __bfloat16_as_ushort(__float2bfloat16_rn(x));
   return __half_as_ushort(__float2half_rn(x));
 }
+
+// The chunks [c0, c1) of its document that a block walks, as a document of its own.
+struct Segment {
+  Seq doc, sq;       // whole; this block's part
+  int c0, c1, nch;   // nch: chunks of the whole document
+  bool live;
+  __device__ __forceinline__ Segment(const GdrArgs& a, const Ws& w, int n, int s) {
+    doc = seq_of(n, a.T, a.cu_seqlens);
+    nch = (doc.len + C - 1) / C;
+    c0 = s * w.seg_chunks;
+    c1 = w.nseg == 1 ? nch : min(nch, c0 + w.seg_chunks);
+    live = s == 0 || c0 < nch;
+    sq.bos = doc.bos + (int64_t)c0 * C;
+    sq.len = min(doc.len - c0 * C, (c1 - c0) * C);
+  }
+  __device__ __forceinline__ bool last() const { return c1 == nch; }
+};
 
 // A [64 tokens x 128 columns] tile of two swizzled panels, read or written one column per thread:
 // `col` 0..127 is the thread's column.

@@ -36,7 +36,9 @@ constexpr uint32_t L_OUT = 2 * L_STAGE, L_SMALL = L_OUT + TILE;
 constexpr uint32_t L_BYTES = L_SMALL + sizeof(Small) + 1024;
 static_assert(L_BYTES <= 232448, "shared memory");
 
-template <int AB16, int KD>
+// SUM: nothing is written but the gradient at the segment's start, from a zero one at its end (the document's
+// last segment: the given one)
+template <int AB16, int KD, bool SUM>
 __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
     rscan_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                  const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmo,
@@ -48,13 +50,19 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
   const uint32_t sb = smem_u32(sm);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the V tiles of a head are neighbours, which read the same K, Q, T and P
-  const int nvt = (a.V + VT - 1) / VT, vt = blockIdx.x % nvt, head = blockIdx.x / nvt;
+  const int nvt = (a.V + VT - 1) / VT, vt = blockIdx.x % nvt, seg = blockIdx.x / nvt % w.nseg, head = blockIdx.x / nvt / w.nseg;
   const int n = doc_of_slot(head / a.HV, w.order), hv = head % a.HV, h = hv / (a.HV / a.H);
   const int v0 = vt * VT;
-  const Seq sq = seq_of(n, a.T, a.cu_seqlens);
-  const int nch = (sq.len + C - 1) / C;
-  const int64_t sh0 = gdr_slot0(a, n, sq, C) * a.HV + hv;  // chunk c is at sh0 + c * HV
-  const int64_t st = ((int64_t)n * a.HV + hv) * a.K * a.V;
+  const Segment part(a, w, n, seg);
+  if (!part.live || (SUM && seg == 0)) return;
+  const Seq sq = part.sq;
+  const int nch = part.c1 - part.c0;
+  const int64_t sh0 = (gdr_slot0(a, n, part.doc, C) + part.c0) * a.HV + hv;  // chunk c is at sh0 + c * HV
+  const int64_t heads = (int64_t)a.n_seqs * a.HV, nh = (int64_t)n * a.HV + hv;
+  const float* last = part.last() ? (a.dfinal_state ? a.dfinal_state + nh * a.K * a.V : nullptr)
+                      : SUM ? nullptr : w.dSend + (seg * heads + nh) * a.K * a.V;
+  float* start = SUM ? w.Bs + (seg * heads + nh) * a.K * a.V
+                 : (seg == 0 && a.dinitial_state ? a.dinitial_state + nh * a.K * a.V : nullptr);
   constexpr int NP = KD / 64;  // panels of K and Q
   constexpr int CT = G::CT, OT = G::OT;
 
@@ -83,7 +91,7 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
   const uint32_t tb = S_.tmem;
   volatile int* ab = &S_.abort;
   int* err = w.err;
-  const bool part = sq.len % C != 0;  // the last chunk, the first one here, is partial
+  const bool partial = sq.len % C != 0;  // the last chunk, the first one here, is partial
 
   if (warp >= G::TMA) G::rest_regs();
   if (warp == G::TMA) {
@@ -96,7 +104,7 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
         if (*ab) break;
         uint8_t* p = sm + s * L_STAGE;
         uint64_t* bar = &S_.full[s];
-        mbar_arrive_expect_tx(bar, 2 * NP * PANEL + 2 * TILE + MATS + AX_N * 4);
+        mbar_arrive_expect_tx(bar, 2 * NP * PANEL + (SUM ? 1 : 2) * TILE + MATS + AX_N * 4);
         const int row = (int)(sq.bos + (int64_t)c * C);
         const int64_t sh = sh0 + (int64_t)c * a.HV;
         for (int i = 0; i < NP; ++i) tma_load_3d(p + L_KQ + 2 * i * PANEL, &tmk, bar, 64 * i, h, row);
@@ -105,8 +113,10 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
         bulk_load(p + L_AX, w.aux + sh * AX_N, AX_N * 4, bar);
         bulk_load(p + L_M, w.mats + sh * MATS, MATS, bar);
         for (int i = 0; i < NP; ++i) tma_load_3d(p + L_KQ + (2 * i + 1) * PANEL, &tmq, bar, 64 * i, h, row);
-        tma_load_3d(p + L_V, &tmv, bar, v0, hv, row);
-        tma_load_3d(p + L_V + PANEL, &tmv, bar, v0 + 64, hv, row);
+        if (!SUM) {
+          tma_load_3d(p + L_V, &tmv, bar, v0, hv, row);
+          tma_load_3d(p + L_V + PANEL, &tmv, bar, v0 + 64, hv, row);
+        }
         ++issued;
       }
       // never leave the block with copies in flight
@@ -123,9 +133,9 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
         const uint32_t p = sb + s * L_STAGE;
         const uint32_t T = p + L_M, P = T + 2 * PANEL;
         if (!spin_wait(&S_.full[s], (t >> 1) & 1, ab, err, 4)) break;
-        if (t == 0 && part && !spin_wait(&S_.kz, 0, ab, err, 8)) break;
+        if (t == 0 && partial && !spin_wait(&S_.kz, 0, ab, err, 8)) break;
         // Z^T over the dV of the chunk before
-        if (t > 0 && !spin_wait(&S_.f_read, (t - 1) & 1, ab, err, 0x20)) break;
+        if (t > 0 && !SUM && !spin_wait(&S_.f_read, (t - 1) & 1, ab, err, 0x20)) break;
         tc_fence_after();
 #pragma unroll
         for (int x = 0; x < 2; ++x)
@@ -189,7 +199,7 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
 #pragma unroll
     for (int i = 0; i < KH; ++i) {
       const int k = KH * hh + i;
-      S[i] = (a.dfinal_state && vin && k < a.K) ? a.dfinal_state[st + (int64_t)k * a.V + v0 + vl] : 0.f;
+      S[i] = (last && vin && k < a.K) ? last[(int64_t)k * a.V + v0 + vl] : 0.f;
     }
     // dS as the operand of chunk c; its hi part also goes to `tile` (two panels of 128 rows), or straight
     // to the workspace for the first chunk
@@ -206,7 +216,7 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
           const uint32_t pan = tile + (k >> 6) * 2 * PANEL;
           sts128(pan + sw128(vl, (k & 63) >> 3), u);
           sts128(pan + sw128(vl, ((k & 63) >> 3) + 1), v);
-        } else if (vin) {
+        } else if (vin && !SUM) {
           uint16_t* g = w.dS1 + ((sh0 + (int64_t)(nch - 1) * a.HV) * a.V + v0 + vl) * a.K + k;
           if (k < a.K) *reinterpret_cast<uint4*>(g) = u;
           if (k + 8 < a.K) *reinterpret_cast<uint4*>(g + 8) = v;
@@ -219,7 +229,7 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
     // <dS, S> at the end of anchor group b, this warp's part
     const int64_t anchors = gdr_slots(a, C * ANCHOR);
     auto put_anchor = [&](int b, bool zero) {
-      const int64_t at = (gdr_slot0(a, n, sq, C * ANCHOR) + b) * a.HV + hv;
+      const int64_t at = (gdr_slot0(a, n, part.doc, C * ANCHOR) + b) * a.HV + hv;
       float d = 0.f;
       if (vin && !zero) {
         const float* g = w.Sf + at * a.K * a.V + v0 + vl;
@@ -232,7 +242,7 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
     };
     if (nch > 0) {
       put_state(0);
-      put_anchor((nch - 1) / ANCHOR, a.dfinal_state == nullptr);
+      if (!SUM && part.last()) put_anchor((part.nch - 1) / ANCHOR, a.dfinal_state == nullptr);
     }
     const int i0 = CT * hh;
     for (int t = 0; t < nch; ++t) {
@@ -304,21 +314,21 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
       fence_async_smem();
       bar_sync<2, G::CHAIN_THREADS>();
       if (threadIdx.x == 32 * G::CHAIN) {
-        if (c > 0)
+        if (c > 0 && !SUM)
           for (int i = 0; i < NP; ++i)
             if (64 * i < a.K)
               store_panel(&tms, sm + s * L_STAGE + L_KQ + 2 * i * PANEL, 64 * i, v0, a.V, sh0 + (int64_t)(c - 1) * a.HV);
         bulk_wait_read();  // then the stage may be loaded again
         mbar_arrive(&S_.empty[s]);
       }
-      if (c > 0 && c % ANCHOR == 0) put_anchor(c / ANCHOR - 1, false);
+      if (const int cd = part.c0 + c; !SUM && cd > 0 && cd % ANCHOR == 0) put_anchor(cd / ANCHOR - 1, false);
     }
     if (threadIdx.x == 32 * G::CHAIN) bulk_wait_all();
-    if (a.dinitial_state && vin) {
+    if (start && vin) {
 #pragma unroll
       for (int i = 0; i < KH; ++i) {
         const int k = KH * hh + i;
-        if (k < a.K) a.dinitial_state[st + (int64_t)k * a.V + v0 + vl] = S[i];
+        if (k < a.K) start[(int64_t)k * a.V + v0 + vl] = S[i];
       }
     }
   } else {
@@ -362,6 +372,10 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.g_ready);
+      if (SUM) {
+        warp_arrive(&S_.empty[s]);
+        continue;
+      }
       float y[OT];
       pipe_wait(&S_.f_full, ph, ab, err, 0x10000);
       tc_fence_after();
@@ -412,7 +426,7 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
   if (warp == G::MMA) tmem_dealloc(tb, 512);
 }
 
-template <int AB16, int KD>
+template <int AB16, int KD, bool SUM>
 cudaError_t launch(const GdrArgs& a, const Ws& w) {
   CUtensorMap q, k, v, o, dv, st;
   cudaError_t e = token_map(&q, a, a.q, a.H, a.K);
@@ -422,19 +436,25 @@ cudaError_t launch(const GdrArgs& a, const Ws& w) {
   if (e == cudaSuccess) e = token_map(&dv, a, a.dv, a.HV, a.V);
   if (e == cudaSuccess) e = matrix_map(&st, a, w.dS1, a.K, gdr_slots(a, C) * a.HV);
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(rscan_kernel<AB16, KD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L_BYTES);
+    e = cudaFuncSetAttribute(rscan_kernel<AB16, KD, SUM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L_BYTES);
   if (e != cudaSuccess) return e;
-  rscan_kernel<AB16, KD><<<a.n_seqs * a.HV * ((a.V + VT - 1) / VT), BwdWarps::THREADS, L_BYTES, a.stream>>>(q, k, v, o, dv, st, a, w);
+  const int64_t blocks = (int64_t)a.n_seqs * a.HV * w.nseg * ((a.V + VT - 1) / VT);
+  rscan_kernel<AB16, KD, SUM><<<(unsigned)blocks, BwdWarps::THREADS, L_BYTES, a.stream>>>(q, k, v, o, dv, st, a, w);
   return cudaGetLastError();
+}
+
+template <int AB16, int KD>
+cudaError_t pick(const GdrArgs& a, const Ws& w, bool sum) {
+  return sum ? launch<AB16, KD, true>(a, w) : launch<AB16, KD, false>(a, w);
 }
 
 }  // namespace
 
-cudaError_t rscan(const GdrArgs& a, const Ws& w, int* launches) {
+cudaError_t rscan(const GdrArgs& a, const Ws& w, bool sum, int* launches) {
   ++*launches;
   const bool small = a.K <= 64;
-  if (a.dtype == DT_BF16) return small ? launch<1, 64>(a, w) : launch<1, 128>(a, w);
-  return small ? launch<0, 64>(a, w) : launch<0, 128>(a, w);
+  if (a.dtype == DT_BF16) return small ? pick<1, 64>(a, w, sum) : pick<1, 128>(a, w, sum);
+  return small ? pick<0, 64>(a, w, sum) : pick<0, 128>(a, w, sum);
 }
 
 }  // namespace gdrtc

@@ -51,7 +51,9 @@ struct Lay {  // offsets of one stage, then of the rest
 };
 static_assert(Lay<true>::BYTES <= 232448 && Lay<false>::BYTES <= 232448, "shared memory");
 
-template <int AB16, int KD, bool BWD>
+// SUM: no output; the state at the segment's end from a zero state (the first segment: the given one) over its V,
+// or, in a head's last tile, as a linear map of the state at its start: the same walk from the identity without V.
+template <int AB16, int KD, bool BWD, bool SUM>
 __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
     scan_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                 const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmo,
@@ -64,20 +66,28 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
   const uint32_t sb = smem_u32(sm);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the V tiles of a head are neighbours, which read the same K, Q, T and P
-  const int nvt = (a.V + VT - 1) / VT, vt = blockIdx.x % nvt, head = blockIdx.x / nvt;
+  const int nvt = (a.V + VT - 1) / VT, tiles = SUM ? nvt + 1 : nvt, segs = SUM ? w.nseg - 1 : w.nseg;
+  const int vt = blockIdx.x % tiles, seg = blockIdx.x / tiles % segs, head = blockIdx.x / tiles / segs;
   const int n = doc_of_slot(head / a.HV, w.order), hv = head % a.HV, h = hv / (a.HV / a.H);
-  const int v0 = vt * VT;
-  const Seq sq = seq_of(n, a.T, a.cu_seqlens);
-  const int nch = (sq.len + C - 1) / C;
-  const int64_t sh0 = gdr_slot0(a, n, sq, C) * a.HV + hv;  // chunk c is at sh0 + c * HV
-  const int64_t st = ((int64_t)n * a.HV + hv) * a.K * a.V;
+  const bool map = SUM && vt == nvt;
+  const int v0 = map ? 0 : vt * VT, width = map ? a.K : a.V;  // of the state: columns it has
+  const Segment part(a, w, n, seg);
+  if (!part.live || (SUM && (part.last() || (map && seg == 0)))) return;
+  const Seq sq = part.sq;
+  const int nch = part.c1 - part.c0;
+  const int64_t sh0 = (gdr_slot0(a, n, part.doc, C) + part.c0) * a.HV + hv;  // chunk c is at sh0 + c * HV
+  const int64_t heads = (int64_t)a.n_seqs * a.HV, nh = (int64_t)n * a.HV + hv;
+  const float* first = seg == 0 ? (a.initial_state ? a.initial_state + nh * a.K * a.V : nullptr)
+                       : SUM ? nullptr : w.Sin + (seg * heads + nh) * a.K * a.V;
+  float* final = SUM ? (map ? w.Ms : w.Bs) + (seg * heads + nh) * a.K * width
+                 : (part.last() && a.final_state ? a.final_state + nh * a.K * a.V : nullptr);
   constexpr int NP = KD / 64;  // panels of K and Q
   constexpr int CT = G::CT, OT = G::OT;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&S_.full[i], 1);
-      mbar_init(&S_.empty[i], 1 + G::CHAIN_WARPS + G::OUT_WARPS);  // last commit, every chain and output warp
+      mbar_init(&S_.empty[i], 1 + G::CHAIN_WARPS + (SUM ? 0 : G::OUT_WARPS));  // last commit, every chain and output warp
     }
     mbar_init(&S_.s_ready, G::CHAIN_WARPS);
     mbar_init(&S_.r_ready, G::CHAIN_WARPS);
@@ -112,15 +122,18 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
         if (*ab) break;
         uint8_t* p = sm + s * L::STAGE;
         uint64_t* bar = &S_.full[s];
-        mbar_arrive_expect_tx(bar, 2 * NP * PANEL + (BWD ? 2 : 1) * TILE + MATS + AX_N * 4);
+        if (SUM) mbar_arrive_expect_tx(bar, NP * PANEL + (map ? 0 : TILE) + MATS / 2 + AX_N * 4);
+        else mbar_arrive_expect_tx(bar, 2 * NP * PANEL + (BWD ? 2 : 1) * TILE + MATS + AX_N * 4);
         const int row = (int)(sq.bos + (int64_t)c * C);
         const int64_t sh = sh0 + (int64_t)c * a.HV;
         for (int i = 0; i < NP; ++i) tma_load_3d(p + L::KQ + 2 * i * PANEL, &tmk, bar, 64 * i, h, row);
-        tma_load_3d(p + L::V, &tmv, bar, v0, hv, row);
-        tma_load_3d(p + L::V + PANEL, &tmv, bar, v0 + 64, hv, row);
+        if (!map) {
+          tma_load_3d(p + L::V, &tmv, bar, v0, hv, row);
+          tma_load_3d(p + L::V + PANEL, &tmv, bar, v0 + 64, hv, row);
+        }
         bulk_load(p + L::AX, w.aux + sh * AX_N, AX_N * 4, bar);
-        bulk_load(p + L::M, w.mats + sh * MATS, MATS, bar);
-        for (int i = 0; i < NP; ++i) tma_load_3d(p + L::KQ + (2 * i + 1) * PANEL, &tmq, bar, 64 * i, h, row);
+        bulk_load(p + L::M, w.mats + sh * MATS, SUM ? MATS / 2 : MATS, bar);
+        for (int i = 0; i < NP && !SUM; ++i) tma_load_3d(p + L::KQ + (2 * i + 1) * PANEL, &tmq, bar, 64 * i, h, row);
         if (BWD) {
           tma_load_3d(p + L::DO, &tmo, bar, v0, hv, row);
           tma_load_3d(p + L::DO + PANEL, &tmo, bar, v0 + 64, hv, row);
@@ -141,7 +154,7 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
         const uint32_t T = p + L::M, P = T + 2 * PANEL;
         // X^T | Y^T
         if (!spin_wait(&S_.full[s], (c >> 1) & 1, ab, err, 4)) break;
-        if ((c + 1) * C > sq.len && !spin_wait(&S_.kz, 0, ab, err, 8)) break;
+        if (!SUM && (c + 1) * C > sq.len && !spin_wait(&S_.kz, 0, ab, err, 8)) break;
         if (!spin_wait(&S_.s_ready, ph, ab, err, 0x10)) break;
         tc_fence_after();
 #pragma unroll
@@ -149,23 +162,23 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
 #pragma unroll
           for (int ks = 0; ks < KD / 16; ++ks)
             umma_ts(tb + T_X, tb + (x ? T_SL : T_SH) + 8 * ks,
-                    sdesc(p + L::KQ + (ks >> 2) * 2 * PANEL + (ks & 3) * 32, 16, 1024), id128, x + ks > 0);
+                    sdesc(p + L::KQ + (ks >> 2) * 2 * PANEL + (ks & 3) * 32, 16, 1024), SUM ? id64 : id128, x + ks > 0);
         umma_commit(&S_.x_full);
         // E^T = V^T T^T, then + (-Gam X)^T T^T; the hi and lo halves are added on reading
-        if (c > 0 && !spin_wait(&S_.o2_free, (c - 1) & 1, ab, err, 0x20)) break;
+        if (!SUM && c > 0 && !spin_wait(&S_.o2_free, (c - 1) & 1, ab, err, 0x20)) break;
         tc_fence_after();
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
+        for (int ks = 0; ks < 4 && !map; ++ks)
           umma(tb + T_D, sdesc(p + L::V + ks * 2048, PANEL, 1024), sdesc(T + ks * 32, 16, 1024), id_v, ks > 0);
         if (!spin_wait(&S_.r_ready, ph, ab, err, 0x40)) break;
         tc_fence_after();
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RH + 8 * ks, sdesc(T + ks * 32, 16, 1024), id128, 1);
+        for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RH + 8 * ks, sdesc(T + ks * 32, 16, 1024), id128, !map || ks > 0);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RL + 8 * ks, sdesc(T + ks * 32, 16, 1024), id64, 1);
         umma_commit(&S_.u_full);
         // dS^T = (w beta E)^T K over X | Y, then E^T (P beta)^T over E
-        if (!spin_wait(&S_.o1_read, ph, ab, err, 0x200)) break;
+        if (!SUM && !spin_wait(&S_.o1_read, ph, ab, err, 0x200)) break;
         if (!spin_wait(&S_.u_ready, ph, ab, err, 0x80)) break;
         tc_fence_after();
 #pragma unroll
@@ -174,11 +187,13 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
           for (int ks = 0; ks < 4; ++ks)
             umma_ts(tb + T_X, tb + (x ? T_WL : T_WH) + 8 * ks, sdesc(p + L::KQ + ks * 2048, 2 * PANEL, 1024), id_d, x + ks > 0);
         umma_commit(&S_.d_full);
+        if (!SUM) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RH + 8 * ks, sdesc(P + ks * 32, 16, 1024), id128, ks > 0);
+          for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RH + 8 * ks, sdesc(P + ks * 32, 16, 1024), id128, ks > 0);
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RL + 8 * ks, sdesc(P + ks * 32, 16, 1024), id64, 1);
-        umma_commit(&S_.o_full);
+          for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RL + 8 * ks, sdesc(P + ks * 32, 16, 1024), id64, 1);
+          umma_commit(&S_.o_full);
+        }
         umma_commit(&S_.empty[s]);
       }
       umma_commit(&S_.done);  // TMEM is freed only after every issued MMA has completed
@@ -193,13 +208,13 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
     constexpr int NY = G::CT >= 32 ? 16 : 8;  // columns per load where registers are short
     const int quad = warp & 3, hh = (warp - G::CHAIN) >> 2;
     const int vl = quad * 32 + lane;
-    const bool vin = v0 + vl < a.V;
+    const bool vin = v0 + vl < width;
     const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
     float S[KH];
 #pragma unroll
     for (int i = 0; i < KH; ++i) {
       const int k = KH * hh + i;
-      S[i] = (a.initial_state && vin && k < a.K) ? a.initial_state[st + (int64_t)k * a.V + v0 + vl] : 0.f;
+      S[i] = (first && vin && k < a.K) ? first[(int64_t)k * a.V + v0 + vl] : map && k == vl && vin ? 1.f : 0.f;
     }
     // S as the operand of the next chunk; for the backward its hi part also goes to `tile` (two panels of
     // 128 rows), or straight to the workspace for the first chunk
@@ -322,22 +337,22 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
         }
         bar_sync<2, G::CHAIN_THREADS>();
       }
-      if (BWD && vin && ((c + 1) % ANCHOR == 0 || c + 1 == nch)) {
-        float* g = w.Sf + ((gdr_slot0(a, n, sq, C * ANCHOR) + c / ANCHOR) * a.HV + hv) * a.K * a.V + v0 + vl;
+      if (const int cd = part.c0 + c; BWD && vin && ((cd + 1) % ANCHOR == 0 || cd + 1 == part.nch)) {
+        float* g = w.Sf + ((gdr_slot0(a, n, part.doc, C * ANCHOR) + cd / ANCHOR) * a.HV + hv) * a.K * a.V + v0 + vl;
 #pragma unroll
         for (int i = 0; i < KH; ++i)
           if (KH * hh + i < a.K) g[(int64_t)(KH * hh + i) * a.V] = S[i];
       }
     }
     if (BWD && threadIdx.x == 32 * G::CHAIN) bulk_wait_all();
-    if (!BWD && a.final_state && vin) {
+    if (!BWD && final && vin) {
 #pragma unroll
       for (int i = 0; i < KH; ++i) {
         const int k = KH * hh + i;
-        if (k < a.K) a.final_state[st + (int64_t)k * a.V + v0 + vl] = S[i];
+        if (k < a.K) final[(int64_t)k * width + v0 + vl] = S[i];
       }
     }
-  } else {
+  } else if (!SUM) {
     // ------------------------------------------------------------------ output
     G::out_regs();
     const int quad = warp & 3, j0 = OT * (warp >> 2);  // tokens j0 .. j0 + OT - 1
@@ -432,36 +447,40 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
   if (warp == G::MMA) tmem_dealloc(tb, 512);
 }
 
-template <int AB16, int KD, bool BWD>
+template <int AB16, int KD, bool BWD, bool SUM>
 cudaError_t launch(const GdrArgs& a, const Ws& w) {
   CUtensorMap q, k, v, o, st, e16;
   cudaError_t e = token_map(&q, a, a.q, a.H, a.K);
   if (e == cudaSuccess) e = token_map(&k, a, a.k, a.H, a.K);
   if (e == cudaSuccess) e = token_map(&v, a, a.v, a.HV, a.V);
-  if (e == cudaSuccess) e = token_map(&o, a, BWD ? a.d_o : a.o, a.HV, a.V);
+  if (e == cudaSuccess) e = token_map(&o, a, BWD ? a.d_o : SUM ? a.v : a.o, a.HV, a.V);
   st = e16 = o;  // unused by the forward
   const int64_t sh = gdr_slots(a, C) * a.HV;
   if (BWD && e == cudaSuccess) e = matrix_map(&st, a, w.S0, a.K, sh);
   if (BWD && e == cudaSuccess) e = matrix_map(&e16, a, w.E, 2 * C, sh);
   constexpr uint32_t bytes = Lay<BWD>::BYTES;
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(scan_kernel<AB16, KD, BWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    e = cudaFuncSetAttribute(scan_kernel<AB16, KD, BWD, SUM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e != cudaSuccess) return e;
-  scan_kernel<AB16, KD, BWD><<<a.n_seqs * a.HV * ((a.V + VT - 1) / VT), Warps<BWD>::THREADS, bytes, a.stream>>>(q, k, v, o, st, e16, a, w);
+  const int tiles = (a.V + VT - 1) / VT + (SUM ? 1 : 0), segs = SUM ? w.nseg - 1 : w.nseg;
+  scan_kernel<AB16, KD, BWD, SUM>
+      <<<(unsigned)((int64_t)a.n_seqs * a.HV * segs * tiles), Warps<BWD>::THREADS, bytes, a.stream>>>(q, k, v, o, st, e16, a, w);
   return cudaGetLastError();
 }
 
-template <int AB16>
-cudaError_t pick(const GdrArgs& a, const Ws& w, bool bwd) {
-  if (a.K <= 64) return bwd ? launch<AB16, 64, true>(a, w) : launch<AB16, 64, false>(a, w);
-  return bwd ? launch<AB16, 128, true>(a, w) : launch<AB16, 128, false>(a, w);
+template <int AB16, int KD>
+cudaError_t pick(const GdrArgs& a, const Ws& w, ScanMode mode) {
+  if (mode == SCAN_BWD) return launch<AB16, KD, true, false>(a, w);
+  return mode == SCAN_SUM ? launch<AB16, KD, false, true>(a, w) : launch<AB16, KD, false, false>(a, w);
 }
 
 }  // namespace
 
-cudaError_t scan(const GdrArgs& a, const Ws& w, bool bwd, int* launches) {
+cudaError_t scan(const GdrArgs& a, const Ws& w, ScanMode mode, int* launches) {
   ++*launches;
-  return a.dtype == DT_BF16 ? pick<1>(a, w, bwd) : pick<0>(a, w, bwd);
+  const bool small = a.K <= 64;
+  if (a.dtype == DT_BF16) return small ? pick<1, 64>(a, w, mode) : pick<1, 128>(a, w, mode);
+  return small ? pick<0, 64>(a, w, mode) : pick<0, 128>(a, w, mode);
 }
 
 }  // namespace gdrtc

@@ -322,3 +322,28 @@ def test_refusals():
     big = inputs(1, 4, 1, 1, 257, 16, torch.float32)[0]
     with pytest.raises(ccq_b200.CCQError, match='K=257'):
         ccq_b200.gated_delta_rule(*(big[n] for n in NAMES))
+
+
+# ------------------------------------------------------------------------------------------------
+# few heads, a long axis: documents in segments that run side by side
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+@pytest.mark.parametrize('B,T,H,HV,K,V,lens', [
+    (1, 1601, 1, 1, 128, 128, None),
+    (2, 1100, 1, 2, 128, 256, None),
+    (1, 2048, 2, 2, 64, 72, None),
+    (1, 1500, 1, 2, 96, 128, [700, 0, 733, 64, 3]),
+    (1, 1700, 1, 1, 128, 128, [5, 1695]),
+])
+@pytest.mark.parametrize('states', [True, False])
+def test_segments(B, T, H, HV, K, V, lens, states, dtype):
+    check(B, T, H, HV, K, V, DT[dtype], lens=lens, states=states)
+
+
+def test_segments_with_gates_at_their_ends():
+    def edit(x):
+        x['beta'][:, ::3] = 0.0
+        x['g'][:, 700] = float('-inf')
+        x['g'][:, 511:513] = float('-inf')
+        x['g'][:, 800:1400] = 0.0
+    check(1, 1600, 1, 1, 128, 128, torch.bfloat16, edit=edit)
