@@ -12,9 +12,8 @@
 // of chunks (measured 4e-6 against 64 bits), as they would not with one rounding each (2.4e-3).  The
 // products cost two or three MMAs instead of one; the scans are bound by the latency of one chunk's
 // chain of three products, not by the MMA rate.  The gradient kernel, whose outputs are
-// rounded to 16 bits next and feed no recurrence, uses single 16-bit operands but for E, which enters
-// every one of its products but two: its rounding alone left 1.6e-3 in dq, dk and dbeta, as much as the
-// outputs' own.
+// rounded to 16 bits next and feed no recurrence, uses single 16-bit operands but for E where it makes W
+// and for W: each of these roundings alone left 1.6e-3 in dq and dk, as much as the outputs' own.
 #pragma once
 
 #include "gdr.h"

@@ -15,8 +15,8 @@
 //   F  = [-Gam X + w beta X2 ; scale Gam X] + [N ; W] K + [N^T ; 0] K + [W^T ; 0] Q
 //
 // X, X2, P and B are read by the epilogue warps, which put the first term of F back into TMEM and [N ; W]
-// into shared memory; the transposed products read the same bytes MN-major, with a panel of zeros for
-// the other half.  60 MMAs an item at V = 128.  Operands are single 16-bit values but for E (see
+// into shared memory; the transposed products read the same bytes MN-major, with the other half's lanes
+// masked.  60 MMAs an item at V = 128.  Operands are single 16-bit values but for W, and E in P (see
 // gdr_tc.cuh).  An item moves 192 KB; the kernel is bound by that and by the serial epilogue between
 // its two groups of products, of which the next item's loads and the last item's stores run beside.
 //
@@ -35,10 +35,9 @@ constexpr uint32_t T_X = 0, T_X2 = 128, T_P = 256, T_B = 320, T_F = 384;
 constexpr uint32_t B_DV = 0, B_DO = PANEL, B_E = 2 * PANEL, B_S = 4 * PANEL, B_DS = 6 * PANEL, B_SIZE = 8 * PANEL;
 constexpr uint32_t L_KQ = 0;                       // two buffers: K over Q in panels of 128 rows
 constexpr uint32_t L_B = 8 * PANEL;                // two steps
-constexpr uint32_t L_W = L_B + 2 * B_SIZE;         // N over W, then zeros
-constexpr uint32_t L_Z = L_W + 2 * PANEL;
+constexpr uint32_t L_W = L_B + 2 * B_SIZE;         // N, W and what W's rounding leaves
 constexpr uint32_t AX_BYTES = (AX_N * 4 + 127) & ~127u;
-constexpr uint32_t L_AX = L_Z + PANEL;             // four
+constexpr uint32_t L_AX = L_W + 3 * PANEL;            // four
 constexpr int RING = 4;
 
 // One value head of an item, written by the TMA thread.  Four in a ring: the loads run at most two steps ahead
@@ -50,7 +49,7 @@ struct Rec {
 struct Small {
   uint64_t full[2], empty[2], qk_empty[2];
   uint64_t rec_full[RING];  // the record and its per-token factors
-  uint64_t x_full, wn_ready, f_full, kz, done;
+  uint64_t p_full, x_full, wn_ready, f_full, kz, done;
   Rec rec[RING];
   float ke[2][C], db[4][C], dg[17];
   uint32_t tmem;
@@ -81,6 +80,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&S_.qk_empty[i], 1);
     }
     for (int i = 0; i < RING; ++i) mbar_init(&S_.rec_full[i], 1);
+    mbar_init(&S_.p_full, 1);
     mbar_init(&S_.x_full, 1);
     mbar_init(&S_.wn_ready, EPI / 32);
     mbar_init(&S_.f_full, 1);
@@ -89,8 +89,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     S_.abort = 0;
     fence_barrier_init();
   }
-  if (tid < EPI) sts128(sb + L_Z + tid * 16, make_uint4(0, 0, 0, 0));
-  fence_async_smem();
   if (warp == 17) tmem_alloc(&S_.tmem, 512);
   tc_fence_before();
   __syncthreads();
@@ -206,15 +204,13 @@ __global__ void __launch_bounds__(THREADS, 1)
               umma(tb + T_B, d, d, id_b, ks > 0);
             }
           }
+          if (vt == nvt - 1) umma_commit(&S_.p_full);  // epilogue A starts on these, beside the products below
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
             umma(tb + T_X, sdesc(p + B_DV + ks * 32, 16, 1024), sdesc(p + B_S + ks * 2048, PANEL, 1024), id_x, vt + ks > 0);
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              umma(tb + T_X2, sdesc(p + B_E + x * PANEL + ks * 2048, PANEL, 1024), sdesc(p + B_DS + ks * 2048, PANEL, 1024),
-                   id_x2, vt + x + ks > 0);
+          for (int ks = 0; ks < 4; ++ks)
+            umma(tb + T_X2, sdesc(p + B_E + ks * 2048, PANEL, 1024), sdesc(p + B_DS + ks * 2048, PANEL, 1024), id_x2, vt + ks > 0);
           umma_commit(&S_.empty[b]);
         }
         if (!ok) break;
@@ -226,10 +222,16 @@ __global__ void __launch_bounds__(THREADS, 1)
           umma(tb + T_F, sdesc(W + ks * 32, 16, 1024), sdesc(KQ + ks * 2048, 2 * PANEL, 1024), id_x, 1);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
-          umma(tb + T_F, sdesc(W + ks * 2048, 2 * PANEL, 1024), sdesc(KQ + ks * 2048, 2 * PANEL, 1024), id_x2, 1);
+          umma_masked(tb + T_F, sdesc(W + PANEL + ks * 32, 16, 1024), sdesc(KQ + ks * 2048, 2 * PANEL, 1024), id_x, 1, ~0u, 0);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
-          umma(tb + T_F, sdesc(W + PANEL + ks * 2048, PANEL, 1024), sdesc(KQ + PANEL + ks * 2048, 2 * PANEL, 1024), id_x2, 1);
+          umma_masked(tb + T_F, sdesc(W + ks * 2048, PANEL, 1024), sdesc(KQ + ks * 2048, 2 * PANEL, 1024), id_x2, 1, 0, ~0u);
+#pragma unroll
+        for (int x = 1; x < 3; ++x)
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma_masked(tb + T_F, sdesc(W + x * PANEL + ks * 2048, 0, 1024), sdesc(KQ + PANEL + ks * 2048, 2 * PANEL, 1024), id_x2, 1, 0,
+                        ~0u);
         umma_commit(&S_.f_full);
       }
       umma_commit(&S_.done);  // TMEM is freed only after every issued MMA has completed
@@ -241,6 +243,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const bool kside = quad < 2;          // rows 0-63: what leads to dK
     const int i = (quad & 1) * 32 + lane; // token
     const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
+    int stored = -1;
     int first_step = 0;                   // step of this record's first loads
     for (int rec = 0;; ++rec, first_step += nvt) {
       const int r = rec % RING;
@@ -248,23 +251,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       // one decision for all warps, so that a wait that gave up cannot leave some of them at a barrier
       if (tid == 0) S_.go = pipe_wait(&S_.rec_full[r], (rec / RING) & 1, ab, err, 0x80) && R.live;
       bar_sync<1, EPI>();
+      if (tid == 256 && stored >= 0) {  // the last item's output has left its buffer
+        bulk_wait_read();
+        mbar_arrive(&S_.qk_empty[stored]);
+      }
+      stored = -1;
       if (!S_.go) break;
       const int valid = R.valid;
       const uint32_t KQ = sb + L_KQ + R.qk * 4 * PANEL;
       const float* ax = reinterpret_cast<const float*>(sm + L_AX + r * AX_BYTES);
-      // dO . O - V . dV: of this chunk's tokens in warps 0 and 1, of the chunks up to the next anchor in the
-      // others; and <dS, S> there
-      float dot = 0.f, later = 0.f;
-      {
-        const int64_t vs = gdr_slots(a, C) * a.HV, va = gdr_slots(a, C * ANCHOR) * a.HV;
-        for (int v = 0; v < (a.V + VT - 1) / VT; ++v) {
-          if ((tid >> 6) <= R.more) {
-            const int64_t at = (v * vs + R.sh + (int64_t)(tid >> 6) * a.HV) * C + (tid & 63);
-            dot += w.dotO[at] - w.dotV[at];
-          }
-          if (tid < ANCHOR_PARTS) later += w.anchor[(v * va + R.anchor) * ANCHOR_PARTS + tid];
-        }
-      }
       if (valid < C && R.first) {
         pipe_wait(&S_.full[first_step & 1], (first_step >> 1) & 1, ab, err, 0x100);
         // the rows past the document belong to another one: what a product sums over must be zero
@@ -272,63 +267,65 @@ __global__ void __launch_bounds__(THREADS, 1)
         fence_async_smem();
         warp_arrive(&S_.kz);
       }
-      pipe_wait(&S_.x_full, rec & 1, ab, err, 0x200);
+      pipe_wait(warp < 8 ? &S_.p_full : &S_.x_full, rec & 1, ab, err, 0x200);
       tc_fence_after();
+      float z[32];
       if (warp < 8) {
         // [N ; W] and the scores' part of dbeta, columns c0 .. c0 + 31
         const int c0 = 32 * (warp >> 2);
-        float z[32];
         const uint32_t row = sb + L_W + (kside ? 0 : PANEL);
         if (c0 > (quad & 1) * 32) {  // the block above the diagonal
 #pragma unroll
-          for (int cc = 0; cc < 4; ++cc) sts128(row + sw128(i, c0 / 8 + cc), make_uint4(0, 0, 0, 0));
-          S_.db[quad][c0 + lane] = 0.f;
+          for (int cc = 0; cc < 4; ++cc) {
+            sts128(row + sw128(i, c0 / 8 + cc), make_uint4(0, 0, 0, 0));
+            if (!kside) sts128(row + PANEL + sw128(i, c0 / 8 + cc), make_uint4(0, 0, 0, 0));
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) z[e] = 0.f;
         } else {
-          const float gh = ax[AX_GH + i], gl = ax[AX_GL + i];
-          const float sx = kside ? -1.f : a.scale;
+          const float gh[2] = {ax[AX_GH + i], ax[AX_GH + i]}, gl[2] = {ax[AX_GL + i], ax[AX_GL + i]};
+          const float sx[2] = {kside ? -1.f : a.scale, kside ? -1.f : a.scale}, m1[2] = {-1.f, -1.f};
           const int top = i < valid ? (kside ? i - 1 : i) : -1;  // last column of this row
 #pragma unroll
           for (int cc = 0; cc < 4; ++cc) {
             float x[8], y[8];
-            tmem_ld8(tl + T_P + c0 + 8 * cc, x);
-            tmem_ld8(tl + T_B + c0 + 8 * cc, y);
-            uint32_t u[4];
+            tmem_ld8x2(tl + T_P + c0 + 8 * cc, tl + T_B + c0 + 8 * cc, x, y);
 #pragma unroll
-            for (int e = 0; e < 8; e += 4) {
+            for (int e = 0; e < 8; e += 2) {
               const int j = c0 + 8 * cc + e;
-              const float4 hj = *reinterpret_cast<const float4*>(ax + AX_GH + j), lj = *reinterpret_cast<const float4*>(ax + AX_GL + j);
-              const float4 bj = *reinterpret_cast<const float4*>(ax + AX_B + j);
-              const float h4[4] = {hj.x, hj.y, hj.z, hj.w}, l4[4] = {lj.x, lj.y, lj.z, lj.w}, b4[4] = {bj.x, bj.y, bj.z, bj.w};
-#pragma unroll
-              for (int f = 0; f < 4; ++f) {
-                const float d = j + f <= top ? sx * ex2((gh - h4[f]) + (gl - l4[f])) * x[e + f] : 0.f;
-                z[8 * cc + e + f] = d * y[e + f];
-                x[e + f] = d * b4[f];
-              }
+              float d[2], l[2];
+              fma2(d, ax + AX_GH + j, m1, gh);
+              fma2(l, ax + AX_GL + j, m1, gl);
+              add2f(d, d, l);
+              d[0] = ex2(d[0]);
+              d[1] = ex2(d[1]);
+              mul2f(x + e, x + e, sx);
+              mul2f(d, d, x + e);
+              d[0] = j <= top ? d[0] : 0.f;  // the masked places can hold anything
+              d[1] = j < top ? d[1] : 0.f;
+              mul2f(z + 8 * cc + e, d, y + e);
+              mul2f(x + e, d, ax + AX_B + j);
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) u[e] = pack2<AB16>(x[2 * e], x[2 * e + 1]);
+            uint32_t u[4], lo[4];
+            split<AB16, 4>(x, u, lo);
             sts128(row + sw128(i, c0 / 8 + cc), make_uint4(u[0], u[1], u[2], u[3]));
+            if (!kside) sts128(row + PANEL + sw128(i, c0 / 8 + cc), make_uint4(lo[0], lo[1], lo[2], lo[3]));
           }
-          lane_sums<32>(z, lane);
-          S_.db[quad][c0 + lane] = z[0];
         }
       } else {
         // the first term of F, half of its columns, and k_i . X2_i
         constexpr int KH = KD / 2;
         const int hf = (warp - 8) >> 2;
-        const float g0 = kside ? -ax[AX_G + i] : ax[AX_SG + i], g1 = ax[AX_WB + i];
-        float ke = 0.f;
+        const float r0 = kside ? -ax[AX_G + i] : ax[AX_SG + i], r1 = ax[AX_WB + i];
+        const float g0[2] = {r0, r0}, g1[2] = {r1, r1};
+        float ke[2] = {0.f, 0.f};
 #pragma unroll
         for (int k0 = 0; k0 < KH; k0 += 16) {
           const int k = KH * hf + k0;
           float x[16];
-          tmem_ld16(tl + T_X + k, x);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] *= g0;
           if (kside) {
             float y[16];
-            tmem_ld16(tl + T_X2 + k, y);
+            tmem_ld16x2(tl + T_X + k, tl + T_X2 + k, x, y);
             const uint32_t p = KQ + (k >> 6) * 2 * PANEL;
 #pragma unroll
             for (int cc = 0; cc < 2; ++cc) {
@@ -337,11 +334,18 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float2 f = unpack2<AB16>(u[e]);
-                ke = fmaf(f.x, y[8 * cc + 2 * e], fmaf(f.y, y[8 * cc + 2 * e + 1], ke));
+                const float f2[2] = {f.x, f.y};
+                fma2(ke, f2, y + 8 * cc + 2 * e, ke);
               }
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = fmaf(g1, y[e], x[e]);
+            for (int e = 0; e < 16; e += 2) mul2f(y + e, y + e, g1);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) fma2(x + e, x + e, g0, y + e);
+          } else {
+            tmem_ld16(tl + T_X + k, x);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) mul2f(x + e, x + e, g0);
           }
           if (!R.first) {
             float y[16];
@@ -355,16 +359,72 @@ __global__ void __launch_bounds__(THREADS, 1)
           tmem_st8(tl + T_F + k, u);
           tmem_st8(tl + T_F + k + 8, u + 8);
         }
-        if (kside) S_.ke[hf][i] = ke;
+        if (kside) S_.ke[hf][i] = ke[0] + ke[1];
         tmem_st_wait();
+      }
+      fence_async_smem();
+      tc_fence_before();
+      warp_arrive(&S_.wn_ready);
+      // dO . O - V . dV: of this chunk's tokens in warps 0 and 1, of the chunks up to the next anchor in the
+      // others; and <dS, S> there.  Asked for here, used after the output.
+      const int64_t vs = gdr_slots(a, C) * a.HV, va = gdr_slots(a, C * ANCHOR) * a.HV;
+      const int64_t at_dot = (R.sh + (int64_t)(tid >> 6) * a.HV) * C + (tid & 63), at_later = R.anchor * ANCHOR_PARTS + tid;
+      const bool has_dot = (tid >> 6) <= R.more, has_later = tid < ANCHOR_PARTS;
+      float dot = has_dot ? w.dotO[at_dot] : 0.f, dotV = has_dot ? w.dotV[at_dot] : 0.f, later = has_later ? w.anchor[at_later] : 0.f;
+      if (warp < 8) {
+        lane_sums<32>(z, lane);
+        S_.db[quad][32 * (warp >> 2) + lane] = z[0];
+      }
+      pipe_wait(&S_.f_full, rec & 1, ab, err, 0x400);
+      tc_fence_after();
+      if (R.last) {
+        // dK over the K rows and dQ over the Q rows, then out
+        constexpr int KQTR = KD / 4;
+        const int k0 = KQTR * (warp >> 2);
+#pragma unroll
+        for (int k = k0; k < k0 + KQTR; k += 16) {
+          float x[16];
+          tmem_ld16(tl + T_F + k, x);
+          uint32_t u[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) u[e] = pack2<AB16>(x[2 * e], x[2 * e + 1]);
+          const uint32_t p = KQ + (k >> 6) * 2 * PANEL;
+          sts128(p + sw128(quad * 32 + lane, (k & 63) >> 3), make_uint4(u[0], u[1], u[2], u[3]));
+          sts128(p + sw128(quad * 32 + lane, ((k & 63) >> 3) + 1), make_uint4(u[4], u[5], u[6], u[7]));
+        }
+        fence_async_smem();
+        bar_sync<1, EPI>();
+        if (valid == C) {
+          if (tid == 256) {
+            for (int p = 0; p < NP; ++p)
+              if (64 * p < a.K) {
+                tma_store_3d(&tmdk, sm + (KQ - sb) + 2 * p * PANEL, 64 * p, R.h, R.row0);
+                tma_store_3d(&tmdq, sm + (KQ - sb) + (2 * p + 1) * PANEL, 64 * p, R.h, R.row0);
+              }
+            bulk_commit();
+          }
+          stored = R.qk;
+        } else {
+          for (int e = tid; e < valid * 2 * NP * 8; e += EPI) {
+            const int t = e / (2 * NP * 8), x = e % (2 * NP * 8), which = x & 1, ch = x >> 1;
+            if (ch * 8 < a.K)
+              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(which ? a.dq : a.dk) +
+                                        ((int64_t)(R.row0 + t) * a.H + R.h) * a.K + ch * 8) =
+                  lds128(KQ + ((ch >> 3) * 2 + which) * PANEL + sw128(t, ch & 7));
+          }
+          bar_sync<1, EPI>();
+          if (tid == 0) mbar_arrive(&S_.qk_empty[R.qk]);
+        }
+      }
+      dot -= dotV;
+      for (int v = 1; v < (a.V + VT - 1) / VT; ++v) {
+        if (has_dot) dot += w.dotO[v * vs * C + at_dot] - w.dotV[v * vs * C + at_dot];
+        if (has_later) later += w.anchor[v * va * ANCHOR_PARTS + at_later];
       }
       {
         const float x = warp_sum(warp < 2 ? later : dot + later);
         if (lane == 0) S_.dg[warp] = x;
       }
-      fence_async_smem();
-      tc_fence_before();
-      warp_arrive(&S_.wn_ready);
       bar_sync<1, EPI>();
       if (warp < 2) {
         const int j = tid;
@@ -389,51 +449,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (j == 0 && R.zero_first) x = 0.f;
         if (j < valid) gate_store(a.dg, a.g_dtype, at, x);
       }
-      pipe_wait(&S_.f_full, rec & 1, ab, err, 0x400);
-      tc_fence_after();
-      if (!R.last) bar_sync<1, EPI>();  // the sums are read before the next value head's are written
-      if (R.last) {
-        // dK over the K rows and dQ over the Q rows, then out
-        constexpr int KQTR = KD / 4;
-        const int k0 = KQTR * (warp >> 2);
-#pragma unroll
-        for (int k = k0; k < k0 + KQTR; k += 16) {
-          float x[16];
-          tmem_ld16(tl + T_F + k, x);
-          uint32_t u[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) u[e] = pack2<AB16>(x[2 * e], x[2 * e + 1]);
-          const uint32_t p = KQ + (k >> 6) * 2 * PANEL;
-          sts128(p + sw128(quad * 32 + lane, (k & 63) >> 3), make_uint4(u[0], u[1], u[2], u[3]));
-          sts128(p + sw128(quad * 32 + lane, ((k & 63) >> 3) + 1), make_uint4(u[4], u[5], u[6], u[7]));
-        }
-        fence_async_smem();
-        bar_sync<1, EPI>();
-        if (valid == C) {
-          if (tid == 0) {
-            for (int p = 0; p < NP; ++p)
-              if (64 * p < a.K) {
-                tma_store_3d(&tmdk, sm + (KQ - sb) + 2 * p * PANEL, 64 * p, R.h, R.row0);
-                tma_store_3d(&tmdq, sm + (KQ - sb) + (2 * p + 1) * PANEL, 64 * p, R.h, R.row0);
-              }
-            bulk_commit();
-            bulk_wait_read();
-            mbar_arrive(&S_.qk_empty[R.qk]);
-          }
-        } else {
-          for (int e = tid; e < valid * 2 * NP * 8; e += EPI) {
-            const int t = e / (2 * NP * 8), x = e % (2 * NP * 8), which = x & 1, ch = x >> 1;
-            if (ch * 8 < a.K)
-              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(which ? a.dq : a.dk) +
-                                        ((int64_t)(R.row0 + t) * a.H + R.h) * a.K + ch * 8) =
-                  lds128(KQ + ((ch >> 3) * 2 + which) * PANEL + sw128(t, ch & 7));
-          }
-          bar_sync<1, EPI>();
-          if (tid == 0) mbar_arrive(&S_.qk_empty[R.qk]);
-        }
-      }
     }
-    if (tid == 0) bulk_wait_all();
+    if (tid == 256) bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
