@@ -33,8 +33,10 @@ struct Ws {
   int nvt;                // NVT
 };
 
-// Columns of V per block of the scans: 32, or 8 where that leaves SMs without a block.
-inline int tile(const GdrArgs& a) { return (int64_t)a.n_seqs * a.HV * ((a.V + 31) / 32) < 148 ? 8 : 32; }
+// Columns of V per block of the scans: 32, or 8 where that leaves half of the SMs without a block.  Forward and
+// backward of 1024 tokens in fp32, 64 blocks of 32: 0.67 ms in eights, 0.92 in 32s at K = V = 64, 0.92 and
+// 1.24 at 128, 1.98 and 2.04 at 256; 128 blocks of 32: 1.25 and 1.04, 1.72 and 1.40, 3.87 and 2.39.
+inline int tile(const GdrArgs& a) { return 2 * (int64_t)a.n_seqs * a.HV * ((a.V + 31) / 32) <= 148 ? 8 : 32; }
 inline int nvt(const GdrArgs& a) { return (a.V + tile(a) - 1) / tile(a); }
 
 size_t carve(const GdrArgs& a, bool bwd, Ws* w) {
@@ -88,7 +90,8 @@ __device__ __forceinline__ void fetch1(float* dst, const TI* src, bool in) {
   else
     *dst = in ? Act<TI>::load(src) : 0.f;
 }
-// the same rows as load_rows, asynchronously for fp32: a warp a row, W columns
+// rows [t0, t0 + C) of a [tokens, heads, W] tensor into dst[C][ld], n columns; zero outside the document and
+// past W.  A warp a row; for fp32 the copies are asynchronous.
 template <typename TI>
 __device__ __forceinline__ void fetch_rows(float* dst, int ld, int n, const TI* src, const Seq& sq, int t0, int heads, int head,
                                            int W) {
@@ -115,19 +118,6 @@ __device__ __forceinline__ void fetch_mat(float* dst, const float* src) {
 }
 static_assert(C * C == THREADS * 4, "a matrix is one 16-byte copy a thread");
 
-// rows [t0, t0 + C) of a [tokens, heads, W] tensor into dst[C][ld], columns [c0, c0 + n); zero
-// outside the document and past W
-template <typename TI>
-__device__ __forceinline__ void load_rows(float* dst, int ld, int n, const TI* src, const Seq& sq, int t0, int heads,
-                                          int head, int W, int c0) {
-  for (int i = threadIdx.x; i < C * n; i += blockDim.x) {
-    const int r = i / n, c = i - r * n;
-    float x = 0.f;
-    if (t0 + r < sq.len && c0 + c < W) x = Act<TI>::load(src + ((sq.bos + t0 + r) * heads + head) * W + c0 + c);
-    dst[r * ld + c] = x;
-  }
-}
-
 // ------------------------------------------------------------------------------------------------
 template <typename TI>
 __global__ void __launch_bounds__(THREADS) prep_kernel(GdrArgs a, Ws w) {
@@ -146,8 +136,8 @@ __global__ void __launch_bounds__(THREADS) prep_kernel(GdrArgs a, Ws w) {
   Seq sq;
   if (!gdr_slot_find(a, slot, C, &n, &c, &sq)) return;
   const int t0 = c * C;
-  load_rows(kt, ld, Kp, reinterpret_cast<const TI*>(a.k), sq, t0, a.H, h, a.K, 0);
-  load_rows(qt, ld, Kp, reinterpret_cast<const TI*>(a.q), sq, t0, a.H, h, a.K, 0);
+  fetch_rows(kt, ld, Kp, reinterpret_cast<const TI*>(a.k), sq, t0, a.H, h, a.K);
+  fetch_rows(qt, ld, Kp, reinterpret_cast<const TI*>(a.q), sq, t0, a.H, h, a.K);
   const int64_t sh = slot * a.HV + hv;
   if (threadIdx.x < 32) {
     const int t = t0 + threadIdx.x;
@@ -169,6 +159,7 @@ __global__ void __launch_bounds__(THREADS) prep_kernel(GdrArgs a, Ws w) {
     ax[C + threadIdx.x] = expf((float)s);
     ax[2 * C + threadIdx.x] = expf((float)(last - s));
   }
+  copies_wait();
   __syncthreads();
   const int64_t mat = sh * C * C;
   for (int e = threadIdx.x; e < C * C; e += THREADS) {
@@ -510,7 +501,7 @@ inline size_t grads_smem(int K) {
 }
 
 template <typename TI>
-__global__ void __launch_bounds__(THREADS) grads_kernel(GdrArgs a, Ws w) {
+__global__ void __launch_bounds__(THREADS, 2) grads_kernel(GdrArgs a, Ws w) {
   extern __shared__ float4 smem4[];
   float* sm = reinterpret_cast<float*>(smem4);
   const int Kp = (a.K + 3) & ~3, ld = Kp + 4;
@@ -532,10 +523,10 @@ __global__ void __launch_bounds__(THREADS) grads_kernel(GdrArgs a, Ws w) {
   Seq sq;
   if (!gdr_slot_find(a, slot, C, &n, &c, &sq)) return;
   const int t0 = c * C;
-  load_rows(kt, ld, Kp, reinterpret_cast<const TI*>(a.k), sq, t0, a.H, h, a.K, 0);
-  load_rows(qt, ld, Kp, reinterpret_cast<const TI*>(a.q), sq, t0, a.H, h, a.K, 0);
+  fetch_rows(kt, ld, Kp, reinterpret_cast<const TI*>(a.k), sq, t0, a.H, h, a.K);
+  fetch_rows(qt, ld, Kp, reinterpret_cast<const TI*>(a.q), sq, t0, a.H, h, a.K);
   const int kc = threadIdx.x & 63, ig = threadIdx.x >> 6;           // column of K, tokens 8 ig .. 8 ig + 7
-  const int pi = threadIdx.x >> 3, pj = (threadIdx.x & 7) * 4;      // row and 4 columns of the C x C products
+  const int pi = threadIdx.x >> 3, pj = threadIdx.x & 7;            // row and columns pj + 8 j of the C x C products
   for (int kb = 0; kb < a.K; kb += KB) {
     float aq[8] = {}, ak[8] = {};
     for (int hv = h * group; hv < (h + 1) * group; ++hv) {
@@ -543,24 +534,28 @@ __global__ void __launch_bounds__(THREADS) grads_kernel(GdrArgs a, Ws w) {
       float xq[8] = {}, xr[8] = {}, xu[8] = {}, dp[4] = {}, da[4] = {}, db = 0.f;
       for (int v0 = 0; v0 < a.V; v0 += VG) {
         __syncthreads();
-        for (int i = threadIdx.x; i < KB * VG; i += THREADS) {
-          const int r = i / VG, v = i % VG;
-          const bool in = kb + r < a.K && v0 + v < a.V;
-          const int64_t at = (sh * a.K + kb + r) * a.V + v0 + v;
-          S0[r * LV + v] = in ? w.S0[at] : 0.f;
-          dS[r * LV + v] = in ? w.dS1[at] : 0.f;
+        {
+          const int v = threadIdx.x % VG;
+          const bool vin = v0 + v < a.V;
+          const int64_t at = v0 + (vin ? v : 0);
+#pragma unroll
+          for (int r = threadIdx.x / VG; r < KB; r += THREADS / VG) {
+            const bool in = vin && kb + r < a.K;
+            const int64_t p = (sh * a.K + (in ? kb + r : 0)) * a.V + at;
+            copy4(S0 + r * LV + v, w.S0 + p, in);
+            copy4(dS + r * LV + v, w.dS1 + p, in);
+          }
+#pragma unroll
+          for (int r = threadIdx.x / VG; r < C; r += THREADS / VG) {
+            const int64_t p = (sh * C + r) * a.V + at;
+            copy4(Ut + r * LV + v, w.U + p, vin);
+            copy4(dR + r * LV + v, w.dR + p, vin);
+            copy4(Rt + r * LV + v, w.R + p, vin);
+            const bool in = vin && t0 + r < sq.len;
+            fetch1(dO + r * LV + v, reinterpret_cast<const TI*>(a.d_o) + (in ? ((sq.bos + t0 + r) * a.HV + hv) * a.V + at : 0), in);
+          }
         }
-        for (int i = threadIdx.x; i < C * VG; i += THREADS) {
-          const int r = i / VG, v = i % VG;
-          const bool in = v0 + v < a.V;
-          const int64_t at = (sh * C + r) * a.V + v0 + v;
-          Ut[r * LV + v] = in ? w.U[at] : 0.f;
-          dR[r * LV + v] = in ? w.dR[at] : 0.f;
-          Rt[r * LV + v] = in ? w.R[at] : 0.f;
-          dO[r * LV + v] = in && t0 + r < sq.len
-                               ? Act<TI>::load(reinterpret_cast<const TI*>(a.d_o) + ((sq.bos + t0 + r) * a.HV + hv) * a.V + v0 + v)
-                               : 0.f;
-        }
+        copies_wait();
         __syncthreads();
         for (int v = 0; v < VG; v += 4) {
           const float4 s = *reinterpret_cast<const float4*>(S0 + kc * LV + v);
@@ -576,23 +571,24 @@ __global__ void __launch_bounds__(THREADS) grads_kernel(GdrArgs a, Ws w) {
           const float4 rr = *reinterpret_cast<const float4*>(dR + pi * LV + v);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float4 u = *reinterpret_cast<const float4*>(Ut + (pj + j) * LV + v);
+            const float4 u = *reinterpret_cast<const float4*>(Ut + (pj + 8 * j) * LV + v);
             dp[j] = dot4(o, u, dp[j]);
             da[j] = dot4(rr, u, da[j]);
           }
-          if (v == pj) db = dot4(rr, *reinterpret_cast<const float4*>(Rt + pi * LV + v), db);
+          if (v == 4 * pj) db = dot4(rr, *reinterpret_cast<const float4*>(Rt + pi * LV + v), db);
         }
       }
       if (threadIdx.x < 3 * C) ax[threadIdx.x] = w.aux[sh * 3 * C + threadIdx.x];
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float d = w.D[sh * C * C + pi * C + pj + j];
+        const int cj = pj + 8 * j;
+        const float d = w.D[sh * C * C + pi * C + cj];
         const float wij = a.scale * d * dp[j], z = -ax[pi] * d * da[j];
-        W[pi * LT + pj + j] = Wt[(pj + j) * LT + pi] = wij;
-        if (pj + j < pi) N[pi * LT + pj + j] = N[(pj + j) * LT + pi] = z;
-        if (pj + j == pi) N[pi * LT + pi] = 0.f;
-        db = fmaf(-w.L[sh * C * C + pi * C + pj + j], da[j], db);
+        W[pi * LT + cj] = Wt[cj * LT + pi] = wij;
+        if (cj < pi) N[pi * LT + cj] = N[cj * LT + pi] = z;
+        if (cj == pi) N[pi * LT + pi] = 0.f;
+        db = fmaf(-w.L[sh * C * C + pi * C + cj], da[j], db);
       }
       if (kb == 0) {
         // dbeta: eight threads share a row
@@ -657,7 +653,8 @@ __global__ void __launch_bounds__(THREADS) grads_kernel(GdrArgs a, Ws w) {
 
 template <typename F>
 cudaError_t allow_smem(F f, size_t bytes) {
-  return bytes > 48 * 1024 ? cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : cudaSuccess;
+  // 48 KB without asking, the static arrays (up to 10 KB) counted in
+  return bytes > 38 * 1024 ? cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : cudaSuccess;
 }
 
 template <typename TI, int VT>

@@ -347,3 +347,23 @@ def test_segments_with_gates_at_their_ends():
         x['g'][:, 511:513] = float('-inf')
         x['g'][:, 800:1400] = 0.0
     check(1, 1600, 1, 1, 128, 128, torch.bfloat16, edit=edit)
+
+
+# ------------------------------------------------------------------------------------------------
+# the exact path: key sizes around its shared-memory steps, and many heads (wider tiles of V)
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('K', [132, 149, 160, 176, 185, 188, 189, 224])
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_key_sizes_past_128(K, dtype):
+    check(1, 70, 1, 1, K, 40, DT[dtype])
+
+
+@pytest.mark.parametrize('B,T,H,HV,K,V,lens', [
+    (3, 100, 26, 26, 64, 32, None),
+    (2, 65, 10, 20, 160, 72, None),
+    (1, 130, 8, 16, 33, 47, [1, 0, 64, 65]),
+    (1, 40, 40, 80, 256, 8, None),
+])
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+def test_exact_path_with_many_heads(B, T, H, HV, K, V, lens, dtype):
+    check(B, T, H, HV, K, V, DT[dtype], lens=lens, states=lens is None)
