@@ -5,6 +5,7 @@
 //   scan   (gdr_tc_scan.cu)   per (document, value head, 128 columns of V): the state, chunk by chunk
 //   rscan  (gdr_tc_rscan.cu)  the same in reverse for the state's gradient
 //   grads  (gdr_tc_grads.cu)  per (chunk, key head): dq, dk, dg, dbeta
+//   join   (gdr_tc_seg.cu)    long documents of few heads, walked in segments side by side
 //
 // Precision.  The tensor cores multiply 16-bit operands.  What enters as an operand of the two scans and is
 // not an input (S, E, T, P and their gradients' counterparts) is given as a sum of two 16-bit numbers,

@@ -14,7 +14,8 @@
 // full), and splitting K or V further would not shorten the chain.  An MMA with its A operand in TMEM
 // takes about 64 cycles for any N up to 128 here, so what can share an A operand is put side by side in N.
 // The rest of a chunk's period is instructions of the chain warps between the products, so V enters by an MMA
-// of its own (beside the chain) and the factors by packed two-value arithmetic.
+// of its own (beside the chain) and the factors by packed two-value arithmetic.  8 x 4096 tokens, 16 heads,
+// K = V = 128: 233 us, 3.6 us a chunk; 331 us with what the backward reads (BWD), 256 MB more written.
 //
 // BWD: instead of O it writes what the backward reads: S0 (16-bit, transposed), E (hi + lo), dO . O and,
 // every ANCHOR chunks, S in fp32.
