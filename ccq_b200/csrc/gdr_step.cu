@@ -18,12 +18,26 @@
 namespace ccq {
 namespace {
 
-__device__ __forceinline__ float4 scale4(const float4& x, float s) { return make_float4(x.x * s, x.y * s, x.z * s, x.w * s); }
+// four columns, two to an instruction
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ void scale4(float4& d, float s) {
+  uint64_t lo, hi;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(lo) : "l"(pair(d.x, d.y)), "l"(pair(s, s)));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(hi) : "l"(pair(d.z, d.w)), "l"(pair(s, s)));
+  unpair(lo, d.x, d.y);
+  unpair(hi, d.z, d.w);
+}
 __device__ __forceinline__ void fma4(float4& d, const float4& x, float s) {
-  d.x = fmaf(x.x, s, d.x);
-  d.y = fmaf(x.y, s, d.y);
-  d.z = fmaf(x.z, s, d.z);
-  d.w = fmaf(x.w, s, d.w);
+  uint64_t lo, hi;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(lo) : "l"(pair(x.x, x.y)), "l"(pair(s, s)), "l"(pair(d.x, d.y)));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(hi) : "l"(pair(x.z, x.w)), "l"(pair(s, s)), "l"(pair(d.z, d.w)));
+  unpair(lo, d.x, d.y);
+  unpair(hi, d.z, d.w);
 }
 __device__ __forceinline__ void add4(float4& d, const float4& x) {
   d.x += x.x;
@@ -109,10 +123,13 @@ __global__ void __launch_bounds__(WARPS * 32) step_kernel(GdrArgs a) {
     load_values<TI, ROWS, VEC4>(qp, row0, a.K, q);
     float4 sk = make_float4(0.f, 0.f, 0.f, 0.f), sqv = sk;
     float dot = 0.f;
+    if (decay == 0.f) {  // empties the state whatever it holds
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) S[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
-      // a zero decay empties the state whatever it holds
-      S[i] = decay == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : scale4(S[i], decay);
+      scale4(S[i], decay);
       fma4(sk, S[i], k[i]);
       fma4(sqv, S[i], q[i]);
       dot = fmaf(k[i], q[i], dot);
