@@ -7,10 +7,10 @@
 // decayed state, since the read after the update is
 //   S_new^T q = S^T q + (k . q) u,
 // so a token costs one reduction over the block.  A state row is read once and written once: with one
-// token the kernel is bound by HBM (8 K V bytes a head).  Small blocks with many rows a thread keep most
-// of an SM's registers in flight as loads while others compute and store (256 requests, 16 heads,
-// K = V = 128, 537 MB of state: 2 warps of 32 rows 102 us, 4 of 16 109 us, 8 of 8 111 us; 128 columns a
-// block instead of 64: 106 us).  With few heads the kernel is bound by latency, so the launcher narrows
+// token the kernel is bound by HBM (8 K V bytes a head), with more by instructions, which packed arithmetic
+// halves.  256 requests, 16 heads, K = V = 128, 537 MB of state: 4 warps of 16 rows a thread 88 us, 6.1 TB/s
+// (four tokens 124 us); 2 of 32 95 us (143), 8 of 8 90 us (174); 128 columns a block instead of 64: 90 us (141).
+// With few heads the kernel is bound by latency, so the launcher narrows
 // the block to 32 or 16 columns until the grid covers the SMs.  Each element is read and written by one
 // thread, so the state may be updated in place.
 #include "gdr.h"
@@ -195,9 +195,11 @@ void pick_rows(const GdrArgs& a) {
 
 template <typename TI>
 void pick_columns(const GdrArgs& a) {
-  // narrower blocks, with more warps to a column, only while the grid would leave SMs idle (148)
+  // narrower blocks only while the grid would leave SMs idle (148).  192 blocks of 64 columns (8 requests of 8
+  // tokens, K = V = 256): 15.8 us, in 32s 18.7; 32 blocks of 64 (4 requests of 16 tokens, K = V = 128): 15.6 us,
+  // in 16s 13.8.
   const int64_t heads = (int64_t)a.n_seqs * a.HV;
-  if (a.V > 32 && heads * ((a.V + 63) / 64) >= 2 * 148) pick_rows<TI, 16, 2, 2, 4>(a);
+  if (a.V > 32 && heads * ((a.V + 63) / 64) >= 148) pick_rows<TI, 16, 2, 4, 4>(a);
   else if (a.V > 16 && heads * ((a.V + 31) / 32) >= 148) pick_rows<TI, 8, 2, 4, 8>(a);
   else pick_rows<TI, 4, 2, 4, 8>(a);
 }
