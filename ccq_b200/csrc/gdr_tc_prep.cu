@@ -9,8 +9,9 @@
 // them: a block has 2 x 64 x 64 x 128 multiply-adds, too few to pay for a TMEM round trip.  The inverse is
 // formed in fp32 accuracy: the four 16 x 16 diagonal blocks by forward substitution, one warp each, then
 // T_21 = -T_22 A_21 T_11 for 16- and for 32-row blocks as three-term TF32 products (2^-21).  What bounds the
-// kernel is instruction issue, about 1900 instructions a warp: 8192 (chunk, head) pairs of K = 128 take 140 us,
-// where their 540 MB alone would take 83.
+// kernel is latency, six short stages with barriers between them: 1.65 instructions a cycle with the five blocks
+// that fit an SM.  8192 (chunk, head) pairs of K = 128 take 140 us, where their 540 MB alone would take 83.
+// (Bands of 16 rows that rotate over the warps, to even out the schedulers: no change.)
 #include "gdr_tc.cuh"
 
 namespace ccq {
