@@ -528,8 +528,12 @@ size_t ccq_gdr_workspace_size(int op, int dtype, int B, int T, int H, int HV, in
   alignas(16) static const int64_t given[2] = {0, 0};  // only whether a pointer is given counts
   a.cu_seqlens = (flags & CCQ_GDR_VARLEN) ? given : nullptr;
   a.fwd_workspace = (flags & CCQ_GDR_HAVE_FWD) ? given : nullptr;
-  if ((flags & CCQ_GDR_UNALIGNED) || !ccq::gdr_tc_supported(a)) return ccq::gdr_simt_workspace(a, op == CCQ_OP_BWD);
-  return ccq::gdr_tc_workspace(a, op == CCQ_OP_BWD);
+  const bool bwd = op == CCQ_OP_BWD;
+  const size_t exact = ccq::gdr_simt_workspace(a, bwd);
+  if (!ccq::gdr_tc_supported(a)) return exact;
+  const size_t tc = ccq::gdr_tc_workspace(a, bwd);
+  // an unaligned o alone leaves a call on the tensor-core path: room for either, and not the size of a call without the flag
+  return flags & CCQ_GDR_UNALIGNED ? (exact > tc ? exact : tc) + 256 : tc;
 }
 
 int ccq_gdr_fwd(int dtype, int B, int T, int H, int HV, int K, int V, const void* q, const void* k, const void* v,

@@ -80,15 +80,21 @@ cudaError_t start(const GdrArgs& a, const Ws& w, int* launches) {
 
 }  // namespace
 
+// The backward takes the forward's workspace without asking who wrote it, so what decides here has to be the same
+// in both calls: the environment is read once, and o, which the backward does not have, is left out (an o off
+// 16 bytes is stored without TMA).  The backward's own tensors only ever add reasons for the exact path, which
+// does not read the forward's workspace.
 bool gdr_tc_supported(const GdrArgs& a) {
-  const char* env = getenv("CCQ_B200_FORCE_SIMT");
-  if (env && env[0] == '1') return false;
+  static const bool forced = [] {
+    const char* env = getenv("CCQ_B200_FORCE_SIMT");
+    return env && env[0] == '1';
+  }();
+  if (forced) return false;
   if (a.dtype != DT_BF16 && a.dtype != DT_F16) return false;
   if (a.T < 1 || a.K > 128 || a.K % 8 != 0 || a.V % 8 != 0) return false;
   if (gdr_slots(a, C) * a.HV >= (1ll << 31)) return false;  // the kernels count (chunk, head) pairs in 32 bits
-  const uintptr_t p = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.o | (uintptr_t)a.d_o |
-                      (uintptr_t)a.dq | (uintptr_t)a.dk | (uintptr_t)a.dv | (uintptr_t)a.workspace |
-                      (uintptr_t)a.fwd_workspace;
+  const uintptr_t p = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.d_o | (uintptr_t)a.dq |
+                      (uintptr_t)a.dk | (uintptr_t)a.dv | (uintptr_t)a.workspace | (uintptr_t)a.fwd_workspace;
   return (p & 15) == 0;
 }
 

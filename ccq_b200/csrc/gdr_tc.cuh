@@ -236,6 +236,15 @@ __device__ __forceinline__ void copy_rows(uint32_t tile, uint16_t* dst, int64_t 
   }
 }
 
+// the same to a tensor off 16 bytes: whole elements
+__device__ __forceinline__ void copy_rows_unaligned(uint32_t tile, uint16_t* dst, int64_t row0, int HV, int hv, int V, int v0,
+                                                    int valid, int t, int count) {
+  for (int i = t; i < valid * VT; i += count) {
+    const int r = i / VT, c = i % VT;
+    if (v0 + c < V) dst[((row0 + r) * HV + hv) * V + v0 + c] = lds16(Column(tile, c).at(r));
+  }
+}
+
 // Warps of a scan: OW for the output (a share of the tokens of one TMEM quadrant each), CW for the chain (a share
 // of the tokens and of K each), then a warpgroup of which the first warp loads and the second issues MMAs.
 // RC, RO, RX: registers of a thread by role, redistributed from an even share.

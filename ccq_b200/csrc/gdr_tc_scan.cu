@@ -360,6 +360,7 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
     const int vl = quad * 32 + lane;
     const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
     const int64_t slots = gdr_slots(a, C);
+    const bool o16 = ((uintptr_t)a.o & 15) == 0;
     for (int c = 0; c < nch; ++c) {
       const int s = c & 1, ph = c & 1;
       const int valid = min(C, sq.len - c * C);
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
         const Column O(out, vl);
 #pragma unroll
         for (int i = 0; i < OT; ++i) sts16(O.at(j0 + i), f2h<AB16>(y[i]));
-        if (valid == C) {
+        if (valid == C && o16) {
           fence_async_smem();
           bar_sync<1, G::OUT_THREADS>();
           if (threadIdx.x == 0) {
@@ -421,7 +422,9 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
           }
         } else {
           bar_sync<1, G::OUT_THREADS>();
-          copy_rows(out, reinterpret_cast<uint16_t*>(a.o), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, G::OUT_THREADS);
+          uint16_t* o = reinterpret_cast<uint16_t*>(a.o);
+          if (o16) copy_rows(out, o, row0, a.HV, hv, a.V, v0, valid, threadIdx.x, G::OUT_THREADS);
+          else copy_rows_unaligned(out, o, row0, a.HV, hv, a.V, v0, valid, threadIdx.x, G::OUT_THREADS);
         }
       } else {
         const Column D(p + L::DO, vl);
@@ -454,7 +457,8 @@ cudaError_t launch(const GdrArgs& a, const Ws& w) {
   cudaError_t e = token_map(&q, a, a.q, a.H, a.K);
   if (e == cudaSuccess) e = token_map(&k, a, a.k, a.H, a.K);
   if (e == cudaSuccess) e = token_map(&v, a, a.v, a.HV, a.V);
-  if (e == cudaSuccess) e = token_map(&o, a, BWD ? a.d_o : SUM ? a.v : a.o, a.HV, a.V);
+  // (an o off 16 bytes takes no map; its place is then not used)
+  if (e == cudaSuccess) e = token_map(&o, a, BWD ? a.d_o : SUM || ((uintptr_t)a.o & 15) ? a.v : a.o, a.HV, a.V);
   st = e16 = o;  // unused by the forward
   const int64_t sh = gdr_slots(a, C) * a.HV;
   if (BWD && e == cudaSuccess) e = matrix_map(&st, a, w.S0, a.K, sh);

@@ -286,7 +286,8 @@ int ccq_decode_step_l2norm(int dtype, int B, int T, int H, int K,
 typedef enum {
   CCQ_GDR_VARLEN = 1,    /* cu_seqlens is given */
   CCQ_GDR_HAVE_FWD = 2,  /* backward: the forward's workspace is given (ccq_gdr_bwd_from) */
-  CCQ_GDR_UNALIGNED = 4  /* a 16-bit tensor is not 16-byte aligned: the call takes the exact path */
+  CCQ_GDR_UNALIGNED = 4  /* a 16-bit tensor is not 16-byte aligned: with q, k, v, d_o, dq, dk or dv the call takes the
+                            exact path (o has no rule); the size is enough for either path */
 } ccq_gdr_flags;
 
 size_t ccq_gdr_workspace_size(int op /* CCQ_OP_FWD or CCQ_OP_BWD */, int dtype, int B, int T, int H, int HV,
@@ -315,7 +316,9 @@ int ccq_gdr_bwd(int dtype, int B, int T, int H, int HV, int K, int V,
 /*
  * The same with the workspace of the ccq_gdr_fwd call on the same inputs, unmodified since (it holds the
  * chunks' inverses and scores: on the tensor-core path the backward then starts from them instead of forming
- * them again; the exact path does not read it).  NULL: as ccq_gdr_bwd.
+ * them again; the exact path does not read it).  NULL: as ccq_gdr_bwd.  Which path wrote it follows from the
+ * sizes, the types and the alignment of q, k and v, none of which may change between the two calls; the
+ * alignment of o and the environment (read at the first call) do not enter.
  */
 int ccq_gdr_bwd_from(int dtype, int B, int T, int H, int HV, int K, int V,
                      const void* q, const void* k, const void* v,
