@@ -510,7 +510,9 @@ int gdr_args(ccq::GdrArgs* out, int dtype, int B, int T, int H, int HV, int K, i
   return CCQ_OK;
 }
 
-int need_workspace(const char* who, size_t need, const void* ws, size_t got) {
+// align: of the widest access to it
+int need_workspace(const char* who, size_t need, const void* ws, size_t got, int align) {
+  if (need > 0 && (uintptr_t)ws % align != 0) return fail(CCQ_ERR_INVALID, "%s: the workspace must be %d-byte aligned", who, align);
   if (need > 0 && (ws == nullptr || got < need))
     return fail(CCQ_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, got);
   return CCQ_OK;
@@ -550,7 +552,7 @@ int ccq_gdr_fwd(int dtype, int B, int T, int H, int HV, int K, int V, const void
   a.final_state = final_state;
   const bool tc = ccq::gdr_tc_supported(a);
   st = need_workspace("ccq_gdr_fwd", tc ? ccq::gdr_tc_workspace(a, false) : ccq::gdr_simt_workspace(a, false), workspace,
-                      workspace_bytes);
+                      workspace_bytes, 16);
   if (st != CCQ_OK) return st;
   int launches = 0;
   cudaError_t e = tc ? ccq::gdr_tc_fwd(a, &launches) : ccq::gdr_simt_fwd(a, &launches);
@@ -588,9 +590,10 @@ int ccq_gdr_bwd_from(int dtype, int B, int T, int H, int HV, int K, int V, const
   a.dq = dq; a.dk = dk; a.dv = dv; a.dg = dg; a.dbeta = dbeta;
   a.dinitial_state = dinitial_state;
   a.fwd_workspace = fwd_workspace;
+  if ((uintptr_t)fwd_workspace & 15) return fail(CCQ_ERR_INVALID, "ccq_gdr_bwd: fwd_workspace must be 16-byte aligned");
   const bool tc = ccq::gdr_tc_supported(a);
   st = need_workspace("ccq_gdr_bwd", tc ? ccq::gdr_tc_workspace(a, true) : ccq::gdr_simt_workspace(a, true), workspace,
-                      workspace_bytes);
+                      workspace_bytes, 16);
   if (st != CCQ_OK) return st;
   int launches = 0;
   cudaError_t e = tc ? ccq::gdr_tc_bwd(a, &launches) : ccq::gdr_simt_bwd(a, &launches);
@@ -711,7 +714,7 @@ int ccq_layer_norm_bwd(int dtype, int form, int64_t rows, int D, const void* x, 
   a.dweight = dweight;
   a.dbias = dbias;
   a.partial = reinterpret_cast<float*>(workspace);
-  st = need_workspace("ccq_layer_norm_bwd", ccq::layer_norm_bwd_workspace(rows, D), workspace, workspace_bytes);
+  st = need_workspace("ccq_layer_norm_bwd", ccq::layer_norm_bwd_workspace(rows, D), workspace, workspace_bytes, 4);
   if (st != CCQ_OK) return st;
   int launches = 0;
   cudaError_t e = ccq::layer_norm_bwd(a, &launches);

@@ -62,13 +62,14 @@ struct GdrArgs {
   cudaStream_t stream;
 };
 
+// Both paths read their workspaces in 16-byte pieces: the entry points refuse one that is not on such a boundary.
 // Exact path: fp32 arithmetic on the CUDA cores, any K <= 256 and any V, fp32 / bf16 / fp16.
 size_t gdr_simt_workspace(const GdrArgs& a, bool bwd);
 cudaError_t gdr_simt_fwd(const GdrArgs& a, int* launches);
 cudaError_t gdr_simt_bwd(const GdrArgs& a, int* launches);
 
 // Tensor-core path (gdr_tc*.cu): 16-bit inputs, K a multiple of 8 up to 128, V a multiple of 8,
-// 16-byte aligned tensors and workspace.  Word 0 of the workspace receives the device error code.
+// 16-byte aligned tensors but for o.  Word 0 of the workspace receives the device error code.
 bool gdr_tc_supported(const GdrArgs& a);
 size_t gdr_tc_workspace(const GdrArgs& a, bool bwd);
 cudaError_t gdr_tc_fwd(const GdrArgs& a, int* launches);

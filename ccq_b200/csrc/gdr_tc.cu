@@ -94,7 +94,7 @@ bool gdr_tc_supported(const GdrArgs& a) {
   if (a.T < 1 || a.K > 128 || a.K % 8 != 0 || a.V % 8 != 0) return false;
   if (gdr_slots(a, C) * a.HV >= (1ll << 31)) return false;  // the kernels count (chunk, head) pairs in 32 bits
   const uintptr_t p = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.d_o | (uintptr_t)a.dq |
-                      (uintptr_t)a.dk | (uintptr_t)a.dv | (uintptr_t)a.workspace | (uintptr_t)a.fwd_workspace;
+                      (uintptr_t)a.dk | (uintptr_t)a.dv;
   return (p & 15) == 0;
 }
 

@@ -282,6 +282,7 @@ int ccq_decode_step_l2norm(int dtype, int B, int T, int H, int K,
  *   K <= 256; inputs must be finite, except that g = -inf resets the state (any g below -1000 does).
  *   final_state may be NULL.  Documents of length zero return their initial state.
  * All sums, the state and the running sums of g are fp32 or wider.
+ * workspace and fwd_workspace must be 16-byte aligned (CCQ_ERR_INVALID).
  */
 typedef enum {
   CCQ_GDR_VARLEN = 1,    /* cu_seqlens is given */
@@ -347,7 +348,8 @@ int ccq_gdr_step(int dtype, int B, int T, int H, int HV, int K, int V,
  *   h: written when residual is given (the sum in x's dtype; the norm reads the unrounded sum);
  *   stats: fp32 [rows, 2] mean and 1 / sqrt(var + eps), NULL when no backward follows.
  * Backward: dh is the gradient arriving on h (or NULL); dx is also the gradient of residual; dweight and
- * dbias may be NULL.  They are summed in a fixed order: the same inputs give the same bits.
+ * dbias may be NULL.  They are summed in a fixed order: the same inputs give the same bits.  The workspace must
+ * be 4-byte aligned (CCQ_ERR_INVALID).
  */
 typedef enum { CCQ_NORM_LAYER = 0, CCQ_NORM_RMS = 1 } ccq_norm_form;
 
