@@ -16,6 +16,7 @@ CCQ_OK, CCQ_ERR_INVALID, CCQ_ERR_UNSUPPORTED, CCQ_ERR_CUDA, CCQ_ERR_WORKSPACE = 
 CCQ_F32, CCQ_BF16, CCQ_F16 = 0, 1, 2
 CCQ_LAMBDA_TOKEN, CCQ_LAMBDA_GATE = 0, 1
 CCQ_OP_FWD, CCQ_OP_BWD, CCQ_OP_DECODE = 0, 1, 2
+CCQ_PATH_TCGEN05 = 2
 PATHS = {0: 'none', 1: 'simt', 2: 'tcgen05', 3: 'decode'}
 
 EXPORTS = ('ccq_last_error', 'ccq_last_path', 'ccq_version', 'ccq_last_launch_count',

@@ -64,7 +64,8 @@ def _head(q, k, v, g, beta, scale, cu, N, h0):
 
 
 def _forward(q, k, v, g, beta, scale, initial_state, output_final_state, cu_seqlens):
-    """One ccq_gdr_fwd call; returns (o, final state or None, what a backward needs)."""
+    """One ccq_gdr_fwd call; returns (o, final state or None, what a backward needs).  Only the tensor-core path's
+    workspace is of use to a backward; the exact path's is let go."""
     index = cuda_index(q, k, v, g, beta, initial_state, cu_seqlens)
     q, k, v, g, beta = _inputs(q, k, v, g, beta)
     cu, N = _seqs(q.shape[0], cu_seqlens, q.shape[1])
@@ -73,8 +74,10 @@ def _forward(q, k, v, g, beta, scale, initial_state, output_final_state, cu_seql
     o = torch.empty_like(v)
     state = torch.empty(shape, device=q.device, dtype=torch.float32) if output_final_state else None
     ws, nbytes = _workspace(_lib.CCQ_OP_FWD, q, v, N, cu)
-    invoke(_lib.load().ccq_gdr_fwd, index, *_head(q, k, v, g, beta, scale, cu, N, h0), o.data_ptr(), ptr(state), ptr(ws),
-           nbytes)
+    lib = _lib.load()
+    invoke(lib.ccq_gdr_fwd, index, *_head(q, k, v, g, beta, scale, cu, N, h0), o.data_ptr(), ptr(state), ptr(ws), nbytes)
+    if lib.ccq_last_path() != _lib.CCQ_PATH_TCGEN05:
+        ws = None
     return o, state, (q, k, v, g, beta, h0, cu, ws)
 
 

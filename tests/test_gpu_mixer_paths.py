@@ -43,3 +43,18 @@ def test_unaligned_output(lib, T, HV, V, lens, dtype):
         outs.append([o, *d])
     for other in outs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(outs[0], other))
+
+
+@pytest.mark.parametrize('dtype,K,kept', [(torch.float32, 64, False), (torch.bfloat16, 136, False), (torch.bfloat16, 64, True)])
+def test_only_a_workspace_the_backward_reads_is_kept(lib, dtype, K, kept):
+    """Between forward and backward a call holds its inputs, o and, on the tensor-core path alone, the forward's
+    workspace (on the exact path 268 bytes a token and head that nobody reads)."""
+    import ccq_b200
+    B, T, H, V = 1, 2048, 4, 64
+    x = [torch.nn.functional.normalize(torch.randn(B, T, H, n, device='cuda'), dim=-1).to(dtype) for n in (K, K, V)]
+    x = [t.requires_grad_(True) for t in (*x, -torch.rand(B, T, H, device='cuda'), torch.rand(B, T, H, device='cuda'))]
+    before = torch.cuda.memory_allocated()
+    o, _ = ccq_b200.gated_delta_rule(*x)
+    more = torch.cuda.memory_allocated() - before - o.numel() * o.element_size()
+    assert (more > 100 * B * T * H) == kept, more
+    assert all(torch.isfinite(d).all() for d in torch.autograd.grad(o.float().sum(), x))
