@@ -2,16 +2,33 @@
 gated delta rule, over whole sequences (training, prefill) and token by token over the generation cache.
 
 The cache is the reference's 4-tuple (ccq/gdn/layer.py:318-336, :394-400): (recurrent state [N, HV, K, V],
-covariance state [N, H, K, K], mean state [N, H, K] or None, position offset), the states fp32.
+covariance state [N, H, K, K], mean state [N, H, K] or None, position offset), the states fp32.  The offset is an
+int, the position all of them have reached; after packed documents, which end at positions of their own, it is
+a tensor [N].  The cleaning read divides by one position for the whole call, so such a cache is continued
+document by document: (state[n:n + 1], cov[n:n + 1], mean[n:n + 1], int(offset[n])).
 """
 from __future__ import annotations
+
+import torch
 
 from .delta_rule import gated_delta_rule, gated_delta_step
 from .ops import decode_step_l2norm, fused_ccq_clean_read_l2norm
 
 
 def _unpack(cache):
-    return cache if cache is not None else (None, None, None, 0)
+    if cache is None:
+        return None, None, None, 0
+    if isinstance(cache[3], torch.Tensor) and cache[3].numel() != 1:
+        raise ValueError(f'the cache holds {cache[3].numel()} documents that ended at positions of their own, and one call has one '
+                         'position: continue them one by one, with the rows of the states and int(offset) of each')
+    return cache
+
+
+def _after(offset, T, cu_seqlens):
+    """The position offset after T tokens; one for each of several packed documents."""
+    if cu_seqlens is None or cu_seqlens.numel() == 2:
+        return offset + T
+    return offset + (cu_seqlens[1:] - cu_seqlens[:-1]).to(torch.int64)
 
 
 def ccq_gated_delta_rule(q, k, v, lambda_h, g, beta, *, scale=None, cache=None, output_cache=False, cu_seqlens=None,
@@ -29,7 +46,7 @@ def ccq_gated_delta_rule(q, k, v, lambda_h, g, beta, *, scale=None, cache=None, 
         subtract_mean=subtract_mean, cu_seqlens=cu_seqlens)
     o, state = gated_delta_rule(q_clean, k_norm, v, g, beta, scale=scale, initial_state=state,
                                 output_final_state=output_cache, cu_seqlens=cu_seqlens)
-    return o, (state, cov, mean, offset + q.shape[1]) if output_cache else None
+    return o, (state, cov, mean, _after(offset, q.shape[1], cu_seqlens)) if output_cache else None
 
 
 def ccq_gated_delta_step(q, k, v, lambda_h, g, beta, cache, *, scale=None, subtract_mean=True, inplace=True):
