@@ -18,9 +18,7 @@ from ._call import cuda_index, invoke, ptr, wants_grad
 from .ops import _dtype_code, _seqs, _state
 
 
-def _inputs(q, k, v, g, beta):
-    """The five inputs checked, contiguous and aligned; k and v in q's dtype, g and beta in their own
-    (another type than float32, bfloat16 or float16 is an error)."""
+def _check(q, k, v, g, beta):
     if q.ndim != 4 or v.ndim != 4:
         raise ValueError(f'q, k must be [B, T, H, K] and v [B, T, HV, V], got {tuple(q.shape)} and {tuple(v.shape)}')
     B, T, H, K = q.shape
@@ -36,6 +34,12 @@ def _inputs(q, k, v, g, beta):
         raise ValueError(f'beta has shape {tuple(beta.shape)}, expected {gates}')
     if HV % H != 0:
         raise ValueError(f'the number of value heads ({HV}) must be a multiple of the number of key heads ({H})')
+
+
+def _inputs(q, k, v, g, beta):
+    """The five inputs checked, contiguous and aligned; k and v in q's dtype, g and beta in their own
+    (another type than float32, bfloat16 or float16 is an error)."""
+    _check(q, k, v, g, beta)
     dt = q.dtype
     return (_aligned(q), _aligned(k if k.dtype == dt else k.to(dt)), _aligned(v if v.dtype == dt else v.to(dt)),
             g.contiguous(), beta.contiguous())
@@ -133,6 +137,22 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, output
     return _forward(q, k, v, g, beta, scale, initial_state, output_final_state, cu_seqlens)[:2]
 
 
+def check_step(q, k, v, g, beta, state, inplace):
+    """Raises what ``gated_delta_step`` of a dense batch would, before anything is written."""
+    cuda_index(q, k, v, g, beta, state)
+    _check(q, k, v, g, beta)
+    for t in (q, g, beta):
+        _dtype_code(t)
+    _check_state(state, (q.shape[0], v.shape[2], q.shape[3], v.shape[3]), inplace)
+
+
+def _check_state(state, shape, inplace):
+    if inplace and (state is None or state.dtype != torch.float32 or not state.is_contiguous()):
+        raise ValueError('inplace needs a contiguous float32 state')
+    if state is not None and tuple(state.shape) != shape:
+        raise ValueError(f'state has shape {tuple(state.shape)}, expected {shape}')
+
+
 def gated_delta_step(q, k, v, g, beta, state=None, *, scale=None, cu_seqlens=None, inplace=False):
     """The same recurrence token by token over a cache (inference; no autograd), meant for one token or
     a few per sequence.
@@ -144,8 +164,7 @@ def gated_delta_step(q, k, v, g, beta, state=None, *, scale=None, cu_seqlens=Non
     q, k, v, g, beta = _inputs(q, k, v, g, beta)
     cu, N = _seqs(q.shape[0], cu_seqlens, q.shape[1])
     shape = (N, v.shape[2], q.shape[3], v.shape[3])
-    if inplace and (state is None or state.dtype != torch.float32 or not state.is_contiguous()):
-        raise ValueError('inplace needs a contiguous float32 state')
+    _check_state(state, shape, inplace)
     h0 = _state(state, shape)
     out = state if inplace else torch.empty(shape, device=q.device, dtype=torch.float32)
     o = torch.empty_like(v, requires_grad=False)

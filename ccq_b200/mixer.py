@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import torch
 
-from .delta_rule import gated_delta_rule, gated_delta_step
+from .delta_rule import check_step, gated_delta_rule, gated_delta_step
 from .ops import decode_step_l2norm, fused_ccq_clean_read_l2norm
 
 
@@ -55,6 +55,7 @@ def ccq_gated_delta_step(q, k, v, lambda_h, g, beta, cache, *, scale=None, subtr
     """
     state, cov, mean, offset = _unpack(cache)
     inplace = inplace and cache is not None
+    check_step(q, k, v, g, beta, state, inplace)  # the cleaning read writes its states before the rule is called
     q_clean, k_norm, cov, mean = decode_step_l2norm(q, k, lambda_h, cov, mean, position_offset=offset,
                                                     subtract_mean=subtract_mean, inplace=inplace)
     o, state = gated_delta_step(q_clean, k_norm, v, g, beta, state, scale=scale, inplace=inplace)

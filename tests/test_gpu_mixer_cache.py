@@ -65,3 +65,32 @@ def test_one_packed_document_keeps_an_int_offset():
     x = inputs(40)
     _, cache = ccq_b200.ccq_gated_delta_rule(*x, output_cache=True, cu_seqlens=torch.tensor([0, 40], device='cuda'))
     assert cache[3] == 40 and isinstance(cache[3], int)
+
+
+@pytest.mark.parametrize('edit', ['half state', 'transposed state', 'state shape', 'value batch', 'gate type', 'beta shape', 'no state'])
+def test_a_refused_step_leaves_the_cache_as_it_was(edit):
+    """The cleaning read and the rule update the cache one after the other: what the rule refuses, neither may do."""
+    import ccq_b200
+    x = inputs(30)
+    _, cache = ccq_b200.ccq_gated_delta_rule(*x, output_cache=True)
+    q, k, v, lam, g, beta = inputs(1, seed=9)
+    state = cache[0]
+    if edit == 'half state':
+        state = state.half()
+    elif edit == 'transposed state':
+        state = state.transpose(2, 3).contiguous().transpose(2, 3)
+    elif edit == 'state shape':
+        state = state[:, :1].contiguous()
+    elif edit == 'value batch':
+        v = torch.cat([v, v])
+    elif edit == 'gate type':
+        g = g.double()
+    elif edit == 'beta shape':
+        beta = beta[..., :1]
+    else:
+        state = None
+    cache = (state, *cache[1:])
+    kept = [t.clone() for t in cache[1:3]]
+    with pytest.raises((ValueError, TypeError)):
+        ccq_b200.ccq_gated_delta_step(q, k, v, lam, g, beta, cache)
+    assert all(torch.equal(a, b) for a, b in zip(kept, cache[1:3]))
