@@ -42,5 +42,13 @@ def cuda_index(*tensors):
     return index
 
 
+def written(*tensors):
+    """Tells autograd that a kernel wrote to these tensors (None among them is skipped): a backward that saved one of
+    them raises, as after an in-place operation of torch, instead of reading the new values."""
+    for t in tensors:
+        if t is not None:
+            torch.autograd.graph.increment_version(t)
+
+
 def wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

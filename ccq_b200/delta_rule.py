@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._call import cuda_index, invoke, ptr, wants_grad
+from ._call import cuda_index, invoke, ptr, wants_grad, written
 from .ops import _dtype_code, _seqs, _state
 
 
@@ -170,4 +170,6 @@ def gated_delta_step(q, k, v, g, beta, state=None, *, scale=None, cu_seqlens=Non
     o = torch.empty_like(v, requires_grad=False)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     invoke(_lib.load().ccq_gdr_step, index, *_head(q, k, v, g, beta, scale, cu, N, h0), out.data_ptr(), o.data_ptr())
+    if inplace:
+        written(out)
     return o, out

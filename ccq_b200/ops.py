@@ -16,6 +16,7 @@ import os
 import torch
 
 from . import _lib
+from ._call import written
 
 _DT = {torch.float32: _lib.CCQ_F32, torch.bfloat16: _lib.CCQ_BF16, torch.float16: _lib.CCQ_F16}
 
@@ -487,6 +488,7 @@ def _decode(q, k, lambda_h, cov_state, mean_state, position_offset, subtract_mea
                                         N, int(position_offset), int(bool(subtract_mean)), _p(cov_in), _p(mean_in),
                                         _p(cov_out), _p(mean_out), _p(qc), _p(kn), _stream(dev))
     _lib.check(st)
+    written(cov_out if cov_out is cov_in else None, mean_out if mean_out is mean_in else None)
     return qc, kn, cov_out, mean_out
 
 

@@ -1,0 +1,61 @@
+"""What the mixer operators tell autograd."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope='module', autouse=True)
+def _lib():
+    if not torch.cuda.is_available():
+        pytest.skip('no CUDA device')
+    from ccq_b200 import _lib as L
+    L.load()
+
+
+def inputs(T=40, B=2, H=2, HV=2, K=128, V=64, dtype=torch.bfloat16):
+    r = lambda *s: torch.randn(*s, device='cuda')  # noqa: E731
+    unit = lambda t: torch.nn.functional.normalize(t, dim=-1)  # noqa: E731
+    x = [unit(r(B, T, H, K)), unit(r(B, T, H, K)), r(B, T, HV, V)]
+    return [t.to(dtype) for t in x] + [-torch.rand(B, T, HV, device='cuda'), r(B, T, HV).sigmoid()]
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('leaf', ['q', 'state'])
+def test_a_step_on_a_saved_state_is_seen(dtype, leaf):
+    """A backward that saved the state raises once a step has written to it, as after an in-place operation of torch."""
+    import ccq_b200
+    x, token = inputs(dtype=dtype), inputs(1, dtype=dtype)
+    state = torch.randn(2, 2, 128, 64, device='cuda')
+    (x[0] if leaf == 'q' else state).requires_grad_(True)
+    loss = ccq_b200.gated_delta_rule(*x, initial_state=state)[0].float().sum()
+    with torch.no_grad():
+        ccq_b200.gated_delta_step(*token, state)                     # a new state: nothing is written
+        loss.backward(retain_graph=True)
+        ccq_b200.gated_delta_step(*token, state, inplace=True)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+
+
+@pytest.mark.parametrize('which', [1, 2])
+def test_a_step_on_a_saved_covariance_or_mean_is_seen(which):
+    import ccq_b200
+    q, k, _, _, _ = inputs()
+    cov, mean = torch.randn(2, 2, 128, 128, device='cuda'), torch.randn(2, 2, 128, device='cuda')
+    one = lambda t, i: t.clone() if i != which else t  # noqa: E731
+    loss = ccq_b200.fused_ccq_clean_read(q.requires_grad_(True), k, 0.5, initial_cov_state=cov,
+                                         initial_mean_state=mean)[0].float().sum()
+    with torch.no_grad():
+        ccq_b200.decode_step(q[:, :1], k[:, :1], 0.5, cov, mean)
+        loss.backward(retain_graph=True)
+        ccq_b200.decode_step(q[:, :1], k[:, :1], 0.5, one(cov, 1), one(mean, 2), inplace=True)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+
+
+def test_steps_in_inference_mode():
+    import ccq_b200
+    with torch.inference_mode():
+        state = torch.zeros(2, 2, 128, 64, device='cuda')
+        o, S = ccq_b200.gated_delta_step(*inputs(1), state, inplace=True)
+        assert S is state and torch.isfinite(o).all() and (state != 0).any()
