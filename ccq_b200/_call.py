@@ -4,6 +4,7 @@ stream handle is read without a stream object."""
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -51,4 +52,9 @@ def written(*tensors):
 
 
 def wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a call goes through its autograd function: a gradient is asked for, or an input carries a forward-mode
+    tangent, which the function refuses and a plain call would drop."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)

@@ -59,3 +59,28 @@ def test_steps_in_inference_mode():
         state = torch.zeros(2, 2, 128, 64, device='cuda')
         o, S = ccq_b200.gated_delta_step(*inputs(1), state, inplace=True)
         assert S is state and torch.isfinite(o).all() and (state != 0).any()
+
+
+def _calls():
+    import ccq_b200
+    x = inputs(dtype=torch.float32)
+    rows, w = torch.randn(5, 64, device='cuda'), torch.ones(64, device='cuda')
+    yield 'rule', x, lambda *t: ccq_b200.gated_delta_rule(*t)[0]
+    yield 'rule with a state', [*x, torch.randn(2, 2, 128, 64, device='cuda')], lambda *t: ccq_b200.gated_delta_rule(*t[:5], initial_state=t[5])[0]
+    yield 'layer norm', [rows, w, w], ccq_b200.layer_norm
+    yield 'rms norm', [rows, w, rows], lambda a, b, c: ccq_b200.rms_norm(a, b, residual=c)[0]
+    yield 'gated', [rows, rows, w], ccq_b200.gated_rms_norm
+
+
+@pytest.mark.parametrize('grad', [True, False])
+def test_forward_mode_is_refused(grad):
+    """There is no forward-mode derivative: an input that carries a tangent raises, whichever it is, and does not
+    come out as a constant."""
+    from torch.autograd import forward_ad
+    for name, x, f in _calls():
+        for i in range(len(x)):
+            with torch.set_grad_enabled(grad), forward_ad.dual_level():
+                y = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(x)]
+                with pytest.raises((RuntimeError, NotImplementedError), match='jvp|forward mode'):
+                    f(*y)
+                assert torch.isfinite(f(*x)).all(), name     # no tangent: an ordinary call
