@@ -58,3 +58,27 @@ def wants_grad(*tensors):
         return True
     return forward_ad._current_level >= 0 and any(
         t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+class _FirstOnly(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, anchor, *grads):
+        return grads
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError('the gated delta rule and the norms have no second derivative')
+
+
+def first_derivative(backward):
+    """For an autograd function's backward: gradients asked for with create_graph=True raise if they are differentiated
+    again, as the kernels' outputs would otherwise count as constants."""
+    def run(ctx, *seen):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *seen)
+        with torch.no_grad():
+            grads = backward(ctx, *seen)
+        real = [t for t in grads if t is not None]
+        real = iter(_FirstOnly.apply(torch.zeros((), device=real[0].device, requires_grad=True), *real))
+        return tuple(None if t is None else next(real) for t in grads)
+    return run

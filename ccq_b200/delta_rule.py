@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._call import cuda_index, invoke, ptr, wants_grad, written
+from ._call import cuda_index, first_derivative, invoke, ptr, wants_grad, written
 from .ops import _dtype_code, _seqs, _state
 
 
@@ -100,6 +100,7 @@ class GatedDeltaRule(torch.autograd.Function):
         return o, state
 
     @staticmethod
+    @first_derivative
     def backward(ctx, do, dstate):
         q, k, v, g, beta, h0, cu, fwd_ws = ctx.saved_tensors
         do = torch.zeros_like(v) if do is None else _aligned(do if do.dtype == v.dtype else do.to(v.dtype))

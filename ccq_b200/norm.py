@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._call import cuda_index, invoke, ptr, wants_grad
+from ._call import cuda_index, first_derivative, invoke, ptr, wants_grad
 from .ops import _dtype_code
 
 
@@ -62,6 +62,7 @@ class LayerNorm(torch.autograd.Function):
         return y, h
 
     @staticmethod
+    @first_derivative
     def backward(ctx, dy, dh):
         x, residual, weight, bias, gate, stats = ctx.saved_tensors
         D = x.shape[-1]

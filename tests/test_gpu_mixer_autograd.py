@@ -84,3 +84,16 @@ def test_forward_mode_is_refused(grad):
                 with pytest.raises((RuntimeError, NotImplementedError), match='jvp|forward mode'):
                     f(*y)
                 assert torch.isfinite(f(*x)).all(), name     # no tangent: an ordinary call
+
+
+def test_a_second_derivative_is_refused():
+    """A penalty on a gradient raises; without the refusal its part through the operators would be left out."""
+    for name, x, f in _calls():
+        x = [t.detach().clone().requires_grad_(True) for t in x]
+        seed = torch.randn_like(f(*x))
+        plain = torch.autograd.grad(f(*x), x, seed)
+        graph = torch.autograd.grad(f(*x), x, seed, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, graph)), name
+        for d in graph:
+            with pytest.raises(RuntimeError, match='second derivative'):
+                (d.square().sum() + sum(t.square().sum() for t in x)).backward()
