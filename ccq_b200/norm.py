@@ -85,6 +85,11 @@ class LayerNorm(torch.autograd.Function):
 
 
 def _norm(x, weight, bias, residual, gate, eps, form):
+    if residual is not None and residual.dtype != x.dtype and x.dtype in (torch.bfloat16, torch.float16) \
+            and torch.promote_types(x.dtype, residual.dtype) != x.dtype:
+        # a residual stream that x's type cannot hold is not rounded to it
+        y, h = _norm(x.float(), weight, bias, residual, gate, eps, form)
+        return y.to(x.dtype), h
     if wants_grad(x, weight, bias, residual, gate):
         return LayerNorm.apply(x, weight, bias, residual, gate, float(eps), form)
     return _forward(x, weight, bias, residual, gate, float(eps), form, False)[:2]
@@ -94,7 +99,8 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, residual=None):
     """Layer norm over the last axis (at most 16384 elements).
 
     weight and bias: [D] or None.  With ``residual`` (x's shape) the norm reads h = x + residual, and the
-    call returns (y, h): h, rounded to x's dtype, is the stream the next block adds to.
+    call returns (y, h): h is the stream the next block adds to.  y has x's dtype, and so has h unless residual's
+    is wider: a float32 stream stays one, and the call then runs in float32 (its casts are passes of their own).
     """
     y, h = _norm(x, weight, bias, residual, None, eps, _lib.CCQ_NORM_LAYER)
     return (y, h) if residual is not None else y
@@ -108,5 +114,5 @@ def rms_norm(x, weight=None, *, eps=1e-5, residual=None):
 
 def gated_rms_norm(x, gate, weight=None, *, eps=1e-5):
     """rms_norm(x) * gate * sigmoid(gate): the norm a GDN layer applies to each head's output
-    (ccq/gdn/layer.py, o_norm); gate has x's shape."""
+    (ccq/gdn/layer.py, o_norm); gate has x's shape and is taken in its dtype."""
     return _norm(x, weight, None, None, gate, eps, _lib.CCQ_NORM_RMS)[0]
