@@ -225,23 +225,22 @@ __device__ __forceinline__ void zero_rows(uint32_t tile, int panels, int from, i
   }
 }
 
-// rows [0, valid) of a staged [64 x 128] tile to a [tokens, HV, V] tensor with plain stores
+// rows [0, valid) of a staged [64 x 128] tile to a [tokens, HV, V] tensor with plain stores; ANY: of whole elements
+// where the tensor is off 16 bytes
+template <bool ANY = false>
 __device__ __forceinline__ void copy_rows(uint32_t tile, uint16_t* dst, int64_t row0, int HV, int hv, int V, int v0,
                                           int valid, int t, int count) {
   for (int i = t; i < valid * 16; i += count) {
     const int r = i >> 4, ch = i & 15;
-    if (v0 + ch * 8 < V)
-      *reinterpret_cast<uint4*>(dst + ((row0 + r) * HV + hv) * V + v0 + ch * 8) =
-          lds128(tile + (ch >> 3) * PANEL + tc::sw128(r, ch & 7));
-  }
-}
-
-// the same to a tensor off 16 bytes: whole elements
-__device__ __forceinline__ void copy_rows_unaligned(uint32_t tile, uint16_t* dst, int64_t row0, int HV, int hv, int V, int v0,
-                                                    int valid, int t, int count) {
-  for (int i = t; i < valid * VT; i += count) {
-    const int r = i / VT, c = i % VT;
-    if (v0 + c < V) dst[((row0 + r) * HV + hv) * V + v0 + c] = lds16(Column(tile, c).at(r));
+    if (v0 + ch * 8 >= V) continue;
+    uint16_t* to = dst + ((row0 + r) * HV + hv) * V + v0 + ch * 8;
+    const uint32_t from = tile + (ch >> 3) * PANEL + tc::sw128(r, ch & 7);
+    if (!ANY || ((uintptr_t)dst & 15) == 0) {
+      *reinterpret_cast<uint4*>(to) = lds128(from);
+    } else {
+#pragma unroll 1
+      for (int e = 0; e < 8; ++e) to[e] = lds16(from + 2 * e);
+    }
   }
 }
 

@@ -360,7 +360,6 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
     const int vl = quad * 32 + lane;
     const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
     const int64_t slots = gdr_slots(a, C);
-    const bool o16 = ((uintptr_t)a.o & 15) == 0;
     for (int c = 0; c < nch; ++c) {
       const int s = c & 1, ph = c & 1;
       const int valid = min(C, sq.len - c * C);
@@ -412,7 +411,7 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
         const Column O(out, vl);
 #pragma unroll
         for (int i = 0; i < OT; ++i) sts16(O.at(j0 + i), f2h<AB16>(y[i]));
-        if (valid == C && o16) {
+        if (valid == C && ((uintptr_t)a.o & 15) == 0) {
           fence_async_smem();
           bar_sync<1, G::OUT_THREADS>();
           if (threadIdx.x == 0) {
@@ -422,9 +421,7 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
           }
         } else {
           bar_sync<1, G::OUT_THREADS>();
-          uint16_t* o = reinterpret_cast<uint16_t*>(a.o);
-          if (o16) copy_rows(out, o, row0, a.HV, hv, a.V, v0, valid, threadIdx.x, G::OUT_THREADS);
-          else copy_rows_unaligned(out, o, row0, a.HV, hv, a.V, v0, valid, threadIdx.x, G::OUT_THREADS);
+          copy_rows<true>(out, reinterpret_cast<uint16_t*>(a.o), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, G::OUT_THREADS);
         }
       } else {
         const Column D(p + L::DO, vl);
