@@ -33,7 +33,7 @@ size_t carve(const GdrArgs& a, bool bwd, Ws* w) {
   const size_t heads = (size_t)a.n_seqs * a.HV, states = heads * a.K * a.V * 4;
   t.nseg = plan_segments(a, &t.seg_chunks);
   t.order = order ? reinterpret_cast<int*>(take(order)) : nullptr;
-  t.mats = take(sh * MATS);
+  t.mats = take(sh * mats_bytes(a.dtype == DT_BF16));
   t.aux = reinterpret_cast<float*>(take(sh * AX_N * 4));
   if (t.nseg > 1) {
     t.Sin = reinterpret_cast<float*>(take(t.nseg * states));
@@ -49,6 +49,10 @@ size_t carve(const GdrArgs& a, bool bwd, Ws* w) {
     t.S0 = reinterpret_cast<uint16_t*>(take(sh * a.K * a.V * 2));
     t.dS1 = reinterpret_cast<uint16_t*>(take(sh * a.K * a.V * 2));
     t.E = reinterpret_cast<uint16_t*>(take(sh * 2 * C * a.V * 2));
+    if (a.dtype == DT_F16) {
+      take(nvt * sh * FX_N * 4);
+      take((size_t)a.B * a.T * a.HV * a.V * 2);
+    }
     t.dotO = reinterpret_cast<float*>(take(nvt * sh * C * 4));
     t.dotV = reinterpret_cast<float*>(take(nvt * sh * C * 4));
     const size_t ah = (size_t)gdr_slots(a, C * ANCHOR) * a.HV;

@@ -15,6 +15,16 @@
 // chain of three products, not by the MMA rate.  The gradient kernel, whose outputs are
 // rounded to 16 bits next and feed no recurrence, uses single 16-bit operands but for E where it makes W
 // and for W: each of these roundings alone left 1.6e-3 in dq and dk, as much as the outputs' own.
+//
+// Range.  bfloat16 has float's exponents; float16 ends at 65504 and its hi + lo loses bits below 2^-8, while states and
+// gradients are fp32 of any size.  For float16 inputs, therefore:
+//   * a product without an input (R T, E P beta, dE T) has bfloat16 operands;
+//   * an operand that meets an input has to be float16.  It is multiplied by a power of two that puts its largest value
+//     into [2^14, 2^15) (pow2_of; hi + lo then keeps 2^-22 of that value), and the product's fp32 sums by the inverse.
+//     "Its" means of a chunk and 128 columns of V, for the stored E and dV also of a token, for N and W of a chunk.
+// Operands that share an accumulator would have to share the factor, so float16 forms R = V - Gam K S0 before the
+// product with T, reads the two products of dS one after the other, and takes the gradient kernel's V in tiles of 128
+// columns; W, the one operand of two sums there, takes N's factor with it, or where N is far larger one for each sum.
 #pragma once
 
 #include "gdr.h"
@@ -27,8 +37,15 @@ constexpr int VT = 128;           // columns of V per block of the scans (TMEM l
 constexpr uint32_t PANEL = 64 * 128;        // 64 rows of 128 bytes, 128-byte swizzle
 constexpr uint32_t TILE = 2 * PANEL;        // 64 rows x 128 columns
 constexpr uint32_t MATS = 4 * PANEL;        // T hi, T lo, P beta hi, P beta lo: 64 x 64 each, swizzled as in shared memory
+// float16: these in bfloat16, then P beta hi, lo in float16 with a factor, for the product with dO
+__host__ __device__ constexpr uint32_t mats_bytes(bool bf16) { return bf16 ? MATS : MATS + 2 * PANEL; }
 // per (chunk, value head) floats, 64 tokens each: Gam, scale Gam, w beta, beta, w, G (hi and lo part); then Gam_C
-constexpr int AX_G = 0, AX_SG = 64, AX_WB = 128, AX_B = 192, AX_W = 256, AX_GH = 320, AX_GL = 384, AX_GC = 448, AX_N = 452;
+constexpr int AX_G = 0, AX_SG = 64, AX_WB = 128, AX_B = 192, AX_W = 256, AX_GH = 320, AX_GL = 384, AX_GC = 448, AX_N = 456;
+// float16 only: what undoes the factor of P beta; bounds on |k| and |q| of the chunk's tokens; the largest |scale| Gam
+constexpr int AX_UP = 449, AX_KN = 450, AX_QN = 451, AX_SM = 452;
+// float16 only, per (V tile, chunk, value head): what undoes the factors of E and dV, by token, and of S0 and dS1; the
+// largest |dO|
+constexpr int FX_E = 0, FX_DV = 64, FX_S = 128, FX_DS = 129, FX_DO = 130, FX_N = 132;
 
 // <dS, S> at a chunk's end, which every dg of the chunk holds, is the sum of the later tokens' dO . O - V . dV
 // plus its value at a later place.  Both dot products are kept to fp32, and every ANCHOR chunks <dS, S>
@@ -40,7 +57,7 @@ constexpr int ANCHOR = 8;
 struct Ws {
   int* err;            // word 0: device error code of the scans
   const int* order;    // launch slot -> document of a packed batch, longest first; nullptr: as they come
-  uint8_t* mats;       // [slots * HV][MATS]
+  uint8_t* mats;       // [slots * HV][mats_bytes]
   float* aux;          // [slots * HV][AX_N]
   // Few heads, a long axis: documents are cut into nseg segments of seg_chunks chunks (a multiple of ANCHOR),
   // which run side by side once the states at their starts are known (gdr_tc_seg.cu).  Index s * heads + head,
@@ -53,12 +70,22 @@ struct Ws {
   // backward only
   uint16_t* S0;        // [slots * HV][V][K] state before the chunk, transposed, 16-bit
   uint16_t* dS1;       // [slots * HV][V][K] gradient of the state after it
-  uint16_t* E;         // [slots * HV][V][2 C] E transposed: hi part, then lo part
+  uint16_t* E;         // [slots * HV][V][2 C] E transposed: hi part, then lo part; float16: then factors and dVs (below)
   float* dotO;         // [V tiles][slots * HV][C]: dO . O
   float* dotV;         // [V tiles][slots * HV][C]: V . dV
   float* Sf;           // [slots of 512 * HV][K][V] fp32 state after every ANCHOR chunks and after the last one
   float* anchor;       // [V tiles][slots of 512 * HV][16]: <dS, S> there, one part per chain warp
 };
+
+// float16 only: [V tiles][slots * HV][FX_N] behind E, and dV times its factors, as dv, behind that.  Not members of Ws:
+// past 128 bytes of it the compiler keeps the arguments in fewer registers and the bfloat16 kernels lose 2 to 5 %.
+__host__ __device__ inline float* factors_of(const GdrArgs& a, const Ws& w) {
+  return reinterpret_cast<float*>(w.E + ((gdr_slots(a, C) * a.HV * 2 * C * a.V + 127) & ~int64_t(127)));
+}
+__host__ __device__ inline uint16_t* scaled_dv_of(const GdrArgs& a, const Ws& w) {
+  const int64_t n = (a.V + VT - 1) / VT * gdr_slots(a, C) * a.HV * FX_N;
+  return reinterpret_cast<uint16_t*>(factors_of(a, w) + ((n + 63) & ~int64_t(63)));
+}
 
 cudaError_t prep(const GdrArgs& a, const Ws& w, int* launches);
 enum ScanMode { SCAN_FWD, SCAN_BWD, SCAN_SUM };  // output; for the backward; a segment's end state only
@@ -157,6 +184,75 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// a power of two that takes a largest value of m to [2^14, 2^15), and its inverse (m below 2^-60 counts as that, so
+// that products of factors stay finite)
+struct Pow2 {
+  float s, u;
+};
+__device__ __forceinline__ Pow2 pow2_of(float m) {
+  const int e = max((int)(__float_as_uint(m) >> 23) - 127, -60);
+  return {__uint_as_float((uint32_t)(141 - e) << 23), __uint_as_float((uint32_t)(113 + e) << 23)};
+}
+template <int N>
+__device__ __forceinline__ float abs_max(const float* x) {
+  float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) m[i & 3] = fmaxf(m[i & 3], fabsf(x[i]));
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+// the largest m of a warp; m is not negative
+__device__ __forceinline__ float warp_max(float m) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))); }
+// per token, the largest |x| of the 128 lanes of four warps, this one being `quad`: N (16 or 32) tokens from j0.  put
+// before a barrier of these warps, get after it.  Only the exponent counts, so the upper halves of two tokens share a
+// word; every step halves the words a lane keeps.  (A reduction instruction a token is several times slower.)
+template <int N>
+__device__ __forceinline__ void token_max_put(const float* x, float (*parts)[C], int j0, int quad, int lane) {
+  uint32_t m[N / 2];
+#pragma unroll
+  for (int j = 0; j < N / 2; ++j)
+    m[j] = __byte_perm(__float_as_uint(x[2 * j]), __float_as_uint(x[2 * j + 1]), 0x7632) & 0x7FFF7FFFu;
+#pragma unroll
+  for (int s = 0; s < 5; ++s) {
+    const int o = 16 >> s, n = (N / 2) >> s;
+    const bool up = (lane & o) != 0;
+    if (n <= 1) {
+      m[0] = tc::max2_bf16(m[0], __shfl_xor_sync(0xffffffffu, m[0], o));
+    } else {
+#pragma unroll
+      for (int i = 0; i < n / 2; ++i) {
+        const uint32_t send = up ? m[i] : m[i + n / 2], keep = up ? m[i + n / 2] : m[i];
+        m[i] = tc::max2_bf16(keep, __shfl_xor_sync(0xffffffffu, send, o));
+      }
+    }
+  }
+  constexpr int LANES = 64 / N;  // that hold the same two tokens
+  if (lane % LANES == 0)
+    *reinterpret_cast<float2*>(&parts[quad][j0 + 2 * (lane / LANES)]) =
+        make_float2(__uint_as_float(m[0] << 16), __uint_as_float(m[0] & 0xFFFF0000u));
+}
+__device__ __forceinline__ float token_max_get(const float (*parts)[C], int j) {
+  return fmaxf(fmaxf(parts[0][j], parts[1][j]), fmaxf(parts[2][j], parts[3][j]));
+}
+// the largest m of W warps, this one being `w`; `parts` (16-byte aligned) is written again only after another barrier of
+// these warps
+template <int ID, int W>
+__device__ __forceinline__ float warps_max(float m, float* parts, int w) {
+  m = warp_max(m);
+  if ((threadIdx.x & 31) == 0) parts[w] = m;
+  tc::bar_sync<ID, 32 * W>();
+  m = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(parts + i);
+    m = fmaxf(fmaxf(m, fmaxf(v.x, v.y)), fmaxf(v.z, v.w));
+  }
+  return m;
+}
+// The factor of a state comes from a bound on it: what it was and 64 max |k| max |w beta E| a chunk, loose by a few powers
+// of two, of which there are 20 to spare; every EXACT chunks it is taken anew.  (A largest value each time, over the
+// chain's warps: 10 % of the scans' time.  w beta E and Gam dV have no such bound where a state decays inside a chunk.)
+constexpr int EXACT = 8;
+
 template <int AB16>
 __device__ __forceinline__ float h2f(uint16_t x) {
   if (AB16) return __uint_as_float((uint32_t)x << 16);
@@ -196,6 +292,12 @@ struct Column {
 __device__ __forceinline__ uint16_t lds16(uint32_t addr) {
   uint16_t v;
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+  return v;
+}
+// the same, free to run ahead of ordinary loads
+__device__ __forceinline__ uint32_t lds16_early(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
   return v;
 }
 __device__ __forceinline__ void sts16(uint32_t addr, uint16_t v) {

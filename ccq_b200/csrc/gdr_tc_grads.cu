@@ -19,7 +19,8 @@
 // masked.  60 MMAs an item at V = 128.  Operands are single 16-bit values but for W, and E in P (see
 // gdr_tc.cuh).  An item moves 192 KB, which bounds the kernel: 8192 items take 302 us, 5.3 TB/s.  What is not on the
 // path from one group of products to the next (statistics, dbeta and dg, waiting for the stores to leave) comes after
-// the output, beside the next item's products; with it in front the same items took 368 us.
+// the output, beside the next item's products; with it in front the same items took 368 us.  float16: 425 us, since N and
+// W are written only when all of them are known, and so is their factor.
 //
 // Warps (576 threads): 0-7 epilogue A (P and B), 8-15 epilogue B (X and X2), all of them the output; 16 TMA,
 // 17 MMA.
@@ -41,17 +42,20 @@ constexpr uint32_t AX_BYTES = (AX_N * 4 + 127) & ~127u;
 constexpr uint32_t L_AX = L_W + 3 * PANEL;            // four
 constexpr int RING = 4;
 
-// One value head of an item, written by the TMA thread.  Four in a ring: the loads run at most two steps ahead
-// of the products, those one value head ahead of the epilogue.
+// One value head of an item (float16: 128 of its columns of V, which have factors of their own), written by the TMA
+// thread.  Four in a ring: the loads run at most two steps ahead of the products, those one record ahead of the epilogue.
 struct Rec {
   int live, hv, h, row0, valid, first, last, qk, more, zero_first;
-  int64_t sh, anchor;
+  int steps, head_first, head_last;  // 64 columns of V each; whether it begins and ends its value head
+  int64_t sh, anchor, factors;
 };
 struct Small {
   uint64_t full[2], empty[2], qk_empty[2];
   uint64_t rec_full[RING];  // the record and its per-token factors
   uint64_t p_full, x_full, wn_ready, f_full, kz, done;
   Rec rec[RING];
+  float top[8];  // float16: largest N or W of each warp of epilogue A
+  int apart;     // float16: N and W have factors of their own
   float ke[2][C], db[4][C], dg[17];
   uint32_t tmem;
   int go, abort;
@@ -73,7 +77,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t sb = smem_u32(sm);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int NP = KD / 64;
-  const int group = a.HV / a.H, nvt = (a.V + 63) / 64;
+  const int group = a.HV / a.H, nvt = (a.V + 63) / 64, parts = AB16 ? 1 : (a.V + VT - 1) / VT;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&S_.full[i], 1);
@@ -110,29 +114,37 @@ __global__ void __launch_bounds__(THREADS, 1)
         Seq sq;
         if (!gdr_slot_find(a, slot, C, &n, &c, &sq)) continue;
         const int row = (int)(sq.bos + (int64_t)c * C), nch = (sq.len + C - 1) / C;
-        for (int g = 0; g < group && ok; ++g, ++rec) {
-          const int hv = h * group + g, r = rec % RING;
+        for (int part = 0; part < group * parts && ok; ++part, ++rec) {
+          const int g = part / parts, vt0 = part % parts * (VT / 64), hv = h * group + g, r = rec % RING;
           const int64_t sh = (int64_t)slot * a.HV + hv;
-          for (int vt = 0; vt < nvt; ++vt, ++step) {
+          const int vt1 = AB16 ? nvt : min(nvt, vt0 + VT / 64);
+          for (int vt = vt0; vt < vt1; ++vt, ++step) {
             const int b = step & 1;
+            const bool begin = part == 0 && vt == 0;
             if (step >= 2 && !pipe_wait(&S_.empty[b], ((step - 2) >> 1) & 1, ab, err, 1)) { ok = false; break; }
-            if (g == 0 && vt == 0 && count >= 2 && !pipe_wait(&S_.qk_empty[count & 1], ((count - 2) >> 1) & 1, ab, err, 2)) {
+            if (begin && count >= 2 && !pipe_wait(&S_.qk_empty[count & 1], ((count - 2) >> 1) & 1, ab, err, 2)) {
               ok = false;
               break;
             }
             if (*ab) { ok = false; break; }
             uint64_t* bar = &S_.full[b];
             uint8_t* p = sm + L_B + b * B_SIZE;
-            mbar_arrive_expect_tx(bar, 2 * NP * PANEL + 4 * PANEL + (g == 0 && vt == 0 ? 2 * NP * PANEL : 0));
-            if (vt == 0) {
+            mbar_arrive_expect_tx(bar, 2 * NP * PANEL + 4 * PANEL + (begin ? 2 * NP * PANEL : 0));
+            if (vt == vt0) {
               Rec& R = S_.rec[r];
               R.live = 1;
               R.hv = hv;
               R.h = h;
               R.row0 = row;
               R.valid = min(C, sq.len - c * C);
-              R.first = g == 0;
-              R.last = g == group - 1;
+              R.first = part == 0;
+              R.last = part == group * parts - 1;
+              if (!AB16) {
+                R.steps = vt1 - vt0;
+                R.head_first = vt0 == 0;
+                R.head_last = vt1 == nvt;
+                R.factors = vt0 / (VT / 64) * gdr_slots(a, C) * a.HV + sh;
+              }
               R.qk = count & 1;
               R.more = min(ANCHOR - 1 - c % ANCHOR, nch - 1 - c);
               R.zero_first = c == 0 && a.initial_state == nullptr;
@@ -140,7 +152,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               R.anchor = (gdr_slot0(a, n, sq, C * ANCHOR) + c / ANCHOR) * a.HV + hv;
               mbar_arrive_expect_tx(&S_.rec_full[r], AX_N * 4);
               bulk_load(sm + L_AX + r * AX_BYTES, w.aux + sh * AX_N, AX_N * 4, &S_.rec_full[r]);
-              if (g == 0) {
+              if (begin) {
                 uint8_t* d = sm + L_KQ + (count & 1) * 4 * PANEL;
                 for (int i = 0; i < NP; ++i) {
                   tma_load_3d(d + 2 * i * PANEL, &tmk, bar, 64 * i, h, row);
@@ -183,7 +195,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!R.live) break;
         const uint32_t KQ = sb + L_KQ + R.qk * 4 * PANEL;
         bool ok = true;
-        for (int vt = 0; vt < nvt; ++vt, ++step) {
+        const int steps = AB16 ? nvt : R.steps;
+        for (int vt = 0; vt < steps; ++vt, ++step) {
           const int b = step & 1;
           const uint32_t p = sb + L_B + b * B_SIZE;
           if (!spin_wait(&S_.full[b], (step >> 1) & 1, ab, err, 0x10)) { ok = false; break; }
@@ -205,7 +218,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               umma(tb + T_B, d, d, id_b, ks > 0);
             }
           }
-          if (vt == nvt - 1) umma_commit(&S_.p_full);  // epilogue A starts on these, beside the products below
+          if (vt == steps - 1) umma_commit(&S_.p_full);  // epilogue A starts on these, beside the products below
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
             umma(tb + T_X, sdesc(p + B_DV + ks * 32, 16, 1024), sdesc(p + B_S + ks * 2048, PANEL, 1024), id_x, vt + ks > 0);
@@ -221,8 +234,9 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
           umma(tb + T_F, sdesc(W + ks * 32, 16, 1024), sdesc(KQ + ks * 2048, 2 * PANEL, 1024), id_x, 1);
+        const bool apart = !AB16 && S_.apart;  // the third panel is W for the transposed product, else W's second part
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
+        for (int ks = 0; ks < 4 && !apart; ++ks)
           umma_masked(tb + T_F, sdesc(W + PANEL + ks * 32, 16, 1024), sdesc(KQ + ks * 2048, 2 * PANEL, 1024), id_x, 1, ~0u, 0);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
@@ -230,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int x = 1; x < 3; ++x)
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
+          for (int ks = 0; ks < 4 && !(apart && x == 1); ++ks)
             umma_masked(tb + T_F, sdesc(W + x * PANEL + ks * 2048, 0, 1024), sdesc(KQ + PANEL + ks * 2048, 2 * PANEL, 1024), id_x2, 1, 0,
                         ~0u);
         umma_commit(&S_.f_full);
@@ -245,8 +259,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int i = (quad & 1) * 32 + lane; // token
     const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
     int stored = -1;
-    int first_step = 0;                   // step of this record's first loads
-    for (int rec = 0;; ++rec, first_step += nvt) {
+    int first_step = 0, steps = 0;        // step of this record's first loads, and how many it has
+    // float16: the factors of F's rows 0-63 (with N, and W for its transpose) and 64-127 (with W), and whether they
+    // differ in this record; this token's dbeta from the columns before
+    [[maybe_unused]] float sN = 1.f, sW = 1.f, head_db = 0.f;
+    [[maybe_unused]] bool apart = false;
+    for (int rec = 0;; ++rec, first_step += AB16 ? nvt : steps) {
       const int r = rec % RING;
       const Rec& R = S_.rec[r];
       // one decision for all warps, so that a wait that gave up cannot leave some of them at a barrier
@@ -259,6 +277,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       stored = -1;
       if (!S_.go) break;
       const int valid = R.valid;
+      if (!AB16) steps = R.steps;
       const uint32_t KQ = sb + L_KQ + R.qk * 4 * PANEL;
       const float* ax = reinterpret_cast<const float*>(sm + L_AX + r * AX_BYTES);
       if (valid < C && R.first) {
@@ -268,6 +287,35 @@ __global__ void __launch_bounds__(THREADS, 1)
         fence_async_smem();
         warp_arrive(&S_.kz);
       }
+      // float16: what undoes the factors of X's and X2's rows, and of P's columns (one a lane)
+      [[maybe_unused]] float uX = 1.f, uX2 = 1.f, uP = 1.f, uRow = 1.f;
+      if constexpr (!AB16) {
+        const float* f = factors_of(a, w) + R.factors * FX_N;
+        uRow = kside ? f[FX_DV + i] : 1.f;
+        if (warp < 8) {
+          uP = f[FX_E + 32 * (warp >> 2) + lane];
+        } else {
+          uX = uRow * f[FX_S];
+          uX2 = f[FX_E + i] * f[FX_DS];
+        }
+      }
+      // and, once the epilogue's first half has N and W, their factors: every warp passes here once a record.  They are one,
+      // and W is hi + lo, unless N is 4096 times W or more.  Inside an item they only fall, so that what is in F already
+      // stays in range.
+      [[maybe_unused]] float turn = 1.f, sF = 1.f;
+      [[maybe_unused]] auto factors = [&] {
+        bar_sync<1, EPI>();
+        const float n = fmaxf(fmaxf(S_.top[0], S_.top[1]), fmaxf(S_.top[4], S_.top[5]));
+        const float t = fmaxf(fmaxf(S_.top[2], S_.top[3]), fmaxf(S_.top[6], S_.top[7]));
+        const float before = kside ? sN : sW;
+        sN = fminf(pow2_of(fmaxf(n, t)).s, R.first ? 0x1p40f : sN);
+        sW = fminf(pow2_of(t).s, R.first ? 0x1p40f : sW);
+        apart = sW > 4096.f * sN;
+        if (!apart) sW = sN;
+        if (tid == 0) S_.apart = apart;
+        sF = kside ? sN : sW;
+        turn = sF / before;
+      };
       pipe_wait(warp < 8 ? &S_.p_full : &S_.x_full, rec & 1, ab, err, 0x200);
       tc_fence_after();
       float z[32];
@@ -275,7 +323,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         // [N ; W] and the scores' part of dbeta, columns c0 .. c0 + 31
         const int c0 = 32 * (warp >> 2);
         const uint32_t row = sb + L_W + (kside ? 0 : PANEL);
-        if (c0 > (quad & 1) * 32) {  // the block above the diagonal
+        const bool above = c0 > (quad & 1) * 32;  // the block above the diagonal
+        auto zero = [&] {
 #pragma unroll
           for (int cc = 0; cc < 4; ++cc) {
             sts128(row + sw128(i, c0 / 8 + cc), make_uint4(0, 0, 0, 0));
@@ -283,41 +332,99 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
 #pragma unroll
           for (int e = 0; e < 32; ++e) z[e] = 0.f;
-        } else {
-          const float gh[2] = {ax[AX_GH + i], ax[AX_GH + i]}, gl[2] = {ax[AX_GL + i], ax[AX_GL + i]};
-          const float sx[2] = {kside ? -1.f : a.scale, kside ? -1.f : a.scale}, m1[2] = {-1.f, -1.f};
-          const int top = i < valid ? (kside ? i - 1 : i) : -1;  // last column of this row
+        };
+        if constexpr (AB16) {
+          if (above) {
+            zero();
+          } else {
+            const float gh[2] = {ax[AX_GH + i], ax[AX_GH + i]}, gl[2] = {ax[AX_GL + i], ax[AX_GL + i]};
+            const float sx[2] = {kside ? -1.f : a.scale, kside ? -1.f : a.scale}, m1[2] = {-1.f, -1.f};
+            const int top = i < valid ? (kside ? i - 1 : i) : -1;  // last column of this row
 #pragma unroll
-          for (int cc = 0; cc < 4; ++cc) {
-            float x[8], y[8];
-            tmem_ld8x2(tl + T_P + c0 + 8 * cc, tl + T_B + c0 + 8 * cc, x, y);
+            for (int cc = 0; cc < 4; ++cc) {
+              float x[8], y[8];
+              tmem_ld8x2(tl + T_P + c0 + 8 * cc, tl + T_B + c0 + 8 * cc, x, y);
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const int j = c0 + 8 * cc + e;
-              float d[2], l[2];
-              fma2(d, ax + AX_GH + j, m1, gh);
-              fma2(l, ax + AX_GL + j, m1, gl);
-              add2f(d, d, l);
-              d[0] = ex2(d[0]);
-              d[1] = ex2(d[1]);
-              mul2f(x + e, x + e, sx);
-              mul2f(d, d, x + e);
-              d[0] = j <= top ? d[0] : 0.f;  // the masked places can hold anything
-              d[1] = j < top ? d[1] : 0.f;
-              mul2f(z + 8 * cc + e, d, y + e);
-              mul2f(x + e, d, ax + AX_B + j);
+              for (int e = 0; e < 8; e += 2) {
+                const int j = c0 + 8 * cc + e;
+                float d[2], l[2];
+                fma2(d, ax + AX_GH + j, m1, gh);
+                fma2(l, ax + AX_GL + j, m1, gl);
+                add2f(d, d, l);
+                d[0] = ex2(d[0]);
+                d[1] = ex2(d[1]);
+                mul2f(x + e, x + e, sx);
+                mul2f(d, d, x + e);
+                d[0] = j <= top ? d[0] : 0.f;  // the masked places can hold anything
+                d[1] = j < top ? d[1] : 0.f;
+                mul2f(z + 8 * cc + e, d, y + e);
+                mul2f(x + e, d, ax + AX_B + j);
+              }
+              uint32_t u[4], lo[4];
+              split<AB16, 4>(x, u, lo);
+              sts128(row + sw128(i, c0 / 8 + cc), make_uint4(u[0], u[1], u[2], u[3]));
+              if (!kside) sts128(row + PANEL + sw128(i, c0 / 8 + cc), make_uint4(lo[0], lo[1], lo[2], lo[3]));
             }
-            uint32_t u[4], lo[4];
-            split<AB16, 4>(x, u, lo);
-            sts128(row + sw128(i, c0 / 8 + cc), make_uint4(u[0], u[1], u[2], u[3]));
-            if (!kside) sts128(row + PANEL + sw128(i, c0 / 8 + cc), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+          }
+        } else {
+          float m = 0.f;
+          if (above) {
+            zero();
+          } else {
+            const int top = i < valid ? (kside ? i - 1 : i) : -1;
+            const float gh = ax[AX_GH + i], gl = ax[AX_GL + i], sx = kside ? -uRow : a.scale;
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc) {
+              float* d = z + 8 * cc;
+              tmem_ld8(tl + T_P + c0 + 8 * cc, d);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const int j = c0 + 8 * cc + e;
+                d[e] *= ex2((gh - ax[AX_GH + j]) + (gl - ax[AX_GL + j])) * (sx * __shfl_sync(0xffffffffu, uP, 8 * cc + e));
+                d[e] = j <= top ? d[e] : 0.f;  // the masked places can hold anything
+                m = fmaxf(m, fabsf(d[e] * ax[AX_B + j]));
+              }
+            }
+          }
+          m = warp_max(m);
+          if (lane == 0) S_.top[warp] = m;
+          factors();
+          if (!above) {
+#pragma unroll
+            for (int cc = 0; cc < 4; ++cc) {
+              float x[8], y[8];
+              uint32_t u[4];
+              tmem_ld8(tl + T_B + c0 + 8 * cc, y);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = z[8 * cc + e] * ax[AX_B + c0 + 8 * cc + e];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) z[8 * cc + e] *= y[e];
+              uint32_t lo[4];
+              float xs[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) xs[e] = x[e] * sF;
+              split<AB16, 4>(xs, u, lo);
+              sts128(row + sw128(i, c0 / 8 + cc), make_uint4(u[0], u[1], u[2], u[3]));
+              if (!kside) {
+                if (apart) {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) lo[e] = pack2<AB16>(x[2 * e] * sN, x[2 * e + 1] * sN);
+                }
+                sts128(row + PANEL + sw128(i, c0 / 8 + cc), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+              }
+            }
           }
         }
       } else {
         // the first term of F, half of its columns, and k_i . X2_i
         constexpr int KH = KD / 2;
         const int hf = (warp - 8) >> 2;
-        const float r0 = kside ? -ax[AX_G + i] : ax[AX_SG + i], r1 = ax[AX_WB + i];
+        float r0 = kside ? -ax[AX_G + i] : ax[AX_SG + i], r1 = ax[AX_WB + i];
+        if constexpr (!AB16) {
+          factors();
+          r0 *= uX * sF;
+          r1 *= uX2 * sF;
+        }
         const float g0[2] = {r0, r0}, g1[2] = {r1, r1};
         float ke[2] = {0.f, 0.f};
 #pragma unroll
@@ -352,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             float y[16];
             tmem_ld16(tl + T_F + k, y);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] += y[e];
+            for (int e = 0; e < 16; ++e) x[e] = AB16 ? x[e] + y[e] : fmaf(y[e], turn, x[e]);
           }
           uint32_t u[16];
 #pragma unroll
@@ -360,7 +467,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           tmem_st8(tl + T_F + k, u);
           tmem_st8(tl + T_F + k + 8, u + 8);
         }
-        if (kside) S_.ke[hf][i] = ke[0] + ke[1];
+        if (kside) S_.ke[hf][i] = AB16 ? ke[0] + ke[1] : (ke[0] + ke[1]) * uX2;
         tmem_st_wait();
       }
       fence_async_smem();
@@ -381,6 +488,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (R.last) {
         // dK over the K rows and dQ over the Q rows, then out
         constexpr int KQTR = KD / 4;
+        [[maybe_unused]] const float back = 1.f / sF;
         const int k0 = KQTR * (warp >> 2);
 #pragma unroll
         for (int k = k0; k < k0 + KQTR; k += 16) {
@@ -388,7 +496,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           tmem_ld16(tl + T_F + k, x);
           uint32_t u[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) u[e] = pack2<AB16>(x[2 * e], x[2 * e + 1]);
+          for (int e = 0; e < 8; ++e) u[e] = AB16 ? pack2<AB16>(x[2 * e], x[2 * e + 1]) : pack2<AB16>(x[2 * e] * back, x[2 * e + 1] * back);
           const uint32_t p = KQ + (k >> 6) * 2 * PANEL;
           sts128(p + sw128(quad * 32 + lane, (k & 63) >> 3), make_uint4(u[0], u[1], u[2], u[3]));
           sts128(p + sw128(quad * 32 + lane, ((k & 63) >> 3) + 1), make_uint4(u[4], u[5], u[6], u[7]));
@@ -430,9 +538,12 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (warp < 2) {
         const int j = tid;
         const int64_t at = (int64_t)(R.row0 + j) * a.HV + R.hv;
-        if (j < valid)
-          gate_store(a.dbeta, a.beta_dtype, at,
-                     S_.db[0][j] + S_.db[1][j] + S_.db[2][j] + S_.db[3][j] + ax[AX_W + j] * (S_.ke[0][j] + S_.ke[1][j]));
+        float db = S_.db[0][j] + S_.db[1][j] + S_.db[2][j] + S_.db[3][j] + ax[AX_W + j] * (S_.ke[0][j] + S_.ke[1][j]);
+        if constexpr (!AB16) {
+          if (!R.head_first) db += head_db;
+          head_db = db;
+        }
+        if (j < valid && (AB16 || R.head_last)) gate_store(a.dbeta, a.beta_dtype, at, db);
         // dg: reverse running sum; warp 1 holds tokens 32..63, whose sum warp 0 adds
         float x = dot;
 #pragma unroll
@@ -448,7 +559,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         x += rest + (warp == 0 ? S_.dg[16] : 0.f);
         // nothing decays at the first token of a document that starts from a zero state
         if (j == 0 && R.zero_first) x = 0.f;
-        if (j < valid) gate_store(a.dg, a.g_dtype, at, x);
+        if (j < valid && (AB16 || R.head_last)) gate_store(a.dg, a.g_dtype, at, x);
       }
     }
     if (tid == 256) bulk_wait_all();
@@ -466,7 +577,7 @@ cudaError_t launch(const GdrArgs& a, const Ws& w) {
   cudaError_t r = token_map(&q, a, a.q, a.H, a.K);
   if (r == cudaSuccess) r = token_map(&k, a, a.k, a.H, a.K);
   if (r == cudaSuccess) r = token_map(&o, a, a.d_o, a.HV, a.V);
-  if (r == cudaSuccess) r = token_map(&dv, a, a.dv, a.HV, a.V);
+  if (r == cudaSuccess) r = token_map(&dv, a, AB16 ? a.dv : scaled_dv_of(a, w), a.HV, a.V);
   if (r == cudaSuccess) r = matrix_map(&e, a, w.E, 2 * C, sh);
   if (r == cudaSuccess) r = matrix_map(&s, a, w.S0, a.K, sh);
   if (r == cudaSuccess) r = matrix_map(&ds, a, w.dS1, a.K, sh);

@@ -2,7 +2,8 @@
 //
 //   T = (1 + strict(D_ij k_i.k_j beta_j))^{-1}    P beta = scale tril(D_ij q_i.k_j) beta_j    D_ij = e^{G_i - G_j}
 //
-// as hi + lo pairs of 16-bit matrices in the swizzled layout the scans' MMAs read, and the per-token factors.
+// as hi + lo pairs of 16-bit matrices in the swizzled layout the scans' MMAs read, and the per-token factors.  The pairs
+// are bfloat16 for either type of input; for float16 a second pair of P beta, in that type, goes straight to memory.
 //
 // One block of four warps per chunk and value head.  The rows come by TMA; k k^T and q k^T (operands the
 // inputs themselves, fp32 sums) run on mma.sync, whose fragments are where the elementwise step wants
@@ -11,7 +12,7 @@
 // T_21 = -T_22 A_21 T_11 for 16- and for 32-row blocks as three-term TF32 products (2^-21).  What bounds the
 // kernel is latency, six short stages with barriers between them: 1.65 instructions a cycle with the five blocks
 // that fit an SM.  8192 (chunk, head) pairs of K = 128 take 140 us, where their 540 MB alone would take 83.
-// (Bands of 16 rows that rotate over the warps, to even out the schedulers: no change.)
+// (Bands of 16 rows that rotate over the warps, to even out the schedulers: no change.)  float16: 162 us, 16 KB more written.
 #include "gdr_tc.cuh"
 
 namespace ccq {
@@ -81,6 +82,7 @@ __device__ __forceinline__ void put(const float (*d)[4], float sign, float* out,
 struct Small {
   uint64_t full;
   float gh[C], gl[C], beta[C];  // G log2(e) as hi + lo
+  float pb, top[2][4];          // float16: largest |scale D beta| (a bound); largest |k|^2 and |q_x| of each warp
 };
 
 // The rows (up to 32 KB) make room, once read, for A and for the images of P; the images of T then replace
@@ -92,7 +94,7 @@ constexpr uint32_t BYTES = OFF_S + sizeof(Small) + 1024;
 static_assert(2 * TILE <= OFF_X, "rows fit");
 
 template <int AB16, int KD>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(128, 5)
     prep_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk, GdrArgs a, Ws w) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -152,7 +154,26 @@ __global__ void __launch_bounds__(128)
       ax[AX_WB + t] = wt * b[j];
       ax[AX_W + t] = wt;
     }
-    if (lane < AX_N - AX_GC) ax[AX_GC + lane] = lane == 0 ? ex2((float)last) : 0.f;
+    if constexpr (!AB16) {
+      const float top = warp_max(fmaxf(ex2((float)Gs[0]), ex2((float)Gs[1])));
+      // the largest G_i - G_j, j <= i, from the smallest G of the lanes before
+      const float G0 = (float)Gs[0], G1 = (float)Gs[1];
+      float low = fminf(G0, G1);
+      const float bt = warp_max(fmaxf(fabsf(b[0]), fabsf(b[1])));
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const float u = __shfl_up_sync(0xffffffffu, low, o);
+        if (lane >= o) low = fminf(low, u);
+      }
+      low = __shfl_up_sync(0xffffffffu, low, 1);
+      low = lane == 0 ? G0 : fminf(low, G0);
+      const float rise = warp_max(fmaxf(G0 - low, G1 - fminf(low, G1)));
+      if (lane == 0) {
+        ax[AX_SM] = fabsf(a.scale) * top;
+        S.pb = fabsf(a.scale) * bt * ex2(rise);
+      }
+    }
+    if (lane < (AB16 ? AX_N - AX_GC : 1)) ax[AX_GC + lane] = lane == 0 ? ex2((float)last) : 0.f;
   }
   __syncthreads();
   // the copy's bytes always arrive; the bound only keeps a broken launch from hanging
@@ -160,8 +181,10 @@ __global__ void __launch_bounds__(128)
     if (tid == 0) atomicOr(w.err, 0x100000);
     return;
   }
+  auto top = [&](int x) { return fmaxf(fmaxf(S.top[x][0], S.top[x][1]), fmaxf(S.top[x][2], S.top[x][3])); };
   // rows 16 warp .. +15 of k k^T and q k^T, columns up to the diagonal
   float kk[8][4] = {}, qk[8][4] = {};
+  [[maybe_unused]] uint32_t qm[2] = {0, 0};  // float16: largest |q_x| of rows (lane >> 2) and + 8, in pairs
   {
     const uint32_t r = 16 * warp + (lane & 15), ac = lane >> 4;                  // A fragments: row, 16-byte chunk
     const uint32_t br = (lane & 7) + ((lane >> 4) << 3), bc = (lane >> 3) & 1;   // B fragments of two 8-column tiles
@@ -171,6 +194,10 @@ __global__ void __launch_bounds__(128)
       const uint32_t p = (ks >> 2) * PANEL, ch = (ks & 3) * 2;
       ldsm4(fk, sk + p + sw128(r, ch + ac));
       ldsm4(fq, sq_ + p + sw128(r, ch + ac));
+      if constexpr (!AB16) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qm[e & 1] = max2_f16(qm[e & 1], fq[e] & 0x7FFF7FFFu);
+      }
 #pragma unroll
       for (int np = 0; np < 4; ++np) {
         if (np <= warp) {
@@ -184,7 +211,36 @@ __global__ void __launch_bounds__(128)
       }
     }
   }
+  if constexpr (!AB16) {
+    const int i0 = 16 * warp + (lane >> 2);
+    float kn = 0.f, qn = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = i0 + 8 * (e >> 1), j = 8 * nt + 2 * (lane & 3) + (e & 1);
+        if (j == i && i < valid) kn = fmaxf(kn, kk[nt][e]);
+      }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float2 x = unpack2<AB16>(qm[e]);
+      if (i0 + 8 * e < valid) qn = fmaxf(qn, fmaxf(x.x, x.y));
+    }
+    kn = warp_max(kn);
+    qn = warp_max(qn);
+    if (lane == 0) {
+      S.top[0][warp] = kn;
+      S.top[1][warp] = qn;
+    }
+  }
   __syncthreads();  // the rows are read: their space becomes A and the images of P
+  Pow2 fp{1.f, 1.f};
+  if constexpr (!AB16) {
+    const float kn = sqrtf(top(0)), qn = top(1) * sqrtf((float)KD);
+    fp = pow2_of(S.pb * kn * qn);
+    if (tid < 3) w.aux[sh * AX_N + AX_UP + tid] = tid == 0 ? fp.u : tid == 1 ? kn : qn;
+  }
+  uint8_t* p16 = w.mats + sh * mats_bytes(AB16) + MATS;
   {
     const int i0 = 16 * warp + (lane >> 2);
     const float gh[2] = {S.gh[i0], S.gh[i0 + 8]}, gl[2] = {S.gl[i0], S.gl[i0 + 8]};
@@ -197,6 +253,7 @@ __global__ void __launch_bounds__(128)
           const uint32_t at = sw128(i0 + 8 * hr, nt) + (lane & 3) * 4;
           *reinterpret_cast<uint32_t*>(sm + OFF_P + at) = 0;
           *reinterpret_cast<uint32_t*>(sm + OFF_P + PANEL + at) = 0;
+          if (!AB16) *reinterpret_cast<uint32_t*>(p16 + at) = *reinterpret_cast<uint32_t*>(p16 + PANEL + at) = 0;
           *reinterpret_cast<float2*>(A + (i0 + 8 * hr) * LDA + j0) = make_float2(0.f, 0.f);
         }
         continue;
@@ -214,10 +271,16 @@ __global__ void __launch_bounds__(128)
         *reinterpret_cast<float2*>(A + i * LDA + j0) = make_float2(a0, a1);
         const float p[2] = {p0, p1};
         uint32_t hi, lo;
-        split<AB16, 1>(p, &hi, &lo);
+        split<1, 1>(p, &hi, &lo);
         const uint32_t at = sw128(i, nt) + (lane & 3) * 4;
         *reinterpret_cast<uint32_t*>(sm + OFF_P + at) = hi;
         *reinterpret_cast<uint32_t*>(sm + OFF_P + PANEL + at) = lo;
+        if constexpr (!AB16) {
+          const float ps[2] = {p0 * fp.s, p1 * fp.s};
+          split<0, 1>(ps, &hi, &lo);
+          *reinterpret_cast<uint32_t*>(p16 + at) = hi;
+          *reinterpret_cast<uint32_t*>(p16 + PANEL + at) = lo;
+        }
       }
     }
   }
@@ -279,7 +342,7 @@ __global__ void __launch_bounds__(128)
     for (int cc = 0; cc < 4; ++cc) {
       const float4 u = *reinterpret_cast<const float4*>(row + 8 * cc), v = *reinterpret_cast<const float4*>(row + 8 * cc + 4);
       const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-      split<AB16, 4>(x, hi + 4 * cc, lo + 4 * cc);
+      split<1, 4>(x, hi + 4 * cc, lo + 4 * cc);
     }
     __syncthreads();
 #pragma unroll
@@ -292,7 +355,7 @@ __global__ void __launch_bounds__(128)
   fence_async_smem();
   __syncthreads();
   if (tid == 0) {
-    uint8_t* dst = w.mats + sh * MATS;
+    uint8_t* dst = w.mats + sh * mats_bytes(AB16);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + i * 2 * PANEL),

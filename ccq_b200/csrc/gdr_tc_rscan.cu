@@ -13,7 +13,8 @@
 // Written out: dV, V . dV per token, for the gradient kernel dS (16-bit, transposed) of every chunk, and every
 // ANCHOR chunks <dS, S>.
 // Bound, as the scan, by the latency of one chunk's chain: 8 x 4096 tokens, 16 heads, K = V = 128 take 333 us,
-// 5.2 us a chunk.  TMEM columns: dS hi, lo
+// 5.2 us a chunk.  float16 422 us: the two terms of D have factors of their own and are read one after the other, dV is
+// also written with a factor a token, and the instructions for both stand in the chain.  TMEM columns: dS hi, lo
 // (64 each), Y and Z (64 each), then dV (128), D (128), dE, then Gam dV as operand (64), scaled dO (64).
 #include "gdr_tc.cuh"
 
@@ -26,7 +27,11 @@ constexpr uint32_t T_SH = 0, T_SL = 64, T_Y = 128, T_Z = 192, T_D = 256, T_EH = 
 
 struct Small {
   uint64_t full[2], empty[2], s_ready, y_full, e_ready, f_full, f_ready, f_read, g_ready, d_full, kz, done;
+  uint64_t d1_full, d1_read;  // float16: the first product of D^T
   float red[4][C];
+  alignas(16) float top[2][16];  // float16: largest dS and Gam dV of each chain warp
+  alignas(16) float vtop[4][C];  // largest dV of each token, by quadrant
+  float undo[2];      // by the chunk's parity: what undoes the factor of the scaled dO
   uint32_t tmem;
   int abort;
 };
@@ -43,7 +48,8 @@ template <int AB16, int KD, bool SUM>
 __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
     rscan_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
                  const __grid_constant__ CUtensorMap tmv, const __grid_constant__ CUtensorMap tmo,
-                 const __grid_constant__ CUtensorMap tmdv, const __grid_constant__ CUtensorMap tms, GdrArgs a, Ws w) {
+                 const __grid_constant__ CUtensorMap tmdv, const __grid_constant__ CUtensorMap tms,
+                 const __grid_constant__ CUtensorMap tmdvs, GdrArgs a, Ws w) {
   using G = BwdWarps;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -82,6 +88,8 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
     mbar_init(&S_.f_full, 1);
     mbar_init(&S_.d_full, 1);
     mbar_init(&S_.done, 1);
+    mbar_init(&S_.d1_full, 1);
+    mbar_init(&S_.d1_read, G::CHAIN_WARPS);
     S_.abort = 0;
     fence_barrier_init();
   }
@@ -112,7 +120,13 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
         tma_load_3d(p + L_DO, &tmo, bar, v0, hv, row);
         tma_load_3d(p + L_DO + PANEL, &tmo, bar, v0 + 64, hv, row);
         bulk_load(p + L_AX, w.aux + sh * AX_N, AX_N * 4, bar);
-        bulk_load(p + L_M, w.mats + sh * MATS, MATS, bar);
+        const uint8_t* mats = w.mats + sh * mats_bytes(AB16);
+        if (AB16) {
+          bulk_load(p + L_M, mats, MATS, bar);
+        } else {  // T, and P beta in float16
+          bulk_load(p + L_M, mats, MATS / 2, bar);
+          bulk_load(p + L_M + MATS / 2, mats + MATS, MATS / 2, bar);
+        }
         for (int i = 0; i < NP; ++i) tma_load_3d(p + L_KQ + (2 * i + 1) * PANEL, &tmq, bar, 64 * i, h, row);
         if (!SUM) {
           tma_load_3d(p + L_V, &tmv, bar, v0, hv, row);
@@ -127,8 +141,8 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
     // ------------------------------------------------------------------ MMA issuer
     if (lane == 0) {
       const uint32_t id_y = idesc_f16(128, 64, AB16, 0, 0), id_z = idesc_f16(128, 64, AB16, 1, 1);
-      const uint32_t id_d = idesc_f16(128, KD, AB16, 0, 1), id_f = idesc_f16(128, 128, AB16, 0, 1);
-      const uint32_t id_f2 = idesc_f16(128, 64, AB16, 0, 1);
+      const uint32_t id_d = idesc_f16(128, KD, AB16, 0, 1);
+      const uint32_t id_f = idesc_f16(128, 128, 1, 0, 1), id_f2 = idesc_f16(128, 64, 1, 0, 1);  // T is bfloat16
       for (int t = 0; t < nch; ++t) {
         const int s = t & 1, ph = t & 1;
         const uint32_t p = sb + s * L_STAGE;
@@ -172,6 +186,10 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
           for (int ks = 0; ks < 4; ++ks)
             umma_ts(tb + T_D, tb + (x ? T_GL : T_GH) + 8 * ks, sdesc(p + L_KQ + PANEL + ks * 2048, 2 * PANEL, 1024), id_d,
                     x + ks > 0);
+        if (!AB16) {  // the next product has a factor of its own: this one is read first
+          umma_commit(&S_.d1_full);
+          if (!spin_wait(&S_.d1_read, ph, ab, err, 0x100)) break;
+        }
         // D^T += (-Gam dV)^T K
         if (!spin_wait(&S_.f_ready, ph, ab, err, 0x200)) break;
         tc_fence_after();
@@ -179,7 +197,8 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
-            umma_ts(tb + T_D, tb + (x ? T_EL : T_EH) + 8 * ks, sdesc(p + L_KQ + ks * 2048, 2 * PANEL, 1024), id_d, 1);
+            umma_ts(tb + T_D, tb + (x ? T_EL : T_EH) + 8 * ks, sdesc(p + L_KQ + ks * 2048, 2 * PANEL, 1024), id_d,
+                    AB16 || x + ks > 0);
         umma_commit(&S_.d_full);
         umma_commit(&S_.empty[s]);
       }
@@ -202,13 +221,31 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
       const int k = KH * hh + i;
       S[i] = (last && vin && k < a.K) ? last[(int64_t)k * a.V + v0 + vl] : 0.f;
     }
+    const int cw = warp - G::CHAIN;
+    [[maybe_unused]] float* fx = factors_of(a, w) + ((int64_t)vt * gdr_slots(a, C) * a.HV + sh0) * FX_N;  // of the first chunk
+    float uS = 1.f, bS = 0.f;  // float16: what undoes the factor of dS, and a bound on dS
     // dS as the operand of chunk c; its hi part also goes to `tile` (two panels of 128 rows), or straight
     // to the workspace for the first chunk
-    auto put_state = [&](uint32_t tile) {
+    auto put_state = [&](uint32_t tile, int c) {
+      Pow2 f{1.f, 1.f};
+      if constexpr (!AB16) {
+        if ((nch - 1 - c) % EXACT == 0) bS = warps_max<2, G::CHAIN_WARPS>(abs_max<KH>(S), S_.top[0], cw);
+        f = pow2_of(bS);
+        uS = f.u;
+        if (!SUM && threadIdx.x == 32 * G::CHAIN) fx[(int64_t)c * a.HV * FX_N + FX_DS] = f.u;
+      }
 #pragma unroll
       for (int i = 0; i < KH; i += 16) {
         uint32_t hi[8], lo[8];
-        split<AB16, 8>(S + i, hi, lo);
+        if constexpr (AB16) {
+          split<AB16, 8>(S + i, hi, lo);
+        } else {
+          float x[16];
+          const float ss[2] = {f.s, f.s};
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) mul2f(x + j, S + i + j, ss);
+          split<AB16, 8>(x, hi, lo);
+        }
         tmem_st8(tl + T_SH + hh * (KH / 2) + i / 2, hi);
         tmem_st8(tl + T_SL + hh * (KH / 2) + i / 2, lo);
         const int k = KH * hh + i;
@@ -242,7 +279,7 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
       if (lane == 0) w.anchor[((int64_t)vt * anchors * a.HV + at) * G::CHAIN_WARPS + warp - G::CHAIN] = d;
     };
     if (nch > 0) {
-      put_state(0);
+      put_state(0, nch - 1);
       if (!SUM && part.last()) put_anchor((part.nch - 1) / ANCHOR, a.dfinal_state == nullptr);
     }
     const int i0 = CT * hh;
@@ -252,30 +289,52 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
       pipe_wait(&S_.full[s], (t >> 1) & 1, ab, err, 0x400);
       pipe_wait(&S_.y_full, ph, ab, err, 0x800);
       tc_fence_after();
+      if constexpr (AB16) {
 #pragma unroll
-      for (int i = 0; i < CT; i += 16) {
+        for (int i = 0; i < CT; i += 16) {
+          float x[16];
+          tmem_ld16(tl + T_Z + i0 + i, x);
+#pragma unroll
+          for (int k = 0; k < 16; k += 8) {
+            float y[8];
+            tmem_ld8(tl + T_Y + i0 + i + k, y);
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+              const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + i + k + j);
+              const float bb[4] = {b.x, b.y, b.z, b.w};
+              float* z = x + k + j;
+              fma2(z, bb, y + j, z);
+              fma2(z + 2, bb + 2, y + j + 2, z + 2);
+            }
+          }
+          st_split16<AB16>(tl + T_EH + (i0 + i) / 2, tl + T_EL + (i0 + i) / 2, x);
+        }
+      } else {
+        static_assert(CT == 16, "one load");
+        const float uP = ax[AX_UP];
         float x[16];
-        tmem_ld16(tl + T_Z + i0 + i, x);
+        tmem_ld16(tl + T_Z + i0, x);
 #pragma unroll
         for (int k = 0; k < 16; k += 8) {
           float y[8];
-          tmem_ld8(tl + T_Y + i0 + i + k, y);
+          tmem_ld8(tl + T_Y + i0 + k, y);
 #pragma unroll
           for (int j = 0; j < 8; j += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + i + k + j);
-            const float bb[4] = {b.x, b.y, b.z, b.w};
-            float* z = x + k + j;
-            fma2(z, bb, y + j, z);
-            fma2(z + 2, bb + 2, y + j + 2, z + 2);
+            const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + k + j);
+            x[k + j] = fmaf(b.x * uS, y[j], x[k + j] * uP);
+            x[k + j + 1] = fmaf(b.y * uS, y[j + 1], x[k + j + 1] * uP);
+            x[k + j + 2] = fmaf(b.z * uS, y[j + 2], x[k + j + 2] * uP);
+            x[k + j + 3] = fmaf(b.w * uS, y[j + 3], x[k + j + 3] * uP);
           }
         }
-        st_split16<AB16>(tl + T_EH + (i0 + i) / 2, tl + T_EL + (i0 + i) / 2, x);
+        st_split16<1>(tl + T_EH + i0 / 2, tl + T_EL + i0 / 2, x);
       }
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.e_ready);
       pipe_wait(&S_.f_full, ph, ab, err, 0x1000);
       tc_fence_after();
+      [[maybe_unused]] float uG[2] = {1.f, 1.f};  // float16: what undoes the factor of Gam dV
 #pragma unroll
       for (int i = 0; i < CT; i += 16) {
         float x[16];
@@ -295,12 +354,40 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
             mul2f(z + 2, z + 2, bb + 2);
           }
         }
+        if constexpr (!AB16) {
+          const float m = warps_max<2, G::CHAIN_WARPS>(abs_max<16>(x), S_.top[1], cw);
+          const Pow2 f = pow2_of(m);
+          const float ss[2] = {f.s, f.s};
+          uG[0] = uG[1] = f.u;
+          bS = fmaf(64.f * ax[AX_KN], m, ax[AX_GC] * bS);
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) mul2f(x + j, x + j, ss);
+        }
         st_split16<AB16>(tl + T_EH + (i0 + i) / 2, tl + T_EL + (i0 + i) / 2, x);
       }
       const float gam[2] = {ax[AX_GC], ax[AX_GC]};
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.f_ready);
+      if constexpr (!AB16) {  // dS = Gam_C dS + the first product
+        pipe_wait(&S_.d1_full, ph, ab, err, 0x2000);
+        pipe_wait(&S_.g_ready, ph, ab, err, 0x2000);  // the factor was left before; the phase lasts until d1_read of this chunk
+        tc_fence_after();
+        const float u = S_.undo[t & 1], uo[2] = {u, u};
+        bS = fmaf(64.f * ax[AX_QN], 32768.f * u, bS);
+#pragma unroll
+        for (int i = 0; i < KH; i += 16) {
+          float x[16];
+          tmem_ld16(tl + T_D + KH * hh + i, x);
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            mul2f(x + j, x + j, uo);
+            fma2(S + i + j, gam, S + i + j, x + j);
+          }
+        }
+        tc_fence_before();
+        warp_arrive(&S_.d1_read);
+      }
       if (warp != G::CHAIN) warp_arrive(&S_.empty[s]);
       pipe_wait(&S_.d_full, ph, ab, err, 0x2000);
       tc_fence_after();
@@ -309,9 +396,12 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
         float x[16];
         tmem_ld16(tl + T_D + KH * hh + i, x);
 #pragma unroll
-        for (int j = 0; j < 16; j += 2) fma2(S + i + j, gam, S + i + j, x + j);
+        for (int j = 0; j < 16; j += 2) {
+          if constexpr (AB16) fma2(S + i + j, gam, S + i + j, x + j);
+          else fma2(S + i + j, uG, x + j, S + i + j);
+        }
       }
-      if (c > 0) put_state(sb + s * L_STAGE + L_KQ);  // every product with the K and Q rows is done: their space is the staging
+      if (c > 0) put_state(sb + s * L_STAGE + L_KQ, c - 1);  // every product with the K and Q rows is done: their space is the staging
       fence_async_smem();
       bar_sync<2, G::CHAIN_THREADS>();
       if (threadIdx.x == 32 * G::CHAIN) {
@@ -339,6 +429,8 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
     const int vl = quad * 32 + lane;
     const uint32_t tl = tb + ((uint32_t)(quad * 32) << 16);
     const int64_t slots = gdr_slots(a, C);
+    [[maybe_unused]] float* fx = factors_of(a, w) + ((int64_t)vt * slots * a.HV + sh0) * FX_N;  // of the first chunk
+    [[maybe_unused]] float top = !AB16 && nch > 0 ? fx[(int64_t)(nch - 1) * a.HV * FX_N + FX_DO] : 0.f;
     for (int t = 0; t < nch; ++t) {
       const int s = t & 1, ph = t & 1, c = nch - 1 - t;
       const int valid = min(C, sq.len - c * C);
@@ -355,6 +447,12 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
       }
       if (t > 0) pipe_wait(&S_.d_full, (t - 1) & 1, ab, err, 0x8000);  // the operand of the chunk before is read
       tc_fence_after();
+      Pow2 fo{1.f, 1.f};
+      if constexpr (!AB16) {  // from a bound: largest |dO|, which the forward scan left, by the largest scale Gam
+        fo = pow2_of(ax[AX_SM] * top);
+        if (threadIdx.x == 0) S_.undo[t & 1] = fo.u;
+        top = c > 0 ? fx[(int64_t)(c - 1) * a.HV * FX_N + FX_DO] : 0.f;
+      }
       {
         const Column D(p + L_DO, vl);
 #pragma unroll
@@ -365,7 +463,10 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
             const float4 b = *reinterpret_cast<const float4*>(ax + AX_SG + i + j);
             const float bb[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[j + e] = i + j + e < valid ? bb[e] * h2f<AB16>(lds16(D.at(i + j + e))) : 0.f;
+            for (int e = 0; e < 4; ++e) {
+              x[j + e] = i + j + e < valid ? bb[e] * h2f<AB16>(lds16(D.at(i + j + e))) : 0.f;
+              if (!AB16) x[j + e] *= fo.s;
+            }
           }
           st_split16<AB16>(tl + T_GH + i / 2, tl + T_GL + i / 2, x);
         }
@@ -390,14 +491,29 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
       }
       tc_fence_before();
       warp_arrive(&S_.f_read);
+      if (!AB16) token_max_put<OT>(y, S_.vtop, j0, quad, lane);
       if (threadIdx.x == 0) bulk_wait_read();  // the stores of the chunk before have read the tile
       bar_sync<1, G::OUT_THREADS>();
       const Column O(sb + L_OUT, vl), V(p + L_V, vl);
 #pragma unroll
       for (int i = 0; i < OT; ++i) sts16(O.at(j0 + i), f2h<AB16>(y[i]));
+      if constexpr (AB16) {
 #pragma unroll
-      for (int i = 0; i < OT; ++i) y[i] = j0 + i < valid ? y[i] * h2f<AB16>(lds16(V.at(j0 + i))) : 0.f;
-      warp_arrive(&S_.empty[s]);
+        for (int i = 0; i < OT; ++i) y[i] = j0 + i < valid ? y[i] * h2f<AB16>(lds16(V.at(j0 + i))) : 0.f;
+        warp_arrive(&S_.empty[s]);
+      } else {  // dV with its factor, for the gradient kernel, takes the place of V
+        static_assert(OT == 32, "a token a lane");
+        const Pow2 f = pow2_of(token_max_get(S_.vtop, j0 + lane));
+        if (quad == 0) fx[(int64_t)c * a.HV * FX_N + FX_DV + j0 + lane] = f.u;
+#pragma unroll
+        for (int i = 0; i < OT; ++i) {
+          const uint32_t at = V.at(j0 + i);
+          const float v = h2f<AB16>(lds16(at));
+          sts16(at, f2h<AB16>(y[i] * __shfl_sync(0xffffffffu, f.s, i)));
+          y[i] = j0 + i < valid ? y[i] * v : 0.f;
+        }
+        if (warp > 0) warp_arrive(&S_.empty[s]);  // warp 0: once the tile is stored
+      }
       lane_sums<OT>(y, lane);
 #pragma unroll
       for (int i = 0; i < OT / 32; ++i) S_.red[quad][j0 + lane * (OT / 32) + i] = y[i];
@@ -407,10 +523,15 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
         if (threadIdx.x == 0) {
           tma_store_3d(&tmdv, sm + L_OUT, v0, hv, (int)row0);
           if (v0 + 64 < a.V) tma_store_3d(&tmdv, sm + L_OUT + PANEL, v0 + 64, hv, (int)row0);
+          if (!AB16) {
+            tma_store_3d(&tmdvs, sm + s * L_STAGE + L_V, v0, hv, (int)row0);
+            if (v0 + 64 < a.V) tma_store_3d(&tmdvs, sm + s * L_STAGE + L_V + PANEL, v0 + 64, hv, (int)row0);
+          }
           bulk_commit();
         }
       } else {
         copy_rows(sb + L_OUT, reinterpret_cast<uint16_t*>(a.dv), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, G::OUT_THREADS);
+        if (!AB16) copy_rows(p + L_V, scaled_dv_of(a, w), row0, a.HV, hv, a.V, v0, valid, threadIdx.x, G::OUT_THREADS);
       }
       if (threadIdx.x < C) {
         const int i = threadIdx.x;
@@ -418,6 +539,10 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
             S_.red[0][i] + S_.red[1][i] + S_.red[2][i] + S_.red[3][i];
       }
       bar_sync<1, G::OUT_THREADS>();  // the sums are read before the next chunk's are written
+      if (!AB16 && warp == 0) {
+        if (lane == 0) bulk_wait_read();
+        warp_arrive(&S_.empty[s]);
+      }
     }
     if (threadIdx.x == 0) bulk_wait_all();
   }
@@ -429,18 +554,20 @@ __global__ void __launch_bounds__(BwdWarps::THREADS, 1)
 
 template <int AB16, int KD, bool SUM>
 cudaError_t launch(const GdrArgs& a, const Ws& w) {
-  CUtensorMap q, k, v, o, dv, st;
+  CUtensorMap q, k, v, o, dv, st, dvs;
   cudaError_t e = token_map(&q, a, a.q, a.H, a.K);
   if (e == cudaSuccess) e = token_map(&k, a, a.k, a.H, a.K);
   if (e == cudaSuccess) e = token_map(&v, a, a.v, a.HV, a.V);
   if (e == cudaSuccess) e = token_map(&o, a, a.d_o, a.HV, a.V);
   if (e == cudaSuccess) e = token_map(&dv, a, a.dv, a.HV, a.V);
   if (e == cudaSuccess) e = matrix_map(&st, a, w.dS1, a.K, gdr_slots(a, C) * a.HV);
+  dvs = dv;
+  if (!AB16 && e == cudaSuccess) e = token_map(&dvs, a, scaled_dv_of(a, w), a.HV, a.V);
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(rscan_kernel<AB16, KD, SUM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L_BYTES);
   if (e != cudaSuccess) return e;
   const int64_t blocks = (int64_t)a.n_seqs * a.HV * w.nseg * ((a.V + VT - 1) / VT);
-  rscan_kernel<AB16, KD, SUM><<<(unsigned)blocks, BwdWarps::THREADS, L_BYTES, a.stream>>>(q, k, v, o, dv, st, a, w);
+  rscan_kernel<AB16, KD, SUM><<<(unsigned)blocks, BwdWarps::THREADS, L_BYTES, a.stream>>>(q, k, v, o, dv, st, dvs, a, w);
   return cudaGetLastError();
 }
 

@@ -17,6 +17,10 @@
 // of its own (beside the chain) and the factors by packed two-value arithmetic.  8 x 4096 tokens, 16 heads,
 // K = V = 128: 233 us, 3.6 us a chunk; 331 us with what the backward reads (BWD), 256 MB more written.
 //
+// float16 (its factors: gdr_tc.cuh): the chain warps form R = V - Gam X, and E^T = R^T T^T is one product in bfloat16.
+// What the factors cost is instructions of the chain warps and their barriers: 287 us, and 439 us for the backward, where E
+// is staged behind S, beside the next chunk's first product, since its tokens' factors take a barrier of their own.
+//
 // BWD: instead of O it writes what the backward reads: S0 (16-bit, transposed), E (hi + lo), dO . O and,
 // every ANCHOR chunks, S in fp32.
 //
@@ -36,6 +40,10 @@ constexpr uint32_t T_SH = 0, T_SL = 64, T_X = 128, T_D = 256, T_RH = 384, T_RL =
 struct Small {
   uint64_t full[2], empty[2], s_ready, x_full, r_ready, u_full, u_ready, d_full, o1_read, o_full, o2_free, kz, done;
   float red[4][C];
+  alignas(16) float top[2][16];  // float16: largest S and w beta E of each chain warp
+  alignas(16) float etop[4][C];  // largest E of each token, by quadrant
+  float dtop[8];              // largest dO of each output warp
+  float undo[2];        // by the chunk's parity: what undoes the factor of S
   uint32_t tmem;
   int abort;
 };
@@ -133,7 +141,7 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
           tma_load_3d(p + L::V + PANEL, &tmv, bar, v0 + 64, hv, row);
         }
         bulk_load(p + L::AX, w.aux + sh * AX_N, AX_N * 4, bar);
-        bulk_load(p + L::M, w.mats + sh * MATS, SUM ? MATS / 2 : MATS, bar);
+        bulk_load(p + L::M, w.mats + sh * mats_bytes(AB16), SUM ? MATS / 2 : MATS, bar);
         for (int i = 0; i < NP && !SUM; ++i) tma_load_3d(p + L::KQ + (2 * i + 1) * PANEL, &tmq, bar, 64 * i, h, row);
         if (BWD) {
           tma_load_3d(p + L::DO, &tmo, bar, v0, hv, row);
@@ -148,6 +156,7 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
     // ------------------------------------------------------------------ MMA issuer
     if (lane == 0) {
       const uint32_t id64 = idesc_f16(128, 64, AB16, 0, 0), id128 = idesc_f16(128, 128, AB16, 0, 0);
+      const uint32_t ib64 = idesc_f16(128, 64, 1, 0, 0), ib128 = idesc_f16(128, 128, 1, 0, 0);  // T and P beta are bfloat16
       const uint32_t id_d = idesc_f16(128, KD, AB16, 0, 1), id_v = idesc_f16(128, 128, AB16, 1, 0);
       for (int c = 0; c < nch; ++c) {
         const int s = c & 1, ph = c & 1;
@@ -165,18 +174,18 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
             umma_ts(tb + T_X, tb + (x ? T_SL : T_SH) + 8 * ks,
                     sdesc(p + L::KQ + (ks >> 2) * 2 * PANEL + (ks & 3) * 32, 16, 1024), SUM ? id64 : id128, x + ks > 0);
         umma_commit(&S_.x_full);
-        // E^T = V^T T^T, then + (-Gam X)^T T^T; the hi and lo halves are added on reading
+        // E^T = V^T T^T, then + (-Gam X)^T T^T (float16: R^T T^T); the hi and lo halves are added on reading
         if (!SUM && c > 0 && !spin_wait(&S_.o2_free, (c - 1) & 1, ab, err, 0x20)) break;
         tc_fence_after();
 #pragma unroll
-        for (int ks = 0; ks < 4 && !map; ++ks)
+        for (int ks = 0; ks < 4 && AB16 && !map; ++ks)
           umma(tb + T_D, sdesc(p + L::V + ks * 2048, PANEL, 1024), sdesc(T + ks * 32, 16, 1024), id_v, ks > 0);
         if (!spin_wait(&S_.r_ready, ph, ab, err, 0x40)) break;
         tc_fence_after();
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RH + 8 * ks, sdesc(T + ks * 32, 16, 1024), id128, !map || ks > 0);
+        for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RH + 8 * ks, sdesc(T + ks * 32, 16, 1024), ib128, (AB16 && !map) || ks > 0);
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RL + 8 * ks, sdesc(T + ks * 32, 16, 1024), id64, 1);
+        for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RL + 8 * ks, sdesc(T + ks * 32, 16, 1024), ib64, 1);
         umma_commit(&S_.u_full);
         // dS^T = (w beta E)^T K over X | Y, then E^T (P beta)^T over E
         if (!SUM && !spin_wait(&S_.o1_read, ph, ab, err, 0x200)) break;
@@ -190,9 +199,9 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
         umma_commit(&S_.d_full);
         if (!SUM) {
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RH + 8 * ks, sdesc(P + ks * 32, 16, 1024), id128, ks > 0);
+          for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RH + 8 * ks, sdesc(P + ks * 32, 16, 1024), ib128, ks > 0);
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RL + 8 * ks, sdesc(P + ks * 32, 16, 1024), id64, 1);
+          for (int ks = 0; ks < 4; ++ks) umma_ts(tb + T_D, tb + T_RL + 8 * ks, sdesc(P + ks * 32, 16, 1024), ib64, 1);
           umma_commit(&S_.o_full);
         }
         umma_commit(&S_.empty[s]);
@@ -217,13 +226,34 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
       const int k = KH * hh + i;
       S[i] = (first && vin && k < a.K) ? first[(int64_t)k * a.V + v0 + vl] : map && k == vl && vin ? 1.f : 0.f;
     }
-    // S as the operand of the next chunk; for the backward its hi part also goes to `tile` (two panels of
+    const int cw = warp - G::CHAIN;
+    [[maybe_unused]] float* fx = factors_of(a, w) + ((int64_t)vt * gdr_slots(a, C) * a.HV + sh0) * FX_N;  // of the first chunk
+    float uS = 1.f, bS = 0.f;  // float16: what undoes the factor of S, and a bound on S
+    // S as the operand of chunk c; for the backward its hi part also goes to `tile` (two panels of
     // 128 rows), or straight to the workspace for the first chunk
-    auto put_state = [&](uint32_t tile) {
+    auto put_state = [&](uint32_t tile, int c) {
+      Pow2 f{1.f, 1.f};
+      if constexpr (!AB16) {
+        if (c % EXACT == 0) bS = warps_max<2, G::CHAIN_WARPS>(abs_max<KH>(S), S_.top[0], cw);
+        f = pow2_of(bS);
+        uS = f.u;
+        if (threadIdx.x == 32 * G::CHAIN) {
+          S_.undo[c & 1] = f.u;
+          if (BWD) fx[(int64_t)c * a.HV * FX_N + FX_S] = f.u;
+        }
+      }
 #pragma unroll
       for (int i = 0; i < KH; i += 16) {
         uint32_t hi[8], lo[8];
-        split<AB16, 8>(S + i, hi, lo);
+        if constexpr (AB16) {
+          split<AB16, 8>(S + i, hi, lo);
+        } else {
+          float x[16];
+          const float ss[2] = {f.s, f.s};
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) mul2f(x + j, S + i + j, ss);
+          split<AB16, 8>(x, hi, lo);
+        }
         tmem_st8(tl + T_SH + hh * (KH / 2) + i / 2, hi);
         tmem_st8(tl + T_SL + hh * (KH / 2) + i / 2, lo);
         if (BWD) {
@@ -244,56 +274,100 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
       tc_fence_before();
       warp_arrive(&S_.s_ready);
     };
-    if (nch > 0) put_state(0);
+    const int i0 = CT * hh;
+    // E of tokens i0 + i .. + 15, its two halves added
+    auto load_e = [&](int i, float* x) {
+      tmem_ld16(tl + T_D + i0 + i, x);
+#pragma unroll
+      for (int k = 0; k < 16; k += NY) {
+        float y[NY];
+        if (NY == 16) tmem_ld16(tl + T_D + 64 + i0 + i + k, y);
+        else tmem_ld8(tl + T_D + 64 + i0 + i + k, y);
+#pragma unroll
+        for (int j = 0; j < NY; j += 2) add2f(x + k + j, x + k + j, y + j);
+      }
+    };
+    // float16, backward: E of this thread's 16 tokens from the operand, hi + lo, which stays until the next chunk's R
+    [[maybe_unused]] auto read_e = [&](float* x) {
+      static_assert(!BWD || CT == 16, "one piece");
+      float h[8], l[8];
+      tmem_ld8(tl + T_RH + i0 / 2, h);
+      tmem_ld8(tl + T_RL + i0 / 2, l);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 u = unpack2<1>(__float_as_uint(h[j])), v = unpack2<1>(__float_as_uint(l[j]));
+        x[2 * j] = u.x + v.x;
+        x[2 * j + 1] = u.y + v.y;
+      }
+    };
+    // E, transposed, to the staging panel (hi) and over the V tile, whose product is done (lo)
+    auto stage_e = [&](uint32_t p, int i, const uint32_t* hi, const uint32_t* lo) {
+      sts128(sb + L::OUT + sw128(vl, (i0 + i) >> 3), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+      sts128(sb + L::OUT + sw128(vl, ((i0 + i) >> 3) + 1), make_uint4(hi[4], hi[5], hi[6], hi[7]));
+      sts128(p + L::V + sw128(vl, (i0 + i) >> 3), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+      sts128(p + L::V + sw128(vl, ((i0 + i) >> 3) + 1), make_uint4(lo[4], lo[5], lo[6], lo[7]));
+    };
+    if (nch > 0) put_state(0, 0);
     for (int c = 0; c < nch; ++c) {
       const int s = c & 1, ph = c & 1;
       const uint32_t p = sb + s * L::STAGE;
       const float* ax = reinterpret_cast<const float*>(sm + s * L::STAGE + L::AX);
-      const int i0 = CT * hh;
       pipe_wait(&S_.full[s], (c >> 1) & 1, ab, err, 0x400);
+      [[maybe_unused]] uint32_t v[AB16 ? 1 : CT / 2];  // float16: this thread's part of V, asked for before X is there
+      if constexpr (!AB16) {
+        const int valid = map ? 0 : min(C, sq.len - c * C);
+        const Column V(p + L::V, vl);
+#pragma unroll
+        for (int i = 0; i < CT; i += 2) {
+          const uint32_t lo = lds16_early(V.at(i0 + i)), hi = lds16_early(V.at(i0 + i + 1));
+          v[i / 2] = (i0 + i < valid ? lo : 0) | (i0 + i + 1 < valid ? hi << 16 : 0);  // behind the document: anything
+        }
+      }
       pipe_wait(&S_.x_full, ph, ab, err, 0x800);
       tc_fence_after();
+      if constexpr (AB16) {
 #pragma unroll
-      for (int i = 0; i < CT; i += 16) {
-        float x[16];
-        tmem_ld16(tl + T_X + i0 + i, x);
+        for (int i = 0; i < CT; i += 16) {
+          float x[16];
+          tmem_ld16(tl + T_X + i0 + i, x);
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(ax + AX_G + i0 + i + j);
-          const float bb[4] = {-b.x, -b.y, -b.z, -b.w};
-          mul2f(x + j, x + j, bb);
-          mul2f(x + j + 2, x + j + 2, bb + 2);
+          for (int j = 0; j < 16; j += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(ax + AX_G + i0 + i + j);
+            const float bb[4] = {-b.x, -b.y, -b.z, -b.w};
+            mul2f(x + j, x + j, bb);
+            mul2f(x + j + 2, x + j + 2, bb + 2);
+          }
+          st_split16<AB16>(tl + T_RH + (i0 + i) / 2, tl + T_RL + (i0 + i) / 2, x);
         }
-        st_split16<AB16>(tl + T_RH + (i0 + i) / 2, tl + T_RL + (i0 + i) / 2, x);
+      } else {
+#pragma unroll
+        for (int i = 0; i < CT; i += 16) {
+          float x[16];
+          tmem_ld16(tl + T_X + i0 + i, x);
+#pragma unroll
+          for (int j = 0; j < 16; j += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(ax + AX_G + i0 + i + j);
+            const float2 v0 = unpack2<AB16>(v[(i + j) / 2]), v1 = unpack2<AB16>(v[(i + j) / 2 + 1]);
+            x[j] = fmaf(-b.x * uS, x[j], v0.x);
+            x[j + 1] = fmaf(-b.y * uS, x[j + 1], v0.y);
+            x[j + 2] = fmaf(-b.z * uS, x[j + 2], v1.x);
+            x[j + 3] = fmaf(-b.w * uS, x[j + 3], v1.y);
+          }
+          st_split16<1>(tl + T_RH + (i0 + i) / 2, tl + T_RL + (i0 + i) / 2, x);
+        }
       }
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.r_ready);
+      if (!AB16 && BWD && c > 0 && threadIdx.x == 32 * G::CHAIN) {
+        bulk_wait_read();  // the chunk before is stored: its stage, and the panel of E, may be written again
+        mbar_arrive(&S_.empty[s ^ 1]);
+      }
       pipe_wait(&S_.u_full, ph, ab, err, 0x1000);
       tc_fence_after();
       const float gam[2] = {ax[AX_GC], ax[AX_GC]};
-#pragma unroll
-      for (int i = 0; i < CT; i += 16) {
-        float x[16];
-        tmem_ld16(tl + T_D + i0 + i, x);
-#pragma unroll
-        for (int k = 0; k < 16; k += NY) {
-          float y[NY];
-          if (NY == 16) tmem_ld16(tl + T_D + 64 + i0 + i + k, y);
-          else tmem_ld8(tl + T_D + 64 + i0 + i + k, y);
-#pragma unroll
-          for (int j = 0; j < NY; j += 2) add2f(x + k + j, x + k + j, y + j);
-        }
-        uint32_t hi[8], lo[8];
-        split<AB16, 8>(x, hi, lo);
-        tmem_st8(tl + T_RH + (i0 + i) / 2, hi);
-        tmem_st8(tl + T_RL + (i0 + i) / 2, lo);
-        if (BWD) {  // E, transposed, to the staging panel (hi) and over the V tile, whose product is done (lo)
-          sts128(sb + L::OUT + sw128(vl, (i0 + i) >> 3), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-          sts128(sb + L::OUT + sw128(vl, ((i0 + i) >> 3) + 1), make_uint4(hi[4], hi[5], hi[6], hi[7]));
-          sts128(p + L::V + sw128(vl, (i0 + i) >> 3), make_uint4(lo[0], lo[1], lo[2], lo[3]));
-          sts128(p + L::V + sw128(vl, ((i0 + i) >> 3) + 1), make_uint4(lo[4], lo[5], lo[6], lo[7]));
-        }
+      [[maybe_unused]] float uW[2] = {1.f, 1.f};        // float16: what undoes the factor of w beta E
+      auto weigh = [&](int i, float* x) {
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
           const float4 b = *reinterpret_cast<const float4*>(ax + AX_WB + i0 + i + j);
@@ -301,13 +375,56 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
           mul2f(x + j, x + j, bb);
           mul2f(x + j + 2, x + j + 2, bb + 2);
         }
-        st_split16<AB16>(tl + T_WH + (i0 + i) / 2, tl + T_WL + (i0 + i) / 2, x);
+      };
+      if constexpr (AB16) {
+#pragma unroll
+        for (int i = 0; i < CT; i += 16) {
+          float x[16];
+          load_e(i, x);
+          uint32_t hi[8], lo[8];
+          split<AB16, 8>(x, hi, lo);
+          tmem_st8(tl + T_RH + (i0 + i) / 2, hi);
+          tmem_st8(tl + T_RL + (i0 + i) / 2, lo);
+          if (BWD) stage_e(p, i, hi, lo);
+          weigh(i, x);
+          st_split16<AB16>(tl + T_WH + (i0 + i) / 2, tl + T_WL + (i0 + i) / 2, x);
+        }
+      } else {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < CT; i += 16) {
+          float x[16];
+          load_e(i, x);
+          st_split16<1>(tl + T_RH + (i0 + i) / 2, tl + T_RL + (i0 + i) / 2, x);
+          weigh(i, x);
+          m = fmaxf(m, abs_max<16>(x));
+        }
+        m = warps_max<2, G::CHAIN_WARPS>(m, S_.top[1], cw);
+        const Pow2 f = pow2_of(m);
+        const float ss[2] = {f.s, f.s};
+        uW[0] = uW[1] = f.u;
+        bS = fmaf(64.f * ax[AX_KN], m, gam[0] * bS);
+#pragma unroll
+        for (int i = 0; i < CT; i += 16) {  // E once more rather than kept: registers
+          float x[16];
+          load_e(i, x);
+          weigh(i, x);
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) mul2f(x + j, x + j, ss);
+          st_split16<AB16>(tl + T_WH + (i0 + i) / 2, tl + T_WL + (i0 + i) / 2, x);
+        }
       }
       tmem_st_wait();
       tc_fence_before();
       warp_arrive(&S_.u_ready);
-      if (!BWD || warp != G::CHAIN) warp_arrive(&S_.empty[s]);
-      if (BWD) {
+      if constexpr (!AB16 && BWD) {
+        float e[16];
+        read_e(e);
+        token_max_put<CT>(e, S_.etop, i0, quad, lane);  // got below
+      }
+      constexpr bool LATE = !AB16 && BWD;  // E is staged behind S, with its tokens' factors
+      if (!LATE && (!BWD || warp != G::CHAIN)) warp_arrive(&S_.empty[s]);
+      if (BWD && !LATE) {
         fence_async_smem();
         bar_sync<2, G::CHAIN_THREADS>();
         if (threadIdx.x == 32 * G::CHAIN) {
@@ -321,11 +438,38 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
       for (int i = 0; i < KH; i += 16) {
         float x[16];
         tmem_ld16(tl + T_X + KH * hh + i, x);
+        if (!AB16) {
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) mul2f(x + j, x + j, uW);
+        }
 #pragma unroll
         for (int j = 0; j < 16; j += 2) fma2(S + i + j, gam, S + i + j, x + j);
       }
-      if (c + 1 < nch) put_state(p + L::KQ);  // every product with the K and Q rows is done: their space is the staging
-      if (BWD) {
+      if (c + 1 < nch) put_state(p + L::KQ, c + 1);  // every product with the K and Q rows is done: their space is the staging
+      if constexpr (LATE) {
+        bar_sync_quad<4, 128>(hh);  // the four warps with these tokens
+        const Pow2 f = pow2_of(token_max_get(S_.etop, i0 + (lane & (CT - 1))));
+        if (quad == 0 && lane < CT) fx[(int64_t)c * a.HV * FX_N + FX_E + i0 + lane] = f.u;
+        float e[16];
+        read_e(e);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) e[j] *= __shfl_sync(0xffffffffu, f.s, j);
+        uint32_t hi[8], lo[8];
+        split<AB16, 8>(e, hi, lo);
+        stage_e(p, 0, hi, lo);
+        fence_async_smem();
+        bar_sync<2, G::CHAIN_THREADS>();
+        if (threadIdx.x == 32 * G::CHAIN) {
+          store_panel(&tme, sm + L::OUT, 0, v0, a.V, sh0 + (int64_t)c * a.HV);
+          store_panel(&tme, sm + s * L::STAGE + L::V, C, v0, a.V, sh0 + (int64_t)c * a.HV);
+          if (c + 1 < nch)
+            for (int i = 0; i < NP; ++i)
+              if (64 * i < a.K)
+                store_panel(&tms, sm + s * L::STAGE + L::KQ + 2 * i * PANEL, 64 * i, v0, a.V, sh0 + (int64_t)(c + 1) * a.HV);
+        }
+        if (warp != G::CHAIN) warp_arrive(&S_.empty[s]);
+      }
+      if (BWD && !LATE) {
         fence_async_smem();
         bar_sync<2, G::CHAIN_THREADS>();
         if (threadIdx.x == 32 * G::CHAIN) {
@@ -380,14 +524,17 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
 #pragma unroll
       for (int i = 0; i < OT; i += 32) tmem_ld32(tl + T_X + 64 + j0 + i, y + i);
       tc_fence_before();
+      // the factor was left before S was ready, the phase of which lasts until o1_read of this chunk
+      if (!AB16) pipe_wait(&S_.s_ready, ph, ab, err, 0x8000);
+      const float uY = AB16 ? 1.f : S_.undo[c & 1];
       warp_arrive(&S_.o1_read);
 #pragma unroll
       for (int i = 0; i < OT; i += 4) {
         const float4 b = *reinterpret_cast<const float4*>(ax + AX_SG + j0 + i);
-        y[i] *= b.x;
-        y[i + 1] *= b.y;
-        y[i + 2] *= b.z;
-        y[i + 3] *= b.w;
+        y[i] *= AB16 ? b.x : b.x * uY;
+        y[i + 1] *= AB16 ? b.y : b.y * uY;
+        y[i + 2] *= AB16 ? b.z : b.z * uY;
+        y[i + 3] *= AB16 ? b.w : b.w * uY;
       }
       pipe_wait(&S_.o_full, ph, ab, err, 0x10000);
       tc_fence_after();
@@ -425,9 +572,18 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
         }
       } else {
         const Column D(p + L::DO, vl);
+        [[maybe_unused]] float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < OT; ++i) y[i] = j0 + i < valid ? y[i] * h2f<AB16>(lds16(D.at(j0 + i))) : 0.f;
+        for (int i = 0; i < OT; ++i) {
+          const float d = j0 + i < valid ? h2f<AB16>(lds16(D.at(j0 + i))) : 0.f;
+          if (!AB16) top = fmaxf(top, fabsf(d));
+          y[i] = j0 + i < valid ? y[i] * d : 0.f;
+        }
         warp_arrive(&S_.empty[s]);
+        if (!AB16) {
+          top = warp_max(top);
+          if (lane == 0) S_.dtop[warp] = top;
+        }
         lane_sums<OT>(y, lane);
 #pragma unroll
         for (int i = 0; i < OT / 32; ++i) S_.red[quad][j0 + lane * (OT / 32) + i] = y[i];
@@ -436,6 +592,11 @@ __global__ void __launch_bounds__(Warps<BWD>::THREADS, 1)
           const int i = threadIdx.x;
           w.dotO[((int64_t)vt * slots * a.HV + sh0 + (int64_t)c * a.HV) * C + i] =
               S_.red[0][i] + S_.red[1][i] + S_.red[2][i] + S_.red[3][i];
+          if (!AB16 && i == 0) {
+#pragma unroll
+            for (int o = 1; o < G::OUT_WARPS; ++o) top = fmaxf(top, S_.dtop[o]);
+            factors_of(a, w)[((int64_t)vt * slots * a.HV + sh0 + (int64_t)c * a.HV) * FX_N + FX_DO] = top;
+          }
         }
         bar_sync<1, G::OUT_THREADS>();
       }

@@ -336,6 +336,18 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   return r;
 }
 
+// the larger of two pairs, each by itself
+__device__ __forceinline__ uint32_t max2_f16(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max2_bf16(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // Named barriers with the id and thread count as immediates.  A bar.sync whose barrier id came from
 // a register (computed from the warp index) did not keep its id on sm_100a: warps meant for
 // different barriers completed one another's (measured with one CTA, two warps per id, one of them

@@ -130,7 +130,9 @@ def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, output
 
     16-bit inputs with K a multiple of 8 up to 128 and V a multiple of 8 run on the tensor cores, where the
     state and its gradient keep fp32 accuracy (about 4e-6) and dq, dk and dbeta that of the 16-bit type;
-    everything else, fp32 inputs among it, runs in fp32 on the CUDA cores.
+    everything else, fp32 inputs among it, runs in fp32 on the CUDA cores.  k and v are taken in q's dtype.  States
+    and their gradients may have any size that fp32 holds, with float16 inputs too; what is returned in float16
+    has that type's range.
     """
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if wants_grad(q, k, v, g, beta, initial_state):
