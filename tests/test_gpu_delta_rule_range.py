@@ -145,3 +145,30 @@ def test_step_and_rule_agree_on_a_large_state():
     b, T = ccq_b200.gated_delta_step(q, k, v, g, beta, h0, scale=1e-4)
     assert torch.isfinite(a).all() and (a.double() - b.double()).norm() <= 1e-3 * b.double().norm()
     assert (S - T).norm() <= 3e-5 * T.norm()
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), 6e4])
+def test_factors_stay_in_their_document(bad):
+    """A document of NaN, infinities or values near float16's end between two others: theirs are the same, bit for bit."""
+    import ccq_b200
+    lens, r = [70, 33, 90], lambda *s: torch.randn(*s, device='cuda')
+    cu = torch.tensor([0] + lens, device='cuda').cumsum(0)
+    T = sum(lens)
+    x = [torch.nn.functional.normalize(r(1, T, 2, 128), dim=-1).half() for _ in range(2)]
+    x += [r(1, T, 4, 256).half(), -torch.rand(1, T, 4, device='cuda'), r(1, T, 4).sigmoid()]
+    d_o = r(1, T, 4, 256).half()
+
+    def run():
+        y = [t.clone().requires_grad_(True) for t in x]
+        o, S = ccq_b200.gated_delta_rule(*y, output_final_state=True, cu_seqlens=cu)
+        return [o, *torch.autograd.grad(o, y, d_o)], S
+
+    clean, S0 = run()
+    for t in x[:3] + [d_o]:
+        t[:, 70:103] = bad
+    dirty, S1 = run()
+    again, _ = run()
+    for a, b, c in zip(clean, dirty, again):
+        assert torch.equal(a[:, :70], b[:, :70]) and torch.equal(a[:, 103:], b[:, 103:])
+        assert torch.equal(b[:, :70], c[:, :70]) and torch.equal(b[:, 103:], c[:, 103:])
+    assert torch.equal(S0[[0, 2]], S1[[0, 2]])
