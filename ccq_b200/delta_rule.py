@@ -118,7 +118,7 @@ class GatedDeltaRule(torch.autograd.Function):
 
 
 def gated_delta_rule(q, k, v, g, beta, *, scale=None, initial_state=None, output_final_state=False, cu_seqlens=None):
-    """Gated delta rule over whole sequences, with gradients.
+    """Gated delta rule over whole sequences, with gradients (of first order, in reverse mode; others raise).
 
     q, k: [B, T, H, K]; v: [B, T, HV, V] with HV a multiple of H (value head h reads key head
     h // (HV // H)); g: [B, T, HV] log decay; beta: [B, T, HV] write strength; scale defaults to
@@ -168,7 +168,7 @@ def gated_delta_step(q, k, v, g, beta, state=None, *, scale=None, cu_seqlens=Non
     cu, N = _seqs(q.shape[0], cu_seqlens, q.shape[1])
     shape = (N, v.shape[2], q.shape[3], v.shape[3])
     _check_state(state, shape, inplace)
-    h0 = _state(state, shape)
+    h0 = state if inplace else _state(state, shape)  # in place it is as the kernel takes it
     out = state if inplace else torch.empty(shape, device=q.device, dtype=torch.float32)
     o = torch.empty_like(v, requires_grad=False)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)

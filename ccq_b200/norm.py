@@ -3,7 +3,7 @@
     h = x (+ residual);   n = (h - mean) / sqrt(var + eps)      (RMS: mean = 0, var = mean of h^2)
     y = n weight (+ bias);   gated: y = n weight gate sigmoid(gate)
 
-The sums are fp32, the outputs are rounded once.  Every call goes to the sm_100a kernels in
+The sums are fp32, the outputs are rounded once.  Gradients are of first order, in reverse mode; others raise.  Every call goes to the sm_100a kernels in
 ``libccq_b200.so``; there is no CPU or eager fallback.
 """
 from __future__ import annotations
