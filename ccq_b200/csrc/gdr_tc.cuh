@@ -19,8 +19,9 @@
 // Range.  bfloat16 has float's exponents; float16 ends at 65504 and its hi + lo loses bits below 2^-8, while states and
 // gradients are fp32 of any size.  For float16 inputs, therefore:
 //   * a product without an input (R T, E P beta, dE T) has bfloat16 operands;
-//   * an operand that meets an input has to be float16.  It is multiplied by a power of two that puts its largest value
-//     into [2^14, 2^15) (pow2_of; hi + lo then keeps 2^-22 of that value), and the product's fp32 sums by the inverse.
+//   * an operand that meets an input has to be float16.  It is multiplied by a power of two that puts its largest value,
+//     or a bound on it, into [2^14, 2^15) (pow2_of; hi + lo then keeps 2^-22 of every value down to 2^-22 of the largest),
+//     and the product's fp32 sums by the inverse.
 //     "Its" means of a chunk and 128 columns of V, for the stored E and dV also of a token, for N and W of a chunk.
 // Operands that share an accumulator would have to share the factor, so float16 forms R = V - Gam K S0 before the
 // product with T, reads the two products of dS one after the other, and takes the gradient kernel's V in tiles of 128
